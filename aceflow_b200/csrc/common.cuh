@@ -78,6 +78,21 @@ inline int fail(int code, const char *fmt, ...) {
 // Validates the context and makes its device current.
 int enter(af_ctx *ctx, const char *fn);
 
+// Puts the caller's current device back when an entry point that made its
+// context's device current returns.
+struct DeviceScope {
+  int prev = -1;
+  DeviceScope() {
+    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+  }
+  ~DeviceScope() {
+    int cur = -1;
+    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
+  }
+  DeviceScope(const DeviceScope &) = delete;
+  DeviceScope &operator=(const DeviceScope &) = delete;
+};
+
 // Grows the context workspace to at least `bytes` (256-byte aligned base).
 int workspace(af_ctx *ctx, size_t bytes, void **out, const char *fn);
 

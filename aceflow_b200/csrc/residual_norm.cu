@@ -1,0 +1,573 @@
+// The seam between two blocks of a decoder layer in one pass: the norm behind
+// a block, its gate and residual scale, the residual add, and the norm in
+// front of the next block.  For a residual row x, a block's output h, gate
+// logits g, weights w1, s, w2 and a factor alpha,
+//     n = h r1 w1,  r1 = 1 / sqrt(mean(h^2) + eps)      (n = h without w1)
+//     z = alpha x + s swish(g) n                        (s, swish(g): 1 without)
+//     y = z r2 w2,  r2 = 1 / sqrt(mean(z^2) + eps)      (no y without w2)
+// The reference runs the add and the norm of its pre-norm layer apart
+// (aceflow-core/src/cpu/mod.rs:672-700, norm.rs:6-59) and has no norm behind a
+// block; DeepNet's alpha (Wang et al. 2022) and a learnt scale per channel
+// (Touvron et al. 2021) are the usual residual scales.
+//
+// Backward, from dz and dy: with zh = z r2, hh = h r1, t = dy w2,
+//     Z  = dz + r2 (t - zh mean(t zh))                  dx = alpha Z
+//     dw2 = sum dy zh,  ds = sum Z swish(g) n,  dg = Z s n swish'(g)
+//     N  = Z s swish(g),  dw1 = sum N hh
+//     dh = r1 (N w1 - hh mean(N w1 hh))
+// mean(N w1 hh) needs Z, which needs the other mean.  Both come from one
+// reduction of three sums: with q = s swish(g) w1 hh,
+//     sum N w1 hh = sum (dz + r2 t) q - r2 mean(t zh) sum zh q.
+// z is formed again in fp32 from x, h and g (reading x costs what reading z
+// would), so the rounding of the stored z does not enter the gradients.
+//
+// Bound: HBM, every row of every tensor moved once.  A row is held in
+// registers by one group of threads; sums, statistics and the row itself are
+// fp32, and each output is rounded once.  The column sums of the weights'
+// gradients stay in registers while a block walks its rows, go out as one
+// partial row per block and are added in a fixed order by a second kernel: no
+// atomics, the same bits every run.
+#include "common.cuh"
+
+namespace {
+
+struct SeamParams {
+  const void *x, *h, *g;  // g NULL: no gate (its type is h's)
+  int64_t ldx, ldh, ldg;
+  int x16, h16, y16;  // bf16 flags
+  const float *w1, *s, *w2;
+  float alpha, eps, inv_d;
+  int rows, d;
+  void *z, *y;     // contiguous rows; y NULL without w2
+  float *stats;    // [2][rows]: r1, r2 (written by the forward when not NULL, read by the backward)
+  const void *dz, *dy;  // either may be NULL (zero)
+  int64_t lddz, lddy;
+  void *dx, *dh, *dg;
+  float *part;  // [3][parts][d]: dw1, ds, dw2
+  int parts;
+};
+
+// VEC consecutive values of a row as they lie in memory: loads are issued
+// without waiting, whatever the type; the conversion comes with the first use.
+template <int VEC>
+struct Raw;
+template <>
+struct Raw<8> {
+  uint4 a, b;
+  __device__ __forceinline__ void load(const void *p, int64_t i, bool b16) {
+    const char *q = static_cast<const char *>(p) + i * (b16 ? 2 : 4);
+    a = __ldcs(reinterpret_cast<const uint4 *>(q));
+    if (!b16) b = __ldcs(reinterpret_cast<const uint4 *>(q) + 1);
+  }
+  __device__ __forceinline__ void get(float (&v)[8], bool b16) const {
+    if (b16) {
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    } else {
+      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+    }
+  }
+};
+template <>
+struct Raw<1> {
+  uint32_t a;
+  __device__ __forceinline__ void load(const void *p, int64_t i, bool b16) {
+    if (b16)
+      a = (uint32_t)__ldcs(static_cast<const unsigned short *>(p) + i) << 16;
+    else
+      a = __ldcs(static_cast<const unsigned int *>(p) + i);
+  }
+  __device__ __forceinline__ void get(float (&v)[1], bool) const { v[0] = __uint_as_float(a); }
+};
+
+template <int VEC>
+__device__ __forceinline__ void put(void *p, int64_t i, const float (&v)[VEC], bool b16);
+template <>
+__device__ __forceinline__ void put<8>(void *p, int64_t i, const float (&v)[8], bool b16) {
+  if (b16) {
+    uint4 r;
+    __nv_bfloat162 *e = reinterpret_cast<__nv_bfloat162 *>(&r);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) e[k] = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+    *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p) + i) = r;
+  } else {
+    float4 *q = reinterpret_cast<float4 *>(static_cast<float *>(p) + i);
+    q[0] = make_float4(v[0], v[1], v[2], v[3]);
+    q[1] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+}
+template <>
+__device__ __forceinline__ void put<1>(void *p, int64_t i, const float (&v)[1], bool b16) {
+  if (b16)
+    static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16(v[0]);
+  else
+    static_cast<float *>(p)[i] = v[0];
+}
+
+template <int VEC>
+__device__ __forceinline__ void weights(const float *w, int col, float (&v)[VEC]) {
+  if constexpr (VEC == 8) {
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(w + col)),
+                 b = __ldg(reinterpret_cast<const float4 *>(w + col) + 1);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+    v[0] = __ldg(w + col);
+  }
+}
+
+__device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
+// swish(g) = g sigmoid(g) and its derivative, with their limit 0 at -inf.
+__device__ __forceinline__ float swish(float g) {
+  const float sg = sigmoid(g);
+  return sg > 0.f || g != g ? g * sg : 0.f;
+}
+__device__ __forceinline__ float swish_slope(float g) {
+  const float sg = sigmoid(g);
+  return sg > 0.f || g != g ? sg * (1.f + g * (1.f - sg)) : 0.f;
+}
+
+// Sums of n values over the row's threads: a warp (one_warp) or the block.
+// `red` holds 2 x 3 x 16 floats; `flip` alternates its halves, so one barrier
+// per sum is enough.
+template <int NV>
+__device__ __forceinline__ void row_sum(float (&v)[NV], bool one_warp, float *red, int &flip) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) v[i] = warp_sum(v[i]);
+  if (one_warp) return;
+  float *r = red + flip * 48;
+  flip ^= 1;
+  const int nw = blockDim.x >> 5, w = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) r[i * 16 + w] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float t = 0.f;
+    for (int k = 0; k < nw; ++k) t += r[i * 16 + k];
+    v[i] = t;
+  }
+}
+
+// Threads of a row: a warp (blockDim.y rows per block) or the whole block
+// (blockDim.y == 1).  Thread k of a row holds values (c * n + k) * VEC ..,
+// c < K, n the row's threads.
+template <int VEC, int K>
+__global__ void __launch_bounds__(512) seam_forward_kernel(SeamParams p) {
+  __shared__ float red[96];
+  int flip = 0;
+  const int n = blockDim.x;
+  const bool one_warp = n == 32;
+  const int row = blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= p.rows) return;  // whole warps where a warp has a row; never where the block has one
+  Raw<VEC> hr[K], gr[K], xr[K];
+#pragma unroll
+  for (int c = 0; c < K; ++c) {
+    const int col = (c * n + (int)threadIdx.x) * VEC;
+    if (col < p.d) {
+      hr[c].load(p.h, row * p.ldh + col, p.h16);
+      if (p.g) gr[c].load(p.g, row * p.ldg + col, p.h16);
+      xr[c].load(p.x, row * p.ldx + col, p.x16);
+    }
+  }
+  float z[K][VEC];
+  float r1 = 1.f;
+  if (p.w1) {
+    float sq[1] = {0.f};
+#pragma unroll
+    for (int c = 0; c < K; ++c) {
+      const int col = (c * n + (int)threadIdx.x) * VEC;
+      if (col < p.d) {
+        float v[VEC];
+        hr[c].get(v, p.h16);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sq[0] = fmaf(v[i], v[i], sq[0]);
+      }
+    }
+    row_sum(sq, one_warp, red, flip);
+    r1 = 1.0f / sqrtf(sq[0] * p.inv_d + p.eps);
+  }
+  float sz[1] = {0.f};
+#pragma unroll
+  for (int c = 0; c < K; ++c) {
+    const int col = (c * n + (int)threadIdx.x) * VEC;
+    if (col < p.d) {
+      float m[VEC], v[VEC];
+      hr[c].get(m, p.h16);
+      if (p.w1) {
+        weights<VEC>(p.w1, col, v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) m[i] = m[i] * r1 * v[i];
+      }
+      if (p.g) {
+        gr[c].get(v, p.h16);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) m[i] *= swish(v[i]);
+      }
+      if (p.s) {
+        weights<VEC>(p.s, col, v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) m[i] *= v[i];
+      }
+      xr[c].get(v, p.x16);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        z[c][i] = fmaf(p.alpha, v[i], m[i]);
+        sz[0] = fmaf(z[c][i], z[c][i], sz[0]);
+      }
+      put<VEC>(p.z, (int64_t)row * p.d + col, z[c], p.x16);
+    }
+  }
+  float r2 = 1.f;
+  if (p.w2) {
+    row_sum(sz, one_warp, red, flip);
+    r2 = 1.0f / sqrtf(sz[0] * p.inv_d + p.eps);
+#pragma unroll
+    for (int c = 0; c < K; ++c) {
+      const int col = (c * n + (int)threadIdx.x) * VEC;
+      if (col < p.d) {
+        float v[VEC];
+        weights<VEC>(p.w2, col, v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = z[c][i] * r2 * v[i];
+        put<VEC>(p.y, (int64_t)row * p.d + col, v, p.y16);
+      }
+    }
+  }
+  if (p.stats && threadIdx.x == 0) {
+    p.stats[row] = r1;
+    p.stats[p.rows + row] = r2;
+  }
+}
+
+template <int VEC, int K>
+__global__ void __launch_bounds__(512) seam_backward_kernel(SeamParams p) {
+  __shared__ float red[96];
+  int flip = 0;
+  const int n = blockDim.x;
+  const bool one_warp = n == 32;
+  float a1[K][VEC], as[K][VEC], a2[K][VEC];  // this thread's columns of dw1, ds, dw2
+#pragma unroll
+  for (int c = 0; c < K; ++c)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) a1[c][i] = as[c][i] = a2[c][i] = 0.f;
+  const int part = blockIdx.x * blockDim.y + threadIdx.y;  // also this row group's place among all
+  for (int row = part; row < p.rows; row += p.parts) {
+    Raw<VEC> hr[K], gr[K], xr[K], dzr[K], dyr[K];
+#pragma unroll
+    for (int c = 0; c < K; ++c) {
+      const int col = (c * n + (int)threadIdx.x) * VEC;
+      if (col < p.d) {
+        hr[c].load(p.h, row * p.ldh + col, p.h16);
+        if (p.g) gr[c].load(p.g, row * p.ldg + col, p.h16);
+        if (p.dz) dzr[c].load(p.dz, row * p.lddz + col, p.x16);
+        if (p.dy) {
+          dyr[c].load(p.dy, row * p.lddy + col, p.y16);
+          xr[c].load(p.x, row * p.ldx + col, p.x16);
+        }
+      }
+    }
+    const float r1 = p.w1 ? p.stats[row] : 1.f, r2 = p.w2 ? p.stats[p.rows + row] : 1.f;
+    // q = d z / d n * w1 * hh, t = dy w2, zh = z r2 and the three sums
+    float sum[3] = {0.f, 0.f, 0.f};  // t zh, (dz + r2 t) q, zh q
+    float zh[K][VEC], e[K][VEC];     // e = dz + r2 t
+#pragma unroll
+    for (int c = 0; c < K; ++c) {
+      const int col = (c * n + (int)threadIdx.x) * VEC;
+      if (col < p.d) {
+        float q[VEC], v[VEC];
+        hr[c].get(q, p.h16);
+        if (p.w1) {
+          weights<VEC>(p.w1, col, v);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) q[i] = q[i] * r1 * v[i];
+        }
+        if (p.g) {
+          gr[c].get(v, p.h16);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) q[i] *= swish(v[i]);
+        }
+        if (p.s) {
+          weights<VEC>(p.s, col, v);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) q[i] *= v[i];
+        }
+        if (p.dz) {
+          dzr[c].get(e[c], p.x16);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) e[c][i] = 0.f;
+        }
+        if (p.dy) {
+          float w[VEC], dy[VEC];
+          xr[c].get(v, p.x16);
+          weights<VEC>(p.w2, col, w);
+          dyr[c].get(dy, p.y16);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            zh[c][i] = fmaf(p.alpha, v[i], q[i]) * r2;
+            a2[c][i] = fmaf(dy[i], zh[c][i], a2[c][i]);
+            const float t = dy[i] * w[i];
+            sum[0] = fmaf(t, zh[c][i], sum[0]);
+            e[c][i] = fmaf(r2, t, e[c][i]);
+            sum[2] = fmaf(zh[c][i], q[i], sum[2]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[1] = fmaf(e[c][i], q[i], sum[1]);
+      }
+    }
+    if (p.w1 || p.dy) row_sum(sum, one_warp, red, flip);
+    const float m2 = p.dy ? r2 * (sum[0] * p.inv_d) : 0.f;  // r2 mean(t zh)
+    const float m1 = (sum[1] - m2 * sum[2]) * p.inv_d;       // mean(N w1 hh)
+#pragma unroll
+    for (int c = 0; c < K; ++c) {
+      const int col = (c * n + (int)threadIdx.x) * VEC;
+      if (col < p.d) {
+        const int64_t at = (int64_t)row * p.d + col;
+        float o[VEC], nn[VEC], v[VEC];
+        if (p.dy) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) e[c][i] = fmaf(-m2, zh[c][i], e[c][i]);  // Z
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[i] = p.alpha * e[c][i];
+        put<VEC>(p.dx, at, o, p.x16);
+        // n, hh
+        float hh[VEC], w1[VEC];
+        hr[c].get(hh, p.h16);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) w1[i] = 1.f;
+        if (p.w1) {
+          weights<VEC>(p.w1, col, w1);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) hh[i] *= r1;
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) nn[i] = hh[i] * w1[i];
+        float s[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[i] = 1.f;
+        if (p.s) weights<VEC>(p.s, col, s);
+        if (p.g) {
+          float gv[VEC];
+          gr[c].get(gv, p.h16);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float sw = swish(gv[i]);
+            as[c][i] = fmaf(e[c][i] * sw, nn[i], as[c][i]);
+            const float zs = e[c][i] * s[i];
+            o[i] = zs * nn[i] * swish_slope(gv[i]);
+            v[i] = zs * sw;
+          }
+          put<VEC>(p.dg, at, o, p.h16);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            as[c][i] = fmaf(e[c][i], nn[i], as[c][i]);
+            v[i] = e[c][i] * s[i];
+          }
+        }
+        if (p.w1) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            a1[c][i] = fmaf(v[i], hh[i], a1[c][i]);
+            v[i] = r1 * (v[i] * w1[i] - hh[i] * m1);
+          }
+        }
+        put<VEC>(p.dh, at, v, p.h16);
+      }
+    }
+  }
+  const int64_t plane = (int64_t)p.parts * p.d;
+#pragma unroll
+  for (int c = 0; c < K; ++c) {
+    const int col = (c * n + (int)threadIdx.x) * VEC;
+    if (col < p.d) {
+      const int64_t at = (int64_t)part * p.d + col;
+      if (p.w1) put<VEC>(p.part, at, a1[c], false);
+      if (p.s) put<VEC>(p.part, plane + at, as[c], false);
+      if (p.w2) put<VEC>(p.part, 2 * plane + at, a2[c], false);
+    }
+  }
+}
+
+// Column sums of up to three [parts][d] planes (blockIdx.y picks the plane):
+// 8 warps share a block of 32 columns, each adds every eighth part in order.
+__global__ void __launch_bounds__(256) seam_columns_kernel(const float *part, int parts, int d, float *o1, float *o2,
+                                                           float *o3) {
+  __shared__ float red[8][32];
+  float *out = blockIdx.y == 0 ? o1 : blockIdx.y == 1 ? o2 : o3;
+  if (!out) return;
+  const int col = blockIdx.x * 32 + threadIdx.x;
+  const float *src = part + (int64_t)blockIdx.y * parts * d + col;
+  float t = 0.f;
+  if (col < d)
+    for (int k = threadIdx.y; k < parts; k += 8) t += src[(int64_t)k * d];
+  red[threadIdx.y][threadIdx.x] = t;
+  __syncthreads();
+  if (threadIdx.y == 0 && col < d) {
+    for (int k = 1; k < 8; ++k) t += red[k][threadIdx.x];
+    out[col] = t;
+  }
+}
+
+constexpr int kMaxWidth = 16384;
+
+// Threads of a row and values per thread for rows of d values.
+struct Shape {
+  int vec, k, threads, rows_per_block;
+};
+Shape shape_of(int d, bool vec8, bool backward) {
+  if (vec8) {
+    const int ch = d / 8;  // 16-byte (bf16) or 32-byte (fp32) chunks
+    if (ch <= 32) return {8, 1, 32, 4};
+    if (backward) {  // five tensors and three column sums per value held: one chunk per thread while it lasts
+      if (ch <= 64) return {8, 1, 64, 1};
+      if (ch <= 128) return {8, 1, 128, 1};
+      if (ch <= 256) return {8, 1, 256, 1};
+      if (ch <= 512) return {8, 1, 512, 1};
+    }
+    if (ch <= 64) return {8, 2, 32, 4};
+    if (ch <= 128) return {8, 1, 128, 1};
+    if (ch <= 256) return {8, 2, 128, 1};
+    if (ch <= 512) return {8, 2, 256, 1};
+    if (ch <= 1024) return {8, 2, 512, 1};
+    return {8, 4, 512, 1};
+  }
+  if (d <= 128) return {1, 4, 32, 4};
+  if (d <= 512) return {1, 4, 128, 1};
+  if (d <= 1024) return {1, 8, 128, 1};
+  if (d <= 2048) return {1, 8, 256, 1};
+  if (d <= 4096) return {1, 8, 512, 1};
+  if (d <= 8192) return {1, 16, 512, 1};
+  return {1, 32, 512, 1};
+}
+
+template <typename F>
+void with_kernel(const Shape &s, F &&f) {
+  if (s.vec == 8) {
+    if (s.k == 1) return f(seam_forward_kernel<8, 1>, seam_backward_kernel<8, 1>);
+    if (s.k == 2) return f(seam_forward_kernel<8, 2>, seam_backward_kernel<8, 2>);
+    return f(seam_forward_kernel<8, 4>, seam_backward_kernel<8, 4>);
+  }
+  if (s.k == 4) return f(seam_forward_kernel<1, 4>, seam_backward_kernel<1, 4>);
+  if (s.k == 8) return f(seam_forward_kernel<1, 8>, seam_backward_kernel<1, 8>);
+  if (s.k == 16) return f(seam_forward_kernel<1, 16>, seam_backward_kernel<1, 16>);
+  return f(seam_forward_kernel<1, 32>, seam_backward_kernel<1, 32>);
+}
+
+// 16-byte accesses of 8 values need rows that start on 16 bytes (bf16; fp32
+// rows are then aligned too).
+bool rows_aligned(const void *p, int64_t ld, int is16) {
+  return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % (is16 ? 8 : 4) == 0);
+}
+
+// Row groups that share the rows of a backward: enough to fill the GPU, few
+// enough that their partial rows stay small beside the data.
+int parts_of(int num_sms, int rows, const Shape &s) {
+  const int per_sm = 512 / (s.threads * s.rows_per_block), blocks = num_sms * (per_sm < 1 ? 1 : per_sm);
+  const int need = (rows + s.rows_per_block - 1) / s.rows_per_block;
+  return (need < blocks ? need : blocks) * s.rows_per_block;
+}
+
+}  // namespace
+
+extern "C" {
+
+int af_residual_norm(af_ctx *ctx, const void *x, int64_t ldx, int x_bf16, const void *h, int64_t ldh, int h_bf16,
+                     const void *gate, int64_t ldg, const float *post_w, const float *scale, const float *pre_w,
+                     float alpha, float eps, int64_t rows, int d, void *z, void *y, int y_bf16, float *stats,
+                     af_stream_t stream) {
+  const char *fn = "af_residual_norm";
+  af::DeviceScope scope;
+  AF_ENTER(ctx, fn);
+  AF_REQUIRE(rows >= 0 && rows < (1ll << 31) && d > 0, "af_residual_norm", "bad sizes");
+  AF_REQUIRE(d <= kMaxWidth, "af_residual_norm", "rows of %d values: at most %d are supported", d, kMaxWidth);
+  if (rows == 0) return AF_OK;
+  AF_REQUIRE(x && h && z && (!pre_w || y), "af_residual_norm", "null argument");
+  SeamParams p = {};
+  p.x = x, p.h = h, p.g = gate, p.ldx = ldx, p.ldh = ldh, p.ldg = ldg;
+  p.x16 = x_bf16 != 0, p.h16 = h_bf16 != 0, p.y16 = y_bf16 != 0;
+  p.w1 = post_w, p.s = scale, p.w2 = pre_w, p.alpha = alpha, p.eps = eps, p.inv_d = 1.0f / (float)d;
+  p.rows = (int)rows, p.d = d, p.z = z, p.y = y, p.stats = stats;
+  const bool vec = d % 8 == 0 && rows_aligned(x, ldx, x_bf16) && rows_aligned(h, ldh, h_bf16) &&
+                   rows_aligned(gate, ldg, h_bf16) && rows_aligned(post_w, 8, 0) && rows_aligned(scale, 8, 0) &&
+                   rows_aligned(pre_w, 8, 0) && rows_aligned(z, d, x_bf16) && rows_aligned(y, d, y_bf16);
+  const Shape s = shape_of(d, vec, false);
+  with_kernel(s, [&](auto fwd, auto) {
+    fwd<<<(unsigned)((rows + s.rows_per_block - 1) / s.rows_per_block), dim3(s.threads, s.rows_per_block), 0,
+          af::stream_of(stream)>>>(p);
+  });
+  return af::launched(ctx, fn);
+}
+
+int af_residual_norm_scratch(af_ctx *ctx, int64_t rows, int d, int64_t *floats) {
+  const char *fn = "af_residual_norm_scratch";
+  af::DeviceScope scope;
+  AF_ENTER(ctx, fn);
+  AF_REQUIRE(floats && rows >= 0 && rows < (1ll << 31) && d > 0 && d <= kMaxWidth, "af_residual_norm_scratch",
+             "bad sizes");
+  const int a = parts_of(ctx->num_sms, (int)rows, shape_of(d, false, true));
+  const int b = d % 8 == 0 ? parts_of(ctx->num_sms, (int)rows, shape_of(d, true, true)) : 0;
+  *floats = 3ll * (a > b ? a : b) * d;
+  return AF_OK;
+}
+
+int af_residual_norm_backward(af_ctx *ctx, const void *dz, int64_t lddz, const void *dy, int64_t lddy, const void *x,
+                              int64_t ldx, int x_bf16, const void *h, int64_t ldh, int h_bf16, const void *gate,
+                              int64_t ldg, int y_bf16, const float *post_w, const float *scale, const float *pre_w,
+                              float alpha, int64_t rows, int d, const float *stats, void *dx, void *dh, void *dgate,
+                              float *dpost_w, float *dscale, float *dpre_w, float *scratch, int64_t scratch_floats,
+                              af_stream_t stream) {
+  const char *fn = "af_residual_norm_backward";
+  af::DeviceScope scope;
+  AF_ENTER(ctx, fn);
+  AF_REQUIRE(rows >= 0 && rows < (1ll << 31) && d > 0, "af_residual_norm_backward", "bad sizes");
+  AF_REQUIRE(d <= kMaxWidth, "af_residual_norm_backward", "rows of %d values: at most %d are supported", d, kMaxWidth);
+  AF_REQUIRE(!dy || pre_w, "af_residual_norm_backward", "dy without the norm that made y");
+  AF_REQUIRE((!post_w || dpost_w) && (!scale || dscale) && (!pre_w || dpre_w), "af_residual_norm_backward",
+             "a weight without room for its gradient");
+  cudaStream_t st = af::stream_of(stream);
+  if (rows == 0) {
+    float *w[3] = {post_w ? dpost_w : nullptr, scale ? dscale : nullptr, pre_w ? dpre_w : nullptr};
+    for (float *q : w)
+      if (q) AF_CUDA(cudaMemsetAsync(q, 0, (size_t)d * 4, st), fn);
+    return AF_OK;
+  }
+  AF_REQUIRE(x && h && dx && dh && (!gate || dgate) && (!(post_w || pre_w) || stats), "af_residual_norm_backward",
+             "null argument");
+  SeamParams p = {};
+  p.x = x, p.h = h, p.g = gate, p.ldx = ldx, p.ldh = ldh, p.ldg = ldg;
+  p.x16 = x_bf16 != 0, p.h16 = h_bf16 != 0, p.y16 = y_bf16 != 0;
+  p.w1 = post_w, p.s = scale, p.w2 = pre_w, p.alpha = alpha, p.inv_d = 1.0f / (float)d;
+  p.rows = (int)rows, p.d = d, p.stats = const_cast<float *>(stats);
+  p.dz = dz, p.dy = dy, p.lddz = lddz, p.lddy = lddy, p.dx = dx, p.dh = dh, p.dg = dgate, p.part = scratch;
+  const bool vec = d % 8 == 0 && rows_aligned(x, ldx, x_bf16) && rows_aligned(h, ldh, h_bf16) &&
+                   rows_aligned(gate, ldg, h_bf16) && rows_aligned(post_w, 8, 0) && rows_aligned(scale, 8, 0) &&
+                   rows_aligned(pre_w, 8, 0) && rows_aligned(dz, lddz, x_bf16) && rows_aligned(dy, lddy, y_bf16) &&
+                   rows_aligned(dx, d, x_bf16) && rows_aligned(dh, d, h_bf16) && rows_aligned(dgate, d, h_bf16) &&
+                   rows_aligned(scratch, 8, 0);
+  const Shape s = shape_of(d, vec, true);
+  p.parts = parts_of(ctx->num_sms, (int)rows, s);
+  const bool sums = post_w || scale || pre_w;
+  AF_REQUIRE(!sums || (scratch && scratch_floats >= 3ll * p.parts * d), "af_residual_norm_backward",
+             "scratch of %lld floats, %lld are needed", (long long)scratch_floats, 3ll * p.parts * d);
+  with_kernel(s, [&](auto, auto bwd) {
+    bwd<<<(unsigned)(p.parts / s.rows_per_block), dim3(s.threads, s.rows_per_block), 0, st>>>(p);
+  });
+  if (int rc = af::launched(ctx, fn)) return rc;
+  if (!sums) return AF_OK;
+  seam_columns_kernel<<<dim3((unsigned)((d + 31) / 32), 3), dim3(32, 8), 0, st>>>(
+      scratch, p.parts, d, post_w ? dpost_w : nullptr, scale ? dscale : nullptr, pre_w ? dpre_w : nullptr);
+  return af::launched(ctx, fn);
+}
+
+}  // extern "C"

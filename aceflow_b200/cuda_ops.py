@@ -7,6 +7,8 @@ makes exactly one ABI call on the tensor's current stream.
 """
 from __future__ import annotations
 
+from typing import NamedTuple, Optional
+
 import torch
 
 from . import _lib
@@ -592,3 +594,353 @@ def sample_rows(logits: torch.Tensor, uniforms: torch.Tensor | None = None, cont
     _lib.call("af_sample_rows", _ctx(logits), _p(logits), rows, V, ctx_ptr, int(stride), int(clen), float(temperature),
               int(top_k), float(top_p), float(repetition_penalty), _p(uniforms), _p(out), _stream(logits))
     return out
+
+
+# ------------------------------------------------------------ rotary positions
+ROTARY_LAYOUTS = ("interleaved", "half")
+
+
+def rotary_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: str | None = None, factor: float = 1.0,
+                       original_length: int | None = None, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                       device=None):
+    """(inv_freq fp32 [rot_dim / 2], scale) for `rotary`: inv_freq[i] =
+    base^(-2i / rot_dim), adapted to contexts `factor` times as long as the
+    trained ones:
+
+    None      unchanged
+    "linear"  every frequency / factor (position interpolation)
+    "ntk"     the base raised so that the slowest frequency is / factor and the
+              fastest stays (base * factor^(rot_dim / (rot_dim - 2)))
+    "yarn"    by parts (Peng et al. 2023): frequencies that make beta_fast or
+              more turns within original_length stay, those with beta_slow or
+              fewer are / factor, a linear ramp between; values are scaled by
+              0.1 ln(factor) + 1 (factor > 1)
+    """
+    import math
+
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rot_dim ({rot_dim}) must be even and at least 2")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"scaling must be None, 'linear', 'ntk' or 'yarn', got {scaling!r}")
+    if not base > 0 or not factor > 0:
+        raise ValueError("base and factor must be positive")
+    if scaling == "ntk" and rot_dim > 2:
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    freq = [base ** (-2.0 * i / rot_dim) for i in range(rot_dim // 2)]
+    scale = 1.0
+    if scaling == "linear":
+        freq = [f / factor for f in freq]
+    elif scaling == "yarn":
+        if original_length is None or original_length <= 0 or not beta_fast > beta_slow:
+            raise ValueError("yarn scaling needs original_length > 0 and beta_fast > beta_slow")
+        out = []
+        for f in freq:
+            turns = original_length * f / (2.0 * math.pi)
+            keep = min(1.0, max(0.0, (turns - beta_slow) / (beta_fast - beta_slow)))
+            out.append(f * keep + f / factor * (1.0 - keep))
+        freq = out
+        scale = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    return torch.tensor(freq, dtype=F32, device=device), scale
+
+
+def _same_device(x: torch.Tensor, **others) -> None:
+    for n, t in others.items():
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{n} is on {t.device}, expected {x.device}")
+
+
+def _rotary_dims(x: torch.Tensor):
+    """(B, T, heads, dim, strides) of x [B, T, heads, dim] or [rows, heads, dim]."""
+    if x.dtype not in (F32, BF16):
+        raise ValueError(f"x: expected float32 or bfloat16, got {x.dtype}")
+    if x.dim() == 3:
+        B, (T, H, D) = 1, x.shape
+        st = (0, x.stride(0), x.stride(1))
+    elif x.dim() == 4:
+        B, T, H, D = x.shape
+        st = x.stride()[:3]
+    else:
+        raise ValueError("x must be [B, T, heads, head_dim] or [rows, heads, head_dim]")
+    if D == 0 or (x.stride(-1) != 1 and D > 1):
+        raise ValueError("x: heads must have unit stride")
+    return B, T, H, D, st
+
+
+def rotary(x: torch.Tensor, inv_freq: torch.Tensor, positions=0, *, layout: str = "interleaved", scale: float = 1.0,
+           inverse: bool = False, inplace: bool = False) -> torch.Tensor:
+    """Rotary positions on x [B, T, heads, dim] or [rows, heads, dim], fp32 or
+    bf16, any strides with whole heads (a view into a packed qkv, for one)
+    (af_rotary).  inv_freq fp32 [rot_dim / 2] turns the first rot_dim values
+    of each head; positions is the first token's position (tokens follow one
+    by one), or an int32 / int64 tensor [T] or [B, T] ([rows] for a 3-D x).
+    inverse turns back (times scale all the same: the gradient).  Returns a
+    new contiguous tensor, or x itself with inplace."""
+    B, T, H, D, st = _rotary_dims(x)
+    _need(inv_freq, F32, "inv_freq")
+    if layout not in ROTARY_LAYOUTS:
+        raise ValueError(f"layout must be one of {ROTARY_LAYOUTS}, got {layout!r}")
+    rot = 2 * inv_freq.numel()
+    if inv_freq.dim() != 1 or not 2 <= rot <= D:
+        raise ValueError(f"inv_freq must hold 1 to {D // 2} frequencies for head_dim {D}")
+    dev = _dev(x)
+    pos, pst, start = None, (0, 0), 0
+    if isinstance(positions, torch.Tensor):
+        pos = positions
+        if pos.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"positions: expected int32 or int64, got {pos.dtype}")
+        if tuple(pos.shape) == (T,):
+            pst = (0, pos.stride(0))
+        elif x.dim() == 4 and tuple(pos.shape) == (B, T):
+            pst = pos.stride()
+        else:
+            raise ValueError(f"positions of shape {tuple(pos.shape)} do not match x {tuple(x.shape)}")
+        _same_device(x, inv_freq=inv_freq, positions=pos)
+    else:
+        start = int(positions)
+        _same_device(x, inv_freq=inv_freq)
+    if inplace:
+        ext = sorted((s, n) for s, n in zip(st + (1,), (B, T, H, D)) if n > 1)
+        reach = 1
+        for s, n in ext:
+            if s < reach:
+                raise ValueError("inplace: elements of x share memory")
+            reach = s * (n - 1) + reach
+        out, ost = x, st
+    else:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        ost = (T * H * D, H * D, D)
+    arr = _lib.ctypes.c_int64 * 3
+    _lib.call("af_rotary", _lib.context(dev), _p(x), _p(out), int(x.dtype == BF16), arr(*st), arr(*ost), B, T, H, D,
+              _p(inv_freq), rot, _p(pos), int(pos is not None and pos.dtype == torch.int64),
+              (_lib.ctypes.c_int64 * 2)(*pst), start, int(layout == "interleaved"), float(scale), int(inverse),
+              _stream(x))
+    return out
+
+
+class _Rotary(torch.autograd.Function):
+    """Autograd node of `rotary`: the gradient is the inverse rotation."""
+
+    @staticmethod
+    def forward(ctx, x, inv_freq, positions, layout, scale, inverse):
+        tensors = (inv_freq, positions) if isinstance(positions, torch.Tensor) else (inv_freq,)
+        ctx.save_for_backward(*tensors)
+        ctx.args = (positions if len(tensors) == 1 else None, layout, scale, inverse)
+        return rotary(x, inv_freq, positions, layout=layout, scale=scale, inverse=inverse)
+
+    @staticmethod
+    def backward(ctx, dout):
+        start, layout, scale, inverse = ctx.args
+        inv_freq = ctx.saved_tensors[0]
+        pos = start if start is not None else ctx.saved_tensors[1]
+        if dout.stride(-1) != 1:
+            dout = dout.contiguous()
+        return rotary(dout, inv_freq, pos, layout=layout, scale=scale, inverse=not inverse), None, None, None, None, None
+
+
+def rotary_autograd(x: torch.Tensor, inv_freq: torch.Tensor, positions=0, *, layout: str = "interleaved",
+                    scale: float = 1.0, inverse: bool = False) -> torch.Tensor:
+    """`rotary` as a differentiable torch op (gradients flow to x; inv_freq
+    and positions are constants)."""
+    return _Rotary.apply(x, inv_freq, positions, layout, float(scale), bool(inverse))
+
+
+# ------------------------------------------------------ the seam between blocks
+class ResidualNormGrads(NamedTuple):
+    """residual_norm_backward's results; None where the input was not given."""
+
+    x: torch.Tensor
+    h: torch.Tensor
+    gate: Optional[torch.Tensor]
+    post_w: Optional[torch.Tensor]
+    scale: Optional[torch.Tensor]
+    pre_w: Optional[torch.Tensor]
+
+
+def _rows_of(t: torch.Tensor, name: str, shape) -> tuple:
+    """(t, row stride) of rows [..., d] with one stride between them (a copy
+    where the leading dimensions have no common one)."""
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype not in (F32, BF16):
+        raise ValueError(f"{name}: expected float32 or bfloat16, got {t.dtype}")
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t, t.stride(0)
+    d = t.shape[-1]
+    if t.is_contiguous():
+        return t, d
+    want = None  # stride that the rows would have as one dimension
+    ok = t.stride(-1) == 1 or d == 1
+    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if want is None:
+            ld = s
+        elif s != want:
+            ok = False
+        want = s * n
+    if not ok or want is None:
+        return t.contiguous(), d
+    return t, ld
+
+
+def _seam_args(x, h, gate, post_w, scale, pre_w):
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError("x must have a non-empty last dimension")
+    d = x.shape[-1]
+    xt, ldx = _rows_of(x, "x", x.shape)
+    ht, ldh = _rows_of(h, "h", x.shape)
+    gt, ldg = (None, 0) if gate is None else _rows_of(gate, "gate", x.shape)
+    if gate is not None and gate.dtype != h.dtype:
+        raise ValueError(f"gate: expected {h.dtype} as h, got {gate.dtype}")
+    for n, w in (("post_w", post_w), ("scale", scale), ("pre_w", pre_w)):
+        if w is not None:
+            _need(w, F32, n)
+            if w.numel() != d:
+                raise ValueError(f"{n} must hold {d} values, got {w.numel()}")
+    _same_device(x, h=h, gate=gate, post_w=post_w, scale=scale, pre_w=pre_w)
+    return d, x.numel() // d, xt, ldx, ht, ldh, gt, ldg
+
+
+def residual_norm(x: torch.Tensor, h: torch.Tensor, *, gate: torch.Tensor | None = None,
+                  post_w: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+                  pre_w: torch.Tensor | None = None, alpha: float = 1.0, eps: float = 1e-6, out_dtype=None,
+                  want_stats: bool = False):
+    """The seam between two blocks in one pass (af_residual_norm): from the
+    residual stream x and a block's output h, both [..., d] fp32 or bf16,
+
+        n = RMSNorm(h) * post_w            (h itself without post_w)
+        z = alpha * x + scale * swish(gate) * n
+        y = RMSNorm(z) * pre_w             (None without pre_w)
+
+    gate [..., d] in h's type; post_w, scale, pre_w fp32 [d].  Returns (z in
+    x's type, y in out_dtype, h's unless given), and with want_stats also the
+    statistics that residual_norm_backward takes."""
+    d, rows, xt, ldx, ht, ldh, gt, ldg = _seam_args(x, h, gate, post_w, scale, pre_w)
+    out_dtype = h.dtype if out_dtype is None else out_dtype
+    if out_dtype not in (F32, BF16):
+        raise ValueError("out_dtype must be float32 or bfloat16")
+    ctx = _ctx(x)
+    z = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = None if pre_w is None else torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    stats = torch.empty(2, rows, dtype=F32, device=x.device) if want_stats else None
+    _lib.call("af_residual_norm", ctx, _p(xt), ldx, int(x.dtype == BF16), _p(ht), ldh, int(h.dtype == BF16), _p(gt),
+              ldg, _p(post_w), _p(scale), _p(pre_w), float(alpha), float(eps), rows, d, _p(z), _p(y),
+              int(out_dtype == BF16), _p(stats), _stream(x))
+    return (z, y, stats) if want_stats else (z, y)
+
+
+def residual_norm_backward(dz: torch.Tensor | None, dy: torch.Tensor | None, x: torch.Tensor, h: torch.Tensor,
+                           stats: torch.Tensor, *, gate: torch.Tensor | None = None,
+                           post_w: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+                           pre_w: torch.Tensor | None = None, alpha: float = 1.0) -> ResidualNormGrads:
+    """Gradients of residual_norm for the upstream gradients dz (x's type) and
+    dy (fp32 or bf16), either None for zero; `stats` and the other arguments as
+    in the forward (af_residual_norm_backward).  Makes its own scratch on
+    every call, so it can be captured into any number of CUDA graphs."""
+    d, rows, xt, ldx, ht, ldh, gt, ldg = _seam_args(x, h, gate, post_w, scale, pre_w)
+    _need(stats, F32, "stats")
+    if tuple(stats.shape) != (2, rows):
+        raise ValueError(f"stats must be [2, {rows}]")
+    if dy is not None and pre_w is None:
+        raise ValueError("dy without pre_w: the forward made no y")
+    dzt, lddz = (None, 0) if dz is None else _rows_of(dz, "dz", x.shape)
+    dyt, lddy = (None, 0) if dy is None else _rows_of(dy, "dy", x.shape)
+    if dz is not None and dz.dtype != x.dtype:
+        raise ValueError(f"dz: expected {x.dtype} as x, got {dz.dtype}")
+    _same_device(x, stats=stats, dz=dz, dy=dy)
+    ctx = _ctx(x)
+    new = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+    g = ResidualNormGrads(new(x), new(h), new(gate), new(post_w), new(scale), new(pre_w))
+    n = _lib.ctypes.c_int64()
+    scratch = None
+    if not (post_w is None and scale is None and pre_w is None):
+        _lib.call("af_residual_norm_scratch", ctx, rows, d, _lib.ctypes.byref(n))
+        scratch = torch.empty(n.value, dtype=F32, device=x.device)
+    _lib.call("af_residual_norm_backward", ctx, _p(dzt), lddz, _p(dyt), lddy, _p(xt), ldx, int(x.dtype == BF16),
+              _p(ht), ldh, int(h.dtype == BF16), _p(gt), ldg, int(dy is not None and dy.dtype == BF16), _p(post_w),
+              _p(scale), _p(pre_w), float(alpha), rows, d, _p(stats), _p(g.x), _p(g.h), _p(g.gate), _p(g.post_w),
+              _p(g.scale), _p(g.pre_w), _p(scratch), n.value, _stream(x))
+    return g
+
+
+class _ResidualNorm(torch.autograd.Function):
+    """Autograd node of residual_norm."""
+
+    @staticmethod
+    def forward(ctx, x, h, gate, post_w, scale, pre_w, alpha, eps, out_dtype):
+        z, y, stats = residual_norm(x, h, gate=gate, post_w=post_w, scale=scale, pre_w=pre_w, alpha=alpha, eps=eps,
+                                    out_dtype=out_dtype, want_stats=True)
+        ctx.save_for_backward(x, h, gate, post_w, scale, pre_w, stats)
+        ctx.alpha = alpha
+        ctx.set_materialize_grads(False)
+        return z, y
+
+    @staticmethod
+    def backward(ctx, dz, dy):
+        x, h, gate, post_w, scale, pre_w, stats = ctx.saved_tensors
+        g = residual_norm_backward(dz, dy, x, h, stats, gate=gate, post_w=post_w, scale=scale, pre_w=pre_w,
+                                   alpha=ctx.alpha)
+        return g.x, g.h, g.gate, g.post_w, g.scale, g.pre_w, None, None, None
+
+
+def residual_norm_autograd(x: torch.Tensor, h: torch.Tensor, *, gate: torch.Tensor | None = None,
+                           post_w: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+                           pre_w: torch.Tensor | None = None, alpha: float = 1.0, eps: float = 1e-6, out_dtype=None):
+    """residual_norm as a differentiable torch op: (z, y), gradients to x, h,
+    gate and the weights."""
+    return _ResidualNorm.apply(x, h, gate, post_w, scale, pre_w, float(alpha), float(eps), out_dtype)
+
+
+# -------------------------------------------------------------- filtered draw
+def _setting(v, name: str, rows: int, dtype, device):
+    """A sampling setting as (device pointer or None, value for all rows)."""
+    if isinstance(v, torch.Tensor):
+        _need(v, dtype, name)
+        if v.numel() != rows:
+            raise ValueError(f"{name} must hold one value per row ({rows}), got {v.numel()}")
+        if v.device != device:
+            raise ValueError(f"{name} is on {v.device}, expected {device}")
+        return v.data_ptr(), 0
+    return None, v
+
+
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                  repetition_penalty=1.0, context: torch.Tensor | None = None, return_logprobs: bool = False):
+    """One token per row of logits [rows, vocab] (fp32 or bf16, unit column
+    stride) under each row's own temperature, top_k, top_p, min_p and
+    repetition_penalty (af_sample_tokens): each a number for all rows or a
+    tensor [rows] on the device (int32 for top_k, else fp32).  uniforms [rows]
+    fp32 in [0, 1) decide the draws.  context [rows, L] int32: ids the penalty
+    applies to (-1 pads).  Returns int32 tokens [rows] (-1 for a row of -inf),
+    and with return_logprobs also their fp32 log-probabilities among what the
+    filters left."""
+    if logits.dtype not in (F32, BF16):
+        raise ValueError(f"logits: expected float32 or bfloat16, got {logits.dtype}")
+    if logits.dim() != 2 or logits.shape[1] == 0 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be [rows, vocab] with unit column stride")
+    rows, V = logits.shape
+    _need(uniforms, F32, "uniforms")
+    if uniforms.numel() != rows:
+        raise ValueError("uniforms must hold one value per row")
+    _same_device(logits, uniforms=uniforms, context=context)
+    dev = logits.device
+    t_ptr, t_all = _setting(temperature, "temperature", rows, F32, dev)
+    k_ptr, k_all = _setting(top_k, "top_k", rows, torch.int32, dev)
+    p_ptr, p_all = _setting(top_p, "top_p", rows, F32, dev)
+    m_ptr, m_all = _setting(min_p, "min_p", rows, F32, dev)
+    r_ptr, r_all = _setting(repetition_penalty, "repetition_penalty", rows, F32, dev)
+    if r_ptr is None and not r_all > 0:
+        raise ValueError("repetition_penalty must be positive")
+    c_ptr, c_stride, c_len = None, 0, 0
+    if context is not None and context.numel():
+        if context.dtype != torch.int32 or context.dim() != 2 or context.shape[0] != rows or (
+                context.stride(1) != 1 and context.shape[1] > 1):
+            raise ValueError("context must be an int32 [rows, L] tensor with unit column stride")
+        c_ptr, c_stride, c_len = _p(context), context.stride(0), context.shape[1]
+    ctx = _ctx(logits)
+    token = torch.empty(rows, dtype=torch.int32, device=dev)
+    logp = torch.empty(rows, dtype=F32, device=dev) if return_logprobs else None
+    _lib.call("af_sample_tokens", ctx, _p(logits), int(logits.dtype == BF16), logits.stride(0), rows, V, c_ptr,
+              c_stride, c_len, t_ptr, float(t_all), k_ptr, int(k_all), p_ptr, float(p_all), m_ptr, float(m_all), r_ptr,
+              float(r_all), _p(uniforms), _p(token), _p(logp), _stream(logits))
+    return (token, logp) if return_logprobs else token

@@ -154,6 +154,59 @@ int af_silu_mul_f32(af_ctx *ctx, const float *gate, const float *up, float *out,
 int af_add_f32(af_ctx *ctx, const float *a, const float *b, float *out, int64_t n, int64_t b_period,
                float scalar, af_stream_t stream);
 
+/* The seam between two blocks of a layer in one pass: norm behind a block,
+ * gate, residual scale, residual add, norm in front of the next block.
+ *   n = h / sqrt(mean(h^2) + eps) * post_w     (n = h when post_w is NULL)
+ *   z = alpha * x + scale * swish(gate) * n    (NULL scale, gate: left out)
+ *   y = z / sqrt(mean(z^2) + eps) * pre_w      (not computed when pre_w is NULL)
+ * The residual add and norm of AceEngine's layer (aceflow-core/src/cpu/mod.rs:
+ * 672-700, norm.rs:6-59), with the norm behind the block, gate and scale that
+ * the reference lacks.
+ *   x, h, gate  [rows][d], rows ldx, ldh, ldg elements apart; x fp32 or bf16,
+ *               h and gate fp32 or bf16 (one type).
+ *   post_w, scale, pre_w  [d] fp32 or NULL.
+ *   z [rows][d] in x's type; y [rows][d] fp32 or bf16 (y_bf16).  fp32 inside;
+ *               y comes from z before z is rounded.  z and y overlap nothing.
+ *   stats [2][rows] fp32 or NULL: 1/rms of h and of z, for the backward.
+ * d <= 16384. */
+int af_residual_norm(af_ctx *ctx, const void *x, int64_t ldx, int x_bf16, const void *h, int64_t ldh, int h_bf16,
+                     const void *gate, int64_t ldg, const float *post_w, const float *scale, const float *pre_w,
+                     float alpha, float eps, int64_t rows, int d, void *z, void *y, int y_bf16, float *stats,
+                     af_stream_t stream);
+/* Gradients of af_residual_norm from dz [rows][d] (x's type) and dy [rows][d]
+ * (y's type), either NULL for zero: dx, dh, dgate [rows][d] in their tensors'
+ * types and, in fp32, dpost_w, dscale, dpre_w [d] (each needed where its
+ * weight is given).  x, h, gate, the weights and alpha as in the forward, stats as it wrote
+ * them.  The weights' gradients are summed in a fixed order (the same bits
+ * every run) by way of `scratch`, af_residual_norm_scratch floats that the
+ * caller owns: calls on several streams or in several graphs take one each. */
+int af_residual_norm_scratch(af_ctx *ctx, int64_t rows, int d, int64_t *floats);
+int af_residual_norm_backward(af_ctx *ctx, const void *dz, int64_t lddz, const void *dy, int64_t lddy, const void *x,
+                              int64_t ldx, int x_bf16, const void *h, int64_t ldh, int h_bf16, const void *gate,
+                              int64_t ldg, int y_bf16, const float *post_w, const float *scale, const float *pre_w,
+                              float alpha, int64_t rows, int d, const float *stats, void *dx, void *dh, void *dgate,
+                              float *dpost_w, float *dscale, float *dpre_w, float *scratch, int64_t scratch_floats,
+                              af_stream_t stream);
+
+/* Rotary positions: each pair (a, b) of a head's first rot_dim values becomes
+ * scale * (a cos t - b sin t, a sin t + b cos t), t = position * inv_freq[i];
+ * the values behind them are copied.  inverse != 0 turns the other way (times
+ * scale all the same): the gradient.  RetNet's rotation of queries and keys
+ * (Sun et al. 2023, eq. 5); the reference has none.
+ *   x, out  [batch][T][heads][head_dim] fp32 or bf16 (is_bf16), unit stride
+ *           within a head; x_strides, out_strides: 3 host int64, elements
+ *           between streams, tokens and heads.  out is x with the same strides
+ *           (in place) or does not overlap it.
+ *   inv_freq [rot_dim / 2] fp32; rot_dim even, <= head_dim.
+ *   positions int32 or int64 (positions_i64), element b * pos_strides[0] +
+ *           t * pos_strides[1] for token t of stream b; NULL: start + t.
+ *   interleaved != 0: pairs (2i, 2i + 1); 0: pairs (i, i + rot_dim / 2).
+ * Angles are formed in 64 bits.  batch * T < 2^31. */
+int af_rotary(af_ctx *ctx, const void *x, void *out, int is_bf16, const int64_t *x_strides, const int64_t *out_strides,
+              int batch, int T, int heads, int head_dim, const float *inv_freq, int rot_dim, const void *positions,
+              int positions_i64, const int64_t *pos_strides, int64_t start, int interleaved, float scale, int inverse,
+              af_stream_t stream);
+
 /* ----------------------------------------------------------------- GEMM */
 /* y[M][N] = x[M][K] . W[N][K]^T (+ bias[N]), fp32 in/out with fp32-accurate
  * accumulation.  Replaces Linear.forward (aceflow/nn/layers.py:29-33) ->
@@ -424,6 +477,34 @@ int af_lm_head_argmax(af_ctx *ctx, const float *x, const float *final_norm, floa
 int af_sample_rows(af_ctx *ctx, const float *logits, int rows, int vocab, const int32_t *context_tokens,
                    int64_t context_stride, int context_len, float temperature, int top_k, float top_p,
                    float repetition_penalty, const float *uniforms, int32_t *out, af_stream_t stream);
+
+/* One token per row of logits under temperature, top-k, top-p and min-p, each
+ * row with its own settings (a batch of streams that ask for different ones).
+ * af_sample_rows' filters in its order (repetition penalty, temperature,
+ * top-k, top-p, draw), with min-p in front of the draw: of the tokens that
+ * the other filters leave, those at least min_p times as likely as the
+ * likeliest.  The sums that decide a token are exact (64-bit whole numbers),
+ * so a row's token does not depend on the batch around it.
+ *   logits  [rows][vocab] fp32 or bf16 (logits_bf16), rows row_stride elements
+ *           apart.  -inf marks a token that may not be drawn, NaN counts as
+ *           -inf; among +inf only these are drawn.  Not modified.
+ *   temperature, top_k, top_p, min_p, penalty: [rows] each, or NULL, and then
+ *           *_all stands for every row.  temperature <= 1e-4 (or NaN): the
+ *           first maximum.  top_k <= 0 and top_p >= 1: no cut; top_p <= 0 or
+ *           NaN: the likeliest token alone; min_p <= 0 or NaN: no cut; min_p >= 1: only
+ *           the maximum and its equals.  penalty 1: none.
+ *   context_tokens, context_stride, context_len: as for af_sample_rows.
+ *   uniforms [rows] in [0, 1).
+ *   token   [rows]: the drawn id, -1 where every logit is -inf or NaN.
+ *   logprob [rows] or NULL: the natural log of the token's probability among
+ *           those that the filters left (0 for a greedy row, -inf beside -1).
+ * vocab <= AF_SAMPLE_TOKENS_MAX_VOCAB.  No workspace. */
+#define AF_SAMPLE_TOKENS_MAX_VOCAB 524287
+int af_sample_tokens(af_ctx *ctx, const void *logits, int logits_bf16, int64_t row_stride, int rows, int vocab,
+                     const int32_t *context_tokens, int64_t context_stride, int context_len, const float *temperature,
+                     float temperature_all, const int32_t *top_k, int top_k_all, const float *top_p, float top_p_all,
+                     const float *min_p, float min_p_all, const float *penalty, float penalty_all,
+                     const float *uniforms, int32_t *token, float *logprob, af_stream_t stream);
 
 /* ------------------------------------------------------- multi-GPU prefill
  * One process per GPU.  Rank 0 creates an id with af_comm_unique_id, the
