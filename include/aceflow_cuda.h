@@ -499,7 +499,7 @@ int af_sample_rows(af_ctx *ctx, const float *logits, int rows, int vocab, const 
  *   logprob [rows] or NULL: the natural log of the token's probability among
  *           those that the filters left (0 for a greedy row, -inf beside -1).
  * vocab <= AF_SAMPLE_TOKENS_MAX_VOCAB.  No workspace. */
-#define AF_SAMPLE_TOKENS_MAX_VOCAB 524287
+#define AF_SAMPLE_TOKENS_MAX_VOCAB 327680
 int af_sample_tokens(af_ctx *ctx, const void *logits, int logits_bf16, int64_t row_stride, int rows, int vocab,
                      const int32_t *context_tokens, int64_t context_stride, int context_len, const float *temperature,
                      float temperature_all, const int32_t *top_k, int top_k_all, const float *top_p, float top_p_all,

@@ -1,7 +1,7 @@
 """The filtered draw (af_sample_tokens) against a float64 evaluation.
 
 The kernel's masses are whole numbers of 2^-44 of the largest weight, each off
-by less than 2^-30 of itself: a row whose deciding border lies within 1e-7 of
+by less than 2^-29 of itself: a row whose deciding border lies within 1e-7 of
 its draw (the oracle reports the distance) is not compared, every other one
 gives the same token.  The log-probability is an fp32 rounding of a value off
 by less than 1e-7.
