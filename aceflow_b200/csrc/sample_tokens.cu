@@ -30,9 +30,9 @@
 // than 2^-29 of itself off), in 64 bits: their sums do not depend on any
 // order, so a row's token is the same in every run and in every launch shape.
 //
-// Bound: a long row by instructions (about 30 per token for the mass, from
-// 256 tabulated powers and a cubic; two histogram additions where step 4
-// runs), a short one by the chain of cluster barriers.
+// Bound: a long row by instructions (about 35 per token for the mass; two
+// histogram additions where step 4 runs), a short one by the chain of cluster
+// barriers.
 #include "common.cuh"
 #include "sm100.cuh"
 
@@ -46,14 +46,12 @@ constexpr int kMaxCtas = 8;              // CTAs of a row's cluster
 constexpr int kList = 2048;              // tokens that are sorted at once
 constexpr int kBins = 46 * 16;           // w down to 2^-46 in sixteenths of an octave
 constexpr int kBinRoom = (kBins + kThreads) / kThreads * kThreads;
-constexpr float kSteps = 256.0f;         // table steps per octave
 constexpr u64 kOne = 1ull << 44;         // the mass of the largest logit
-constexpr uint32_t kNothing = 0x007fffffu;  // key of -inf: keys above it are candidates
 
-// Logit to key: larger key, larger logit; -0 and +0 are one key.  NaN counts
-// as -inf: it is never drawn.
+// A logit as it is kept: NaN counts as -inf (it is never drawn), -0 is +0.
+__device__ __forceinline__ float kept(float x) { return x == x ? x + 0.0f : -INFINITY; }
+// Logit to key: larger key, larger logit.
 __device__ __forceinline__ uint32_t key_of(float x) {
-  x = x == x ? x + 0.0f : -INFINITY;
   const uint32_t b = __float_as_uint(x);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
@@ -79,24 +77,25 @@ struct SampleParams {
   float *logprob;
 };
 
-// Shared memory of a CTA, byte offsets: this, the keys, then the bits of the
-// context's tokens.  It is addressed by 32-bit shared addresses throughout, the
+// Shared memory of a CTA, byte offsets: this with the slice's logits, then the
+// bits of the context's tokens.  It is addressed by 32-bit shared addresses throughout, the
 // same for this CTA's memory and (after mapa) another's.
 struct Layout {
   static constexpr uint32_t list = 0;                      // u64 [kList]: (~key, index), ascending is the order
   static constexpr uint32_t run = list + 8 * kList;        // u64 [kList]: running mass along the list; step 5's sums
+  static constexpr uint32_t lo = run;                      // u32 [kBinRoom], hi alike: this CTA's bins, done with
+  static constexpr uint32_t hi = lo + 4 * kBinRoom;        //   before a list is ordered
   static constexpr uint32_t bins = run + 8 * kList;        // u64 [kBinRoom]: running masses (counts) of the row's bins
-  static constexpr uint32_t lo = bins + 8 * kBinRoom;      // u32 [kBinRoom], hi alike: this CTA's bins
-  static constexpr uint32_t hi = lo + 4 * kBinRoom;
-  static constexpr uint32_t power = hi + 4 * kBinRoom;     // u32 pairs [256]: 2^(31 - j / 256) rounded, and as fp32
-  static constexpr uint32_t slot = power + 8 * 256;        // u64 [2][2][kMaxCtas]
-  static constexpr uint32_t warp = slot + 8 * 4 * kMaxCtas;  // u64 [2][kWarps]
-  static constexpr uint32_t before = warp + 8 * 2 * kWarps;  // u64 [2]
+  static constexpr uint32_t power = bins + 8 * kBinRoom;   // double [16]: 2^(44 - j / 16)
+  static constexpr uint32_t slot = power + 8 * 16;           // u64 [2][kMaxCtas]
+  static constexpr uint32_t warp = slot + 8 * 2 * kMaxCtas;  // u64 [kWarps]
+  static constexpr uint32_t before = warp + 8 * kWarps;      // u64 [2]
   static constexpr uint32_t listed = before + 16;            // u32, then found
   static constexpr uint32_t found = listed + 4;
-  static constexpr uint32_t keys = found + 12;  // u32 [slice]
+  static constexpr uint32_t logits = found + 12;  // float [slice]
 };
-static_assert(Layout::keys % 16 == 0, "keys are read sixteen bytes at a time");
+static_assert(Layout::logits % 16 == 0, "logits are read sixteen bytes at a time");
+static_assert(8 * kList >= 8 * kBinRoom, "the bins lie where the running masses come");
 
 __device__ __forceinline__ u64 lds64(uint32_t a) {
   u64 v;
@@ -150,44 +149,58 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
 }
 
-// The mass of a token: w = 2^(-t / 256), t = (max - l) 256 log2(e) / T formed
-// in two fp32 parts; w = 2^(-i / 256) 2^(-f / 256), i = rint(t), the first
-// factor from the table, the second 1 + (g + g^2/2 + g^3/6) with |g| < 0.00136.
+// The mass of a token: w = 2^-t, t = (max - l) log2(e) / T, in 64 bits.  With k
+// the whole number next to 16 t and f = t - k / 16, 2^-f is the Taylor series of
+// exp(-f ln 2) to its fourth power (|f| <= 1/32: 2^-34 off), 2^(-(k mod 16) / 16)
+// comes from a table whose 16 doubles lie in 32 different banks, and the octave
+// k / 16 goes into the exponent.  The 64-bit pipe has half the fp32 rate and
+// nothing else to do here.
 struct Weigher {
-  float top, ch, cl;
-  uint32_t power;  // Layout::power's address
-  // The place of t's whole steps, or -1 where w < 2^-46.
-  __device__ __forceinline__ int step(float x, float &f) const {
-    const float d = top - x, bb = d - top, e = (top - (d - bb)) - (x + bb);  // d + e = top - x
-    const float t = __fmul_rn(d, ch);
-    if (!(t < 46.0f * kSteps)) return -1;
-    const float tl = fmaf(d, ch, -t) + fmaf(e, ch, d * cl);
-    const float r = __fadd_rn(t, 12582912.0f);  // 1.5 * 2^23: rounds to a whole number
-    f = (t - (r - 12582912.0f)) + tl;
-    return __float_as_int(r) - 0x4b400000;
+  float top, ch;
+  double dtop, c;
+  uint32_t power;
+  // t in fp32: never smaller for a smaller logit.
+  __device__ __forceinline__ float lead(float x) const { return __fmul_rn(top - x, ch); }
+  __device__ __forceinline__ static bool some(float t) { return t < 46.0f; }
+  // k, and 31 bits of w with the shift that makes them the mass, one shift for
+  // all tokens of a k.  Only for some(lead(x)).
+  __device__ __forceinline__ uint32_t bits(float x, int &k, int &shift) const {
+    const double t = (dtop - (double)x) * c;
+    const double r = t + 422212465065984.0;  // 1.5 * 2^48: sixteenths stand in the low bits
+    k = __double2loint(r);
+    const double f = t - (r - 422212465065984.0);
+    double q = fma(f, 0.009618129107628477, -0.05550410866482158);  // (-ln 2)^n / n!, n = 4 .. 1
+    q = fma(f, q, 0.24022650695910072);
+    q = fma(f, q, -0.6931471805599453);
+    const int octave = k >> 4;
+    shift = max(13 - octave, 0);
+    u64 table;  // not volatile: nothing writes it any more, so loads of several tokens may overlap
+    asm("ld.shared.u64 %0, [%1];" : "=l"(table) : "r"(power + 8 * (k & 15)));
+    const double w = __hiloint2double((int)(table >> 32) - (octave << 20), (int)(uint32_t)table);
+    // w 2^-f, behind 2^(52 + shift): the bits above the shift stand in the low word
+    return (uint32_t)__double2loint(fma(w, f * q, w + __hiloint2double(0x43300000 + (shift << 20), 0)));
   }
-  // 31 bits of w and their shift: the mass is q << shift.
-  __device__ __forceinline__ uint32_t bits(int i, float f, int &shift) const {
-    const uint32_t at = power + 8 * (i & 255);
-    const float g = f * -0.0027076061740622863f;  // ln 2 / 256
-    const float ex = fmaf(g * g, fmaf(g, 0.16666667f, 0.5f), g);
-    const uint32_t q = lds32(at) + (uint32_t)(__float_as_int(fmaf(__uint_as_float(lds32(at + 4)), ex, 12582912.0f)) - 0x4b400000);
-    const int o = i >> 8;
-    shift = max(13 - o, 0);
-    return o > 13 ? q >> min(o - 13, 31) : q;
+  __device__ __forceinline__ u64 operator()(float x) const {
+    if (!some(lead(x))) return 0;
+    int k, shift;
+    const uint32_t q = bits(x, k, shift);
+    return (u64)__funnelshift_l(q, 0u, shift) << 32 | (q << shift);
   }
-  __device__ __forceinline__ u64 operator()(uint32_t key) const {
-    float f;
-    const int i = step(value_of(key), f);
-    if (i < 0) return 0;
-    int sh;
-    const uint32_t q = bits(i, f, sh);
-    return (u64)q << sh;
+  // log(w / mass): w's logarithm needs none.
+  __device__ __forceinline__ float log_share(float x, u64 mass) const {
+    return (float)(((double)x - dtop) * c * 0.6931471805599453 - log((double)mass * (1.0 / (double)kOne)));
   }
-  // The bin by the leading part of t alone: never smaller for a smaller logit.
-  __device__ __forceinline__ int bin(uint32_t key) const {
-    const float t = __fmul_rn(top - value_of(key), ch);
-    return t < 46.0f * kSteps ? (__float_as_int(__fadd_rn(t, 12582912.0f)) - 0x4b400000) >> 4 : kBins;
+  // The sixteenth of an octave by t's fp32 form, for counts.
+  __device__ __forceinline__ int bin(float x) const {
+    const float t = lead(x);
+    return some(t) ? __float_as_int(__fadd_rd(t * 16.0f, 12582912.0f)) - 0x4b400000 : kBins;
+  }
+  // Bounds on the logits of all tokens with t below (above) the given one.
+  __device__ __forceinline__ float logit_below(double t) const {
+    return fmaxf(__double2float_rd(dtop - (t + 1.0 / 64) / c), -3.4028235e38f);
+  }
+  __device__ __forceinline__ float logit_above(double t) const {
+    return __double2float_ru(dtop - (t - 1.0 / 64) / c);
   }
 };
 
@@ -207,89 +220,157 @@ struct Row {
   int n, base, ctas, rank;  // tokens of this CTA, their first index, CTAs of the row, this one's place
   int flip = 0;
 
-  // Totals of a and b over the row (max: the larger a).  One cluster barrier;
-  // the slots alternate, so the next exchange cannot overtake a reader.
-  __device__ void totals(u64 &a, u64 &b, bool max_a = false) {
+  // This CTA's value to every CTA of the row, from warp 0; then a cluster
+  // barrier.  The slots alternate, so the next exchange cannot overtake a reader.
+  __device__ __forceinline__ uint32_t exchange(u64 v) {
+    const uint32_t slot = sm + Layout::slot + 8 * kMaxCtas * flip;
+    flip ^= 1;
+    if (threadIdx.x < (unsigned)ctas) sts64(in_cta(slot + 8 * rank, threadIdx.x), v);
+    cluster_barrier();
+    return slot;
+  }
+  // The sum over all threads of the row.
+  __device__ u64 total(u64 v) {
     const int lane = threadIdx.x & 31;
-    auto reduce = [&](int width) {
-      for (int o = width / 2; o; o >>= 1) {
-        const u64 v = __shfl_xor_sync(0xffffffffu, a, o);
-        a = max_a ? (v > a ? v : a) : a + v;
-        b += __shfl_xor_sync(0xffffffffu, b, o);
-      }
-    };
-    reduce(32);
-    const uint32_t warp = sm + Layout::warp, slot = sm + Layout::slot + 16 * kMaxCtas * flip;
-    if (lane == 0) {
-      sts64(warp + 8 * (threadIdx.x >> 5), a);
-      sts64(warp + 8 * (kWarps + (threadIdx.x >> 5)), b);
-    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0) sts64(sm + Layout::warp + 8 * (threadIdx.x >> 5), v);
     __syncthreads();
     if (threadIdx.x < 32) {
-      a = b = 0;
-      if (lane < kWarps) a = lds64(warp + 8 * lane), b = lds64(warp + 8 * (kWarps + lane));
-      reduce(32);
-      if (lane < ctas) {
-        sts64(in_cta(slot + 8 * rank, lane), a);
-        sts64(in_cta(slot + 8 * (kMaxCtas + rank), lane), b);
-      }
+      v = lane < kWarps ? lds64(sm + Layout::warp + 8 * lane) : 0;
+#pragma unroll
+      for (int o = kWarps / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      v = __shfl_sync(0xffffffffu, v, 0);
     }
-    cluster_barrier();
-    a = b = 0;
-    if (lane < ctas) a = lds64(slot + 8 * lane), b = lds64(slot + 8 * (kMaxCtas + lane));
-    reduce(32);
-    flip ^= 1;
+    const uint32_t slot = exchange(v);
+    v = 0;
+    for (int c = 0; c < ctas; ++c) v += lds64(slot + 8 * c);
+    return v;
+  }
+  // The largest key over all threads of the row.
+  __device__ uint32_t largest(uint32_t v) {
+    const int lane = threadIdx.x & 31;
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (lane == 0) sts32(sm + Layout::warp + 8 * (threadIdx.x >> 5), v);
+    __syncthreads();
+    if (threadIdx.x < 32) v = __reduce_max_sync(0xffffffffu, lane < kWarps ? lds32(sm + Layout::warp + 8 * lane) : 0);
+    const uint32_t slot = exchange(v);
+    v = 0;
+    for (int c = 0; c < ctas; ++c) v = max(v, lds32(slot + 8 * c));
+    return v;
   }
 
   template <typename F>
-  __device__ __forceinline__ void each(F &&f) const {  // f(key, index in the slice), four keys a load
-    const int n4 = (n + 3) / 4;  // keys behind n are 0: no candidates
+  __device__ __forceinline__ void each(F &&f) const {  // f(logit, index in the slice), four a load
+    const int n4 = (n + 3) / 4;  // logits behind n are -inf: no candidates
     for (int i = threadIdx.x; i < n4; i += kThreads) {
-      const uint4 k = lds128(sm + Layout::keys + 16 * i);
-      f(k.x, 4 * i), f(k.y, 4 * i + 1), f(k.z, 4 * i + 2), f(k.w, 4 * i + 3);
+      const uint4 v = lds128(sm + Layout::logits + 16 * i);
+      f(__uint_as_float(v.x), 4 * i), f(__uint_as_float(v.y), 4 * i + 1);
+      f(__uint_as_float(v.z), 4 * i + 2), f(__uint_as_float(v.w), 4 * i + 3);
     }
   }
 
-  // Puts the tokens that `take` accepts on the first CTA's list (those that do
-  // not fit are only counted).
+  // Brings the tokens of the row whose logits lie in [lo, hi] and that `take`
+  // accepts onto the first CTA's list; returns their number.  More than kList
+  // are only counted.  Each CTA lists its own, then moves them behind those of
+  // the CTAs before it.  Ends with a cluster barrier.
   template <typename F>
-  __device__ void gather(F &&take) {
-    const uint32_t listed = in_cta(sm + Layout::listed, 0), list = in_cta(sm + Layout::list, 0);
-    each([&](uint32_t k, int i) {
-      if (k > kNothing && take(k)) {
-        const uint32_t at = add32(listed, 1u);
-        if (at < kList) sts64(list + 8 * at, (u64)~k << 32 | (unsigned)(base + i));
+  __device__ unsigned collect(float lo, float hi, F &&take) {
+    const uint32_t listed = sm + Layout::listed, list = sm + Layout::list;
+    if (threadIdx.x == 0) sts32(listed, 0);
+    __syncthreads();
+    each([&](float x, int i) {
+      if (x >= lo && x <= hi && take(x)) {
+        const unsigned group = __activemask(), lane = threadIdx.x & 31;  // one addition for the lanes that are here
+        uint32_t at = 0;
+        if (lane == __ffs(group) - 1) at = add32(listed, __popc(group));
+        at = __shfl_sync(group, at, __ffs(group) - 1) + __popc(group & ((1u << lane) - 1));
+        if (at < kList) sts64(list + 8 * at, (u64)~key_of(x) << 32 | (unsigned)(base + i));
       }
     });
+    __syncthreads();
+    const unsigned own = lds32(listed);
+    const uint32_t slot = exchange(own);
+    unsigned all = 0, before = 0;
+    for (int c = 0; c < ctas; ++c) {
+      const unsigned have = (unsigned)lds64(slot + 8 * c);
+      all += have;
+      before += c < rank ? have : 0;
+    }
+    if (rank && all <= kList) {
+      const uint32_t to = in_cta(list, 0) + 8 * before;
+      for (unsigned i = threadIdx.x; i < own; i += kThreads) sts64(to + 8 * i, lds64(list + 8 * i));
+    }
+    cluster_barrier();
+    return all;
   }
 
-  // Sorts the list's m tokens and sums their masses along it (one CTA).
   __device__ __forceinline__ u64 listed_at(int i) const { return lds64(sm + Layout::list + 8 * i); }
-  __device__ __forceinline__ uint32_t key_at(int i) const { return (uint32_t)~(listed_at(i) >> 32); }
+  __device__ __forceinline__ float logit_at(int i) const { return value_of((uint32_t)~(listed_at(i) >> 32)); }
   __device__ __forceinline__ u64 run_at(int i) const { return lds64(sm + Layout::run + 8 * i); }
-  template <typename W>
-  __device__ void order_list(int m, const W &weigh) {
-    const uint32_t list = sm + Layout::list;
-    int size = 2;
-    while (size < m) size <<= 1;
-    for (int i = m + (int)threadIdx.x; i < size; i += kThreads) sts64(list + 8 * i, ~0ull);
-    for (int k = 2; k <= size; k <<= 1)
-      for (int j = k >> 1; j; j >>= 1) {
+  // Bitonic sort of the list, E neighbours per thread in registers: partners in
+  // the same thread or warp trade without shared memory.
+  template <int E>
+  __device__ void sort_list(int m, int size) {
+    const uint32_t list = sm + Layout::list + 8 * E * threadIdx.x;
+    const int first = E * threadIdx.x;
+    u64 v[E];
+#pragma unroll
+    for (int r = 0; r < E; ++r) v[r] = first + r < m ? lds64(list + 8 * r) : ~0ull;
+    for (int k = 2; k <= size; k <<= 1) {
+      int j = k >> 1;
+      for (; j >= 32 * E; j >>= 1) {  // partners in other warps
         __syncthreads();
-        for (int i = threadIdx.x; i < size / 2; i += kThreads) {
-          const int a = ((i & ~(j - 1)) << 1) | (i & (j - 1)), b = a | j;
-          const u64 x = lds64(list + 8 * a), y = lds64(list + 8 * b);
-          if ((x > y) == ((a & k) == 0)) {
-            sts64(list + 8 * a, y);
-            sts64(list + 8 * b, x);
-          }
+#pragma unroll
+        for (int r = 0; r < E; ++r) sts64(list + 8 * r, v[r]);
+        __syncthreads();
+        const bool small = ((first & j) == 0) == ((first & k) == 0);
+        const uint32_t other = sm + Layout::list + 8 * (first ^ j);
+#pragma unroll
+        for (int r = 0; r < E; ++r) {
+          const u64 o = lds64(other + 8 * r);
+          v[r] = (o < v[r]) == small ? o : v[r];
         }
       }
+      for (; j >= E; j >>= 1) {
+        const bool small = ((first & j) == 0) == ((first & k) == 0);
+#pragma unroll
+        for (int r = 0; r < E; ++r) {
+          const u64 o = __shfl_xor_sync(0xffffffffu, v[r], j / E);
+          v[r] = (o < v[r]) == small ? o : v[r];
+        }
+      }
+#pragma unroll
+      for (int jj = E / 2; jj; jj >>= 1)
+        if (jj <= j) {
+#pragma unroll
+          for (int r = 0; r < E; ++r)
+            if (!(r & jj)) {
+              const bool up = ((first + r) & k) == 0;
+              const u64 x = v[r], y = v[r | jj];
+              v[r] = (x < y) == up ? x : y;
+              v[r | jj] = (x < y) == up ? y : x;
+            }
+        }
+    }
     __syncthreads();
+#pragma unroll
+    for (int r = 0; r < E; ++r) sts64(list + 8 * r, v[r]);
+    __syncthreads();
+  }
+  // Sorts the list's m tokens and sums their masses along it (one CTA).
+  template <typename W>
+  __device__ void order_list(int m, const W &weigh) {
+    int size = 2;
+    while (size < m) size <<= 1;
+    if (size <= kThreads)
+      sort_list<1>(m, size);
+    else
+      sort_list<kList / kThreads>(m, size);
     u64 before = 0;
     for (int i = 0; i < m; i += kThreads) {
       const int at = i + (int)threadIdx.x;
-      before = scan(at < m ? weigh(key_at(at)) : 0, before, sm + Layout::run + 8 * at);
+      before = scan(at < m ? weigh(logit_at(at)) : 0, before, sm + Layout::run + 8 * at);
     }
     __syncthreads();
   }
@@ -325,6 +406,10 @@ struct Row {
     return c;
   }
 
+  __device__ void clear_bins() {
+    for (int b = threadIdx.x; b < 2 * kBinRoom; b += kThreads) sts32(sm + Layout::lo + 4 * b, 0);  // lo and hi
+    __syncthreads();
+  }
   // Sums the bins of all CTAs into running masses (counts) over the bins: every CTA
   // does it for itself.  Call between two cluster barriers.
   __device__ void run_bins(bool counts) {
@@ -361,10 +446,11 @@ struct Row {
       cluster_barrier();
       for (int i = threadIdx.x; i < 512; i += kThreads) sts64(mass + 8 * i, 0);
       __syncthreads();
-      each([&](uint32_t k, int) {
-        if (k > kNothing && (shift == 24 || (k >> (shift + 8)) == (at.key >> (shift + 8)))) {
+      each([&](float x, int) {
+        const uint32_t k = key_of(x);
+        if (x > -INFINITY && (shift == 24 || (k >> (shift + 8)) == (at.key >> (shift + 8)))) {
           red64(count + 8 * (k >> shift & 255), 1ull);
-          red64(mass + 8 * (k >> shift & 255), weigh(k));
+          red64(mass + 8 * (k >> shift & 255), weigh(x));
         }
       });
       cluster_barrier();
@@ -393,7 +479,7 @@ struct Row {
     }
     cluster_barrier();
     if (by_mass) {
-      const u64 w = weigh(at.key), need = target - at.above;
+      const u64 w = weigh(value_of(at.key)), need = target - at.above;
       at.rank = w ? (unsigned)((need + w - 1) / w) : 1u;
     } else {
       at.rank = (unsigned)(target - before_n);
@@ -402,33 +488,36 @@ struct Row {
   }
 
   // The index of a place's token, on every thread of the CTA that holds it; -1 elsewhere.
-  __device__ int token_at(uint32_t key, unsigned place) {
-    const int per = (n + kThreads - 1) / kThreads, i0 = min((int)threadIdx.x * per, n), i1 = min(i0 + per, n);
-    const uint32_t keys = sm + Layout::keys, found = sm + Layout::found;
-    unsigned have = 0;
-    for (int i = i0; i < i1; ++i) have += lds32(keys + 4 * i) == key;
+  __device__ int token_at(float logit, unsigned place) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = (n + kWarps * 32 - 1) / (kWarps * 32) * 32, i0 = min(warp * per, n), i1 = min(i0 + per, n);
+    const uint32_t logits = sm + Layout::logits, found = sm + Layout::found;
+    auto is = [&](int i) { return i < i1 && __uint_as_float(lds32(logits + 4 * i)) == logit; };
+    unsigned have = 0;  // in this warp's stretch of the slice
+    for (int i = i0; i < i1; i += 32)
+      have += __popc(__ballot_sync(0xffffffffu, is(i + lane)));
     if (threadIdx.x == 0) sts32(found, ~0u);
-    const u64 through = scan(have, 0, sm + Layout::run + 8 * threadIdx.x);  // of this CTA
-    const uint32_t slot = sm + Layout::slot + 16 * kMaxCtas * flip;
-    u64 mine = threadIdx.x ? 0 : through, none = 0;
+    const u64 own = scan(lane ? 0 : have, 0, sm + Layout::run + 8 * threadIdx.x);  // of this CTA
     __syncthreads();
-    totals(mine, none);
-    u64 before = run_at(threadIdx.x) - have;
+    const uint32_t slot = exchange(own);
+    u64 before = run_at(32 * warp) - have;
     for (int c = 0; c < rank; ++c) before += lds64(slot + 8 * c);
     if (before < place && place <= before + have)
-      for (int i = i0; i < i1; ++i)
-        if (lds32(keys + 4 * i) == key && ++before == place) sts32(found, base + i);
+      for (int i = i0; i < i1; i += 32) {
+        const bool hit = is(i + lane);
+        const unsigned hits = __ballot_sync(0xffffffffu, hit);
+        if (hit && before + __popc(hits & ((2u << lane) - 1)) == place) sts32(found, base + i + lane);
+        before += __popc(hits);
+      }
     __syncthreads();
     return (int)lds32(found);
   }
 };
 
-__device__ __forceinline__ float log_share(u64 w, u64 mass) { return (float)(log((double)w) - log((double)mass)); }
-
 __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
-  const uint32_t sm = sm100::smem_u32(smem), keys = sm + Layout::keys;
-  const uint32_t seen = keys + 4 * p.slice;  // a bit for each token of the context in this slice
+  const uint32_t sm = sm100::smem_u32(smem), logits = sm + Layout::logits;
+  const uint32_t seen = logits + 4 * p.slice;  // a bit for each token of the context in this slice
   const int tid = threadIdx.x, ctas = (int)cluster_ctas(), rank = (int)cluster_ctarank();
   const int r = blockIdx.x / ctas;
   const int base = rank * p.slice, n = max(0, min(p.slice, p.V - base));
@@ -441,7 +530,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
   const int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
   const float u = fminf(fmaxf(p.uniforms[r], 0.0f), 0.99999994f);
 
-  // the slice as keys
+  // the slice
   const bool penalise = p.ctx_len > 0 && pen != 1.0f;
   if (penalise) {
     for (int i = tid; i < (n + 31) / 32; i += kThreads) sts32(seen + 4 * i, 0);
@@ -453,89 +542,112 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
     }
     __syncthreads();
   }
-  uint32_t kmax = 0;
+  float top = -INFINITY;
   auto keep = [&](float x, int i) {
     if (penalise && (lds32(seen + 4 * (i >> 5)) >> (i & 31) & 1)) x = x > 0.f ? x / pen : x * pen;
-    const uint32_t k = key_of(x);
-    kmax = max(kmax, k);
-    return k;
+    x = kept(x);
+    top = fmaxf(top, x);
+    return __float_as_uint(x);
   };
   const int64_t at0 = (int64_t)r * p.ld + base;
+  constexpr int kBatch = 8;  // loads a thread has in flight
+  auto scalar = [&](int from, auto &&load) {
+    for (int i0 = from + tid; i0 < n; i0 += kBatch * kThreads) {
+      float v[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (i0 + j * kThreads < n) v[j] = load(i0 + j * kThreads);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (i0 + j * kThreads < n) sts32(logits + 4 * (i0 + j * kThreads), keep(v[j], i0 + j * kThreads));
+    }
+  };
   if (p.b16) {
     const __nv_bfloat16 *l = static_cast<const __nv_bfloat16 *>(p.logits) + at0;
     const int nv = p.vec ? n / 8 : 0;
-    for (int i = tid; i < nv; i += kThreads) {
-      const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(l) + i);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-      uint32_t k[8];
+    for (int i0 = tid; i0 < nv; i0 += kBatch * kThreads) {
+      uint4 v[kBatch];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        k[2 * j] = keep(__uint_as_float(w[j] << 16), 8 * i + 2 * j);
-        k[2 * j + 1] = keep(__uint_as_float(w[j] & 0xffff0000u), 8 * i + 2 * j + 1);
+      for (int j = 0; j < kBatch; ++j)
+        if (i0 + j * kThreads < nv) v[j] = __ldcs(reinterpret_cast<const uint4 *>(l) + i0 + j * kThreads);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + j * kThreads;
+        if (i < nv) {
+          const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+          uint32_t k[8];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            k[2 * c] = keep(__uint_as_float(w[c] << 16), 8 * i + 2 * c);
+            k[2 * c + 1] = keep(__uint_as_float(w[c] & 0xffff0000u), 8 * i + 2 * c + 1);
+          }
+          sts128(logits + 32 * i, k[0], k[1], k[2], k[3]);
+          sts128(logits + 32 * i + 16, k[4], k[5], k[6], k[7]);
+        }
       }
-      sts128(keys + 32 * i, k[0], k[1], k[2], k[3]);
-      sts128(keys + 32 * i + 16, k[4], k[5], k[6], k[7]);
     }
-    for (int i = 8 * nv + tid; i < n; i += kThreads) sts32(keys + 4 * i, keep(__bfloat162float(l[i]), i));
+    scalar(8 * nv, [&](int i) { return __bfloat162float(l[i]); });
   } else {
     const float *l = static_cast<const float *>(p.logits) + at0;
     const int nv = p.vec ? n / 4 : 0;
-    for (int i = tid; i < nv; i += kThreads) {
-      const float4 v = __ldcs(reinterpret_cast<const float4 *>(l) + i);
-      const uint32_t a = keep(v.x, 4 * i), b = keep(v.y, 4 * i + 1), c = keep(v.z, 4 * i + 2), d = keep(v.w, 4 * i + 3);
-      sts128(keys + 16 * i, a, b, c, d);
+    for (int i0 = tid; i0 < nv; i0 += kBatch * kThreads) {
+      float4 v[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (i0 + j * kThreads < nv) v[j] = __ldcs(reinterpret_cast<const float4 *>(l) + i0 + j * kThreads);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + j * kThreads;
+        if (i < nv) {
+          const uint32_t a = keep(v[j].x, 4 * i), b = keep(v[j].y, 4 * i + 1), c = keep(v[j].z, 4 * i + 2),
+                         d = keep(v[j].w, 4 * i + 3);
+          sts128(logits + 16 * i, a, b, c, d);
+        }
+      }
     }
-    for (int i = 4 * nv + tid; i < n; i += kThreads) sts32(keys + 4 * i, keep(__ldcs(l + i), i));
+    scalar(4 * nv, [&](int i) { return l[i]; });
   }
-  for (int i = n + tid; i < min(p.slice, (n + 3) & ~3); i += kThreads) sts32(keys + 4 * i, 0);  // behind the slice: no candidates
-  if (tid < 256) {
-    const double v = exp2(31.0 - tid / 256.0);
-    sts32(sm + Layout::power + 8 * tid, (uint32_t)__double2ull_rn(v));
-    sts32(sm + Layout::power + 8 * tid + 4, __float_as_uint((float)v));
-  }
-  for (int b = tid; b < 2 * kBinRoom; b += kThreads) sts32(sm + Layout::lo + 4 * b, 0);  // lo and hi
-  if (tid == 0) sts32(sm + Layout::listed, 0);
+  for (int i = n + tid; i < min(p.slice, (n + 3) & ~3); i += kThreads) sts32(logits + 4 * i, 0xff800000u);  // -inf
+  if (tid < 16) sts64(sm + Layout::power + 8 * tid, (u64)__double_as_longlong(exp2(44.0 - tid / 16.0)));
   __syncthreads();
 
   // 1. the maximum
-  u64 best = kmax, live = 0;
-  row.totals(best, live, true);
-  kmax = (uint32_t)best;
-  const float top = value_of(kmax);
+  top = value_of(row.largest(key_of(top)));
   auto write = [&](int token, float logp) {
     p.token[r] = token;
     if (p.logprob) p.logprob[r] = logp;
   };
-  if (kmax <= kNothing) {
+  if (!(top > -INFINITY)) {
     if (rank == 0 && tid == 0) write(-1, -INFINITY);
     return;
   }
   if (!(temp > 1e-4f)) {
-    const int t = row.token_at(kmax, 1);
+    const int t = row.token_at(top, 1);
     if (t >= 0 && tid == 0) write(t, 0.f);
     return;
   }
-  const double c = 256.0 * 1.4426950408889634 / (double)temp;
-  Weigher weigh{top, (float)c, (float)(c - (double)(float)c), sm + Layout::power};
+  const double c = 1.4426950408889634 / (double)fminf(temp, 1e36f);  // octaves of w per unit of a logit
+  const Weigher weigh{top, (float)c, (double)top, c, sm + Layout::power};
 
   const bool cut_p = !(top_p >= 1.0f), cut_k = top_k > 0 && top_k < p.V, cut_m = min_p > 0.0f;
   const double share = cut_p ? (top_p > 0.f ? (double)top_p : 0.0) : 1.0;
   const u64 floor_m = cut_m ? (u64)ceil(fmin((double)min_p, 1.0) * (double)kOne) : 1;
-  u64 z = 0, none = 0;
+  u64 z = 0;
   if (top < INFINITY) {
     int end = 0, m = 0;
     if (cut_k) {
       // 2. counts: the tokens through the bin that holds the k-th
-      row.each([&](uint32_t k, int) {
-        if (k > kNothing) red32(sm + Layout::lo + 4 * weigh.bin(k), 1u);
+      row.clear_bins();
+      row.each([&](float x, int) {
+        if (x > -INFINITY) red32(sm + Layout::lo + 4 * weigh.bin(x), 1u);
       });
       cluster_barrier();
       row.run_bins(true);
       const int last = row.bin_of((u64)top_k);
       m = (int)min(row.through_bin(last), (u64)(kList + 1));
-      if (m <= kList) row.gather([&](uint32_t k) { return weigh.bin(k) <= last; });
-      cluster_barrier();
       if (m <= kList) {
+        m = (int)row.collect(last < kBins ? weigh.logit_below((last + 1) / 16.0) : -3.4028235e38f, INFINITY,
+                             [&](float x) { return weigh.bin(x) <= last; });
         if (rank) return;
         row.order_list(m, weigh);
         end = min(top_k, m);
@@ -543,37 +655,31 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
       }
     } else {
       // 2. the sum of all masses, then the tokens that can still matter
-      if (cut_p || !cut_m) {
-        row.each([&](uint32_t k, int) { z += weigh(k); });
-        row.totals(z, none);
-      }
       u64 least = floor_m;
       if (cut_p || !cut_m) {
+        row.each([&](float x, int) { z += weigh(x); });
+        z = row.total(z);
         const double behind = (cut_p ? 1.0 - share : 1.0 - (double)u) * (double)z / (double)p.V;
         const u64 t = behind > 2.0 ? (u64)behind - 1 : 1;
         least = t > least ? t : least;
       }
-      row.gather([&](uint32_t k) { return weigh(k) >= least; });
-      cluster_barrier();
-      const unsigned left = lds32(in_cta(sm + Layout::listed, 0));
-      if (left <= kList) {
-        cluster_barrier();
+      const float lowest = weigh.logit_below(44.0 - log2((double)least));
+      m = (int)row.collect(lowest, INFINITY, [&](float x) { return weigh(x) >= least; });
+      if (m <= kList) {
         if (rank) return;
-        m = (int)left;
         row.order_list(m, weigh);
         end = m;
         if (!cut_p && cut_m) z = row.run_at(m - 1);
       } else {
         // 4. masses by bins; the crossing of top_p and the draw each in one bin
-        row.each([&](uint32_t k, int) {
-          float f;
-          const int i = weigh.step(value_of(k), f);
-          if (i >= 0) {
-            int s;
-            const uint32_t q = weigh.bits(i, f, s);
-            if (((u64)q << s) >= least) {
-              red32(sm + Layout::lo + 4 * (i >> 4), q & 0xffffu);
-              red32(sm + Layout::hi + 4 * (i >> 4), q >> 16);
+        row.clear_bins();
+        row.each([&](float x, int) {
+          if (x >= lowest && weigh.some(weigh.lead(x))) {
+            int k, shift;
+            const uint32_t q = weigh.bits(x, k, shift);
+            if (((u64)q << shift) >= least) {
+              red32(sm + Layout::lo + 4 * k, q & 0xffffu);
+              red32(sm + Layout::hi + 4 * k, q >> 16);
             }
           }
         });
@@ -582,7 +688,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
         const u64 held = row.through_bin(kBins);
         u64 mass = cut_m ? held : z;  // of the kept tokens, unless top_p crosses before
         const u64 over = (u64)floor(share * (double)z) + 1;
-        bool fits = true, done = false;
+        bool fits = true;
         for (int pass = cut_p && over <= held ? 0 : 1; pass < 2 && fits; ++pass) {
           u64 target = over;
           if (pass) {
@@ -592,15 +698,12 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
           }
           const int b = row.bin_of(target);
           const u64 before = b ? row.through_bin(b - 1) : 0;
-          if (rank == 0 && tid == 0) sts32(sm + Layout::listed, 0);
-          cluster_barrier();
-          row.gather([&](uint32_t k) {
-            float f;
-            const int i = weigh.step(value_of(k), f);
-            return i >= 0 && (i >> 4) == b && weigh(k) >= least;
-          });
-          cluster_barrier();
-          const unsigned in_bin = lds32(in_cta(sm + Layout::listed, 0));
+          const unsigned in_bin =
+              row.collect(weigh.logit_below((b + 0.5) / 16.0), weigh.logit_above((b - 0.5) / 16.0), [&](float x) {
+                int k = -1, shift;
+                const uint32_t q = weigh.some(weigh.lead(x)) ? weigh.bits(x, k, shift) : 0;
+                return k == b && ((u64)q << shift) >= least;
+              });
           fits = in_bin <= kList;
           if (fits && rank == 0) {
             row.order_list((int)in_bin, weigh);
@@ -608,16 +711,12 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
                               (int)in_bin - 1);
             if (tid == 0) {
               sts64(sm + Layout::before, before + row.run_at(i));
-              if (pass) write((int)(uint32_t)row.listed_at(i), log_share(weigh(row.key_at(i)), mass));
+              if (pass) write((int)(uint32_t)row.listed_at(i), weigh.log_share(row.logit_at(i), mass));
             }
           }
+          if (fits && pass) return;
           cluster_barrier();
-          if (fits && !pass) mass = lds64(in_cta(sm + Layout::before, 0));
-          done = fits && pass;
-        }
-        if (done) {
-          cluster_barrier();
-          return;
+          if (fits) mass = lds64(in_cta(sm + Layout::before, 0));
         }
       }
     }
@@ -629,27 +728,28 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
       }
       if (cut_m)
         end = min(end, max(1, row.count_places(end, [&](int i) {
-                return weigh(row.key_at(i)) >= floor_m;
+                return weigh(row.logit_at(i)) >= floor_m;
               })));
       // without a cut the list is the head of a longer row: the whole row's mass counts
       const u64 mass = cut_k || cut_p || cut_m ? row.run_at(end - 1) : z;
       u64 target = (u64)ceil((double)u * (double)mass);
       target = target < 1 ? 1 : target;
       const int i = min(row.count_places(end, [&](int j) { return row.run_at(j) < target; }), end - 1);
-      if (tid == 0) write((int)(uint32_t)row.listed_at(i), log_share(weigh(row.key_at(i)), mass));
+      if (tid == 0) write((int)(uint32_t)row.listed_at(i), weigh.log_share(row.logit_at(i), mass));
       return;
     }
   }
 
   // 5. places by digits of the key
   const bool inf = top == INFINITY;  // only its equals have mass
-  auto mass_of = [&](uint32_t k) { return inf ? (k == kmax ? kOne : 0ull) : weigh(k); };
+  auto mass_of = [&](float x) { return inf ? (x == top ? kOne : 0ull) : weigh(x); };
   z = 0;
-  live = 0;
-  row.each([&](uint32_t k, int) { z += mass_of(k), live += k > kNothing; });
-  row.totals(z, live);
-  Place stop{kNothing, 1u, z};
-  auto through = [&](const Place &a) { return a.above + (u64)a.rank * mass_of(a.key); };
+  u64 live = 0;
+  row.each([&](float x, int) { z += mass_of(x), live += x > -INFINITY; });
+  z = row.total(z);
+  live = row.total(live);
+  Place stop{0u, 1u, z};
+  auto through = [&](const Place &a) { return a.key ? a.above + (u64)a.rank * mass_of(value_of(a.key)) : a.above; };
   if (cut_k && (u64)top_k < live) {
     stop = row.descend(false, (u64)top_k, mass_of);
     z = through(stop);
@@ -659,20 +759,19 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
     if (over <= z) stop = shorter(row.descend(true, over, mass_of), stop);
   }
   if (cut_m) {
-    u64 kept = 0;
-    row.each([&](uint32_t k, int) {
-      const u64 w = mass_of(k);
-      kept += w >= floor_m ? w : 0;
+    u64 kept_m = 0;
+    row.each([&](float x, int) {
+      const u64 w = mass_of(x);
+      kept_m += w >= floor_m ? w : 0;
     });
-    row.totals(kept, none);
-    stop = shorter(row.descend(true, kept, mass_of), stop);
+    stop = shorter(row.descend(true, row.total(kept_m), mass_of), stop);
   }
   const u64 mass = through(stop);
   u64 target = (u64)ceil((double)u * (double)mass);
   target = target < 1 ? 1 : (target > mass ? mass : target);
   const Place at = shorter(row.descend(true, target, mass_of), stop);
-  const int t = row.token_at(at.key, at.rank);
-  if (t >= 0 && tid == 0) write(t, log_share(mass_of(at.key), mass));
+  const int t = row.token_at(value_of(at.key), at.rank);
+  if (t >= 0 && tid == 0) write(t, inf ? -logf((float)(mass >> 44)) : weigh.log_share(value_of(at.key), mass));
 }
 
 }  // namespace
@@ -704,7 +803,7 @@ extern "C" int af_sample_tokens(af_ctx *ctx, const void *logits, int logits_bf16
   SampleParams p{logits, logits_bf16 != 0, row_stride, vocab, slice, vec, context_tokens, context_stride, context_len,
                  temperature, top_p, min_p, penalty, top_k, temperature_all, top_p_all, min_p_all, penalty_all,
                  top_k_all, uniforms, token, logprob};
-  auto bytes = [](int s) { return (size_t)Layout::keys + (size_t)s * 4 + (size_t)((s + 31) / 32) * 4; };
+  auto bytes = [](int s) { return (size_t)Layout::logits + (size_t)s * 4 + (size_t)((s + 31) / 32) * 4; };
   static std::atomic<unsigned long long> attr_devices{0};
   if (int rc = af::smem_attr(ctx, reinterpret_cast<const void *>(sample_tokens_kernel),
                              bytes((AF_SAMPLE_TOKENS_MAX_VOCAB / kMaxCtas + 7) & ~7), attr_devices, fn))
