@@ -9,19 +9,20 @@
 //   top-k  the first k;  Z = F at its end
 //   top-p  through the first place where F > top_p Z
 //   min-p  while w >= min_p (the largest w is 1)
-// and the draw is the first place where F >= u M, M = F at the shortest
-// prefix's end.  So the row is never sorted.  A cluster of CTAs holds it in
-// shared memory, one slice each (one read of the logits from HBM), and
+// so the shortest prefix is the one with the least mass M, and the draw is the
+// first place where F >= u M.  The row is never sorted.  A cluster of CTAs
+// holds it in shared memory, one slice each (one read of the logits), and
 //   1. finds the maximum;
 //   2. with top-k: counts the tokens in bins of 1/16 octave of w and takes the
 //      bins through the one that holds the k-th; else: sums w, which bounds
 //      from below the w of any token that can still matter (a token below
 //      (1 - top_p) Z / V lies behind the crossing: all such tokens together
 //      weigh less than (1 - top_p) Z);
-//   3. if at most kList tokens are left, the first CTA sorts them, sums along
-//      them and reads every place off; this is the usual case;
-//   4. else (a broad nucleus) the masses go into the same bins, a place's bin
-//      follows from their running sum, and only that bin's tokens are sorted;
+//   3. if at most kList tokens are left, the first CTA reads the places off
+//      them: it sums their masses by bins, finds a place's bin from the running
+//      sum and sorts that bin's few tokens; this is the usual case;
+//   4. else (a broad nucleus) the row's masses go into the bins, and the first
+//      CTA gets a place's bin alone and does the same in finer ones;
 //   5. else (a bin of more than kList tokens: great numbers of equal or nearly
 //      equal logits, or a top_k above kList) every place is found by
 //      descending the digits of its key over histograms.
@@ -32,7 +33,7 @@
 //
 // Bound: a long row by instructions (about 35 per token for the mass; two
 // histogram additions where step 4 runs), a short one by the chain of cluster
-// barriers.
+// barriers and the latency of 64-bit arithmetic.
 #include "common.cuh"
 #include "sm100.cuh"
 
@@ -42,11 +43,13 @@ using u64 = unsigned long long;
 using sm100::cluster_ctarank;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxCtas = 8;              // CTAs of a row's cluster
-constexpr int kList = 2048;              // tokens that are sorted at once
-constexpr int kBins = 46 * 16;           // w down to 2^-46 in sixteenths of an octave
-constexpr int kBinRoom = (kBins + kThreads) / kThreads * kThreads;
-constexpr u64 kOne = 1ull << 44;         // the mass of the largest logit
+constexpr int kMaxCtas = 8;       // CTAs of a row's cluster
+constexpr int kList = 2048;       // tokens the first CTA takes over at once
+constexpr int kSome = 512;        // of them, those of one bin that are sorted at once
+constexpr int kBins = 46 * 16;    // w down to 2^-46 in sixteenths of an octave; the rest behind them
+constexpr int kBinRoom = 2 * kThreads;
+constexpr u64 kOne = 1ull << 44;  // the mass of the largest logit
+constexpr float kLowest = -3.4028235e38f;
 
 // A logit as it is kept: NaN counts as -inf (it is never drawn), -0 is +0.
 __device__ __forceinline__ float kept(float x) { return x == x ? x + 0.0f : -INFINITY; }
@@ -78,15 +81,18 @@ struct SampleParams {
 };
 
 // Shared memory of a CTA, byte offsets: this with the slice's logits, then the
-// bits of the context's tokens.  It is addressed by 32-bit shared addresses throughout, the
-// same for this CTA's memory and (after mapa) another's.
+// bits of the context's tokens.  It is addressed by 32-bit shared addresses
+// throughout.
 struct Layout {
-  static constexpr uint32_t list = 0;                      // u64 [kList]: (~key, index), ascending is the order
-  static constexpr uint32_t run = list + 8 * kList;        // u64 [kList]: running mass along the list; step 5's sums
-  static constexpr uint32_t lo = run;                      // u32 [kBinRoom], hi alike: this CTA's bins, done with
-  static constexpr uint32_t hi = lo + 4 * kBinRoom;        //   before a list is ordered
-  static constexpr uint32_t bins = run + 8 * kList;        // u64 [kBinRoom]: running masses (counts) of the row's bins
-  static constexpr uint32_t power = bins + 8 * kBinRoom;   // double [16]: 2^(44 - j / 16)
+  static constexpr uint32_t list = 0;                  // u64 [kList]: (~key, index), ascending is the order
+  static constexpr uint32_t run = list + 8 * kList;    // u64 [kList]: running mass along a sorted list
+  static constexpr uint32_t lo = run;                  // u32 [kBinRoom], hi alike: bins while they are filled
+  static constexpr uint32_t hi = lo + 4 * kBinRoom;
+  static constexpr uint32_t some = run;                // u64 [kSome]: the tokens of one bin of the list,
+  static constexpr uint32_t some_run = some + 8 * kSome;  // u64 [kSome]: and their running mass
+  static constexpr uint32_t bins = run + 8 * kList;    // u64 [kBinRoom]: running masses (counts) over the row's bins
+  static constexpr uint32_t own_bins = hi + 4 * kBinRoom;  // alike, over the list's, until the whole list is sorted
+  static constexpr uint32_t power = bins + 8 * kBinRoom;   // double [16]
   static constexpr uint32_t slot = power + 8 * 16;           // u64 [2][kMaxCtas]
   static constexpr uint32_t warp = slot + 8 * 2 * kMaxCtas;  // u64 [kWarps]
   static constexpr uint32_t before = warp + 8 * kWarps;      // u64 [2]
@@ -95,30 +101,31 @@ struct Layout {
   static constexpr uint32_t logits = found + 12;  // float [slice]
 };
 static_assert(Layout::logits % 16 == 0, "logits are read sixteen bytes at a time");
-static_assert(8 * kList >= 8 * kBinRoom, "the bins lie where the running masses come");
+static_assert(16 * kBinRoom <= 8 * kList && 16 * kSome <= 8 * kBinRoom, "what shares the running masses' place fits");
+static_assert(kBins < kBinRoom, "every bin has room");
 
 __device__ __forceinline__ u64 lds64(uint32_t a) {
   u64 v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+  asm volatile("ld.shared.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ void sts64(uint32_t a, u64 v) {
-  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
+  asm volatile("st.shared.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
 __device__ __forceinline__ void sts32(uint32_t a, uint32_t v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
 __device__ __forceinline__ uint32_t add32(uint32_t a, uint32_t v) {
   uint32_t old;
-  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(a), "r"(v) : "memory");
+  asm volatile("atom.shared.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(a), "r"(v) : "memory");
   return old;
 }
-// This CTA's memory alone: the additions whose old value nobody needs, and vectors.
+// Additions whose old value nobody needs.
 __device__ __forceinline__ void red32(uint32_t a, uint32_t v) {
   asm volatile("red.shared.add.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
@@ -132,6 +139,21 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
 }
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// Another CTA's memory, by an address from in_cta (slower, this CTA's own too:
+// such an access leaves the SM).
+__device__ __forceinline__ u64 far64(uint32_t a) {
+  u64 v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t far32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void put_far64(uint32_t a, u64 v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
 // The same address in the cluster's CTA `rank`.
 __device__ __forceinline__ uint32_t in_cta(uint32_t a, uint32_t rank) {
@@ -149,55 +171,61 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
 }
 
-// The mass of a token: w = 2^-t, t = (max - l) log2(e) / T, in 64 bits.  With k
-// the whole number next to 16 t and f = t - k / 16, 2^-f is the Taylor series of
-// exp(-f ln 2) to its fourth power (|f| <= 1/32: 2^-34 off), 2^(-(k mod 16) / 16)
-// comes from a table whose 16 doubles lie in 32 different banks, and the octave
-// k / 16 goes into the exponent.  The 64-bit pipe has half the fp32 rate and
-// nothing else to do here.
+// 2^(44 - (j + 1/2) / 16): the middle of each sixteenth of the first octave.
+__constant__ double kPower[16] = {17215221774114.625, 16485352848845.686, 15786427971528.205, 15117135216047.139,
+                                  14476218277650.682, 13862474114786.947, 13274750690919.037, 12711944812079.727,
+                                  12173000056106.76,  11656904789671.754, 11162690269380.588, 10689428823380.896,
+                                  10236232110063.44,  9802249450588.832,  9386666232109.658,  8988702378690.727};
+
+// The mass of a token: w = 2^-t, t = (max - l) log2(e) / T.  b = floor(16 t) by
+// t's fp32 form (never smaller for a smaller logit) is its bin; in 64 bits, with
+// f = t - (b + 1/2) / 16, 2^-f is the Taylor series of exp(-f ln 2) to its
+// fourth power (|f| <= 1/32: 2^-34 off), 2^-((b mod 16 + 1/2) / 16) comes from a
+// table whose 16 doubles lie in 32 different banks, and the octave b / 16 goes
+// into the exponent.  The 64-bit pipe has half the fp32 rate and nothing else
+// to do here.
 struct Weigher {
   float top, ch;
   double dtop, c;
   uint32_t power;
-  // t in fp32: never smaller for a smaller logit.
   __device__ __forceinline__ float lead(float x) const { return __fmul_rn(top - x, ch); }
   __device__ __forceinline__ static bool some(float t) { return t < 46.0f; }
-  // k, and 31 bits of w with the shift that makes them the mass, one shift for
-  // all tokens of a k.  Only for some(lead(x)).
-  __device__ __forceinline__ uint32_t bits(float x, int &k, int &shift) const {
-    const double t = (dtop - (double)x) * c;
-    const double r = t + 422212465065984.0;  // 1.5 * 2^48: sixteenths stand in the low bits
-    k = __double2loint(r);
-    const double f = t - (r - 422212465065984.0);
+  // floor(16 t): behind 1.5 * 2^23 a sum holds no fraction.
+  __device__ __forceinline__ static int sixteenths(float t) {
+    return __float_as_int(__fadd_rd(t * 16.0f, 12582912.0f)) - 0x4b400000;
+  }
+  __device__ __forceinline__ int bin(float x) const {
+    const float t = lead(x);
+    return some(t) ? sixteenths(t) : kBins;
+  }
+  // The mass in a bin is its 31 bits << shift.
+  __device__ __forceinline__ static int shift(int b) { return max(13 - (b >> 4), 0); }
+  __device__ __forceinline__ uint32_t bits(float x, int b) const {
+    const double t = fma(dtop - (double)x, c, -0.03125);
+    const double f = t - (__hiloint2double(0x42f80000, b) - 422212465065984.0);  // 1.5 * 2^48 + b / 16
     double q = fma(f, 0.009618129107628477, -0.05550410866482158);  // (-ln 2)^n / n!, n = 4 .. 1
     q = fma(f, q, 0.24022650695910072);
     q = fma(f, q, -0.6931471805599453);
-    const int octave = k >> 4;
-    shift = max(13 - octave, 0);
-    u64 table;  // not volatile: nothing writes it any more, so loads of several tokens may overlap
-    asm("ld.shared.u64 %0, [%1];" : "=l"(table) : "r"(power + 8 * (k & 15)));
-    const double w = __hiloint2double((int)(table >> 32) - (octave << 20), (int)(uint32_t)table);
-    // w 2^-f, behind 2^(52 + shift): the bits above the shift stand in the low word
-    return (uint32_t)__double2loint(fma(w, f * q, w + __hiloint2double(0x43300000 + (shift << 20), 0)));
+    u64 table;  // not volatile: nothing writes it any more, so the loads of several tokens may overlap
+    asm("ld.shared.u64 %0, [%1];" : "=l"(table) : "r"(power + 8 * (b & 15)));
+    const double w = __hiloint2double((int)(table >> 32) - ((b >> 4) << 20), (int)(uint32_t)table);
+    // behind 2^(52 + shift) the bits above the shift stand in the low word
+    return (uint32_t)__double2loint(fma(w, f * q, w) + __hiloint2double(0x43300000 + (shift(b) << 20), 0));
   }
   __device__ __forceinline__ u64 operator()(float x) const {
-    if (!some(lead(x))) return 0;
-    int k, shift;
-    const uint32_t q = bits(x, k, shift);
-    return (u64)__funnelshift_l(q, 0u, shift) << 32 | (q << shift);
+    const float t = lead(x);
+    const int b = sixteenths(fminf(t, 46.0f)), s = shift(b);
+    const uint32_t q = bits(x, b);
+    const u64 m = (u64)__funnelshift_l(q, 0u, s) << 32 | (q << s);
+    return some(t) ? m : 0;
   }
   // log(w / mass): w's logarithm needs none.
   __device__ __forceinline__ float log_share(float x, u64 mass) const {
     return (float)(((double)x - dtop) * c * 0.6931471805599453 - log((double)mass * (1.0 / (double)kOne)));
   }
-  // The sixteenth of an octave by t's fp32 form, for counts.
-  __device__ __forceinline__ int bin(float x) const {
-    const float t = lead(x);
-    return some(t) ? __float_as_int(__fadd_rd(t * 16.0f, 12582912.0f)) - 0x4b400000 : kBins;
-  }
   // Bounds on the logits of all tokens with t below (above) the given one.
   __device__ __forceinline__ float logit_below(double t) const {
-    return fmaxf(__double2float_rd(dtop - (t + 1.0 / 64) / c), -3.4028235e38f);
+    return fmaxf(__double2float_rd(dtop - (t + 1.0 / 64) / c), kLowest);
   }
   __device__ __forceinline__ float logit_above(double t) const {
     return __double2float_ru(dtop - (t - 1.0 / 64) / c);
@@ -215,34 +243,43 @@ __device__ __forceinline__ Place shorter(const Place &a, const Place &b) {
   return a.key > b.key || (a.key == b.key && a.rank <= b.rank) ? a : b;
 }
 
+// A place on the first CTA's list: the mass through it, and its token.
+struct Pick {
+  u64 through;
+  uint32_t token;
+  float logit;
+};
+
 struct Row {
   uint32_t sm;  // this CTA's shared memory
   int n, base, ctas, rank;  // tokens of this CTA, their first index, CTAs of the row, this one's place
   int flip = 0;
 
-  // This CTA's value to every CTA of the row, from warp 0; then a cluster
-  // barrier.  The slots alternate, so the next exchange cannot overtake a reader.
+  // ---- over the row
+  // This CTA's value to every CTA of the row, then a cluster barrier.  The slots
+  // alternate, so the next exchange cannot overtake a reader.
   __device__ __forceinline__ uint32_t exchange(u64 v) {
     const uint32_t slot = sm + Layout::slot + 8 * kMaxCtas * flip;
     flip ^= 1;
-    if (threadIdx.x < (unsigned)ctas) sts64(in_cta(slot + 8 * rank, threadIdx.x), v);
+    if (threadIdx.x < (unsigned)ctas) put_far64(in_cta(slot + 8 * rank, threadIdx.x), v);
     cluster_barrier();
     return slot;
   }
-  // The sum over all threads of the row.
-  __device__ u64 total(u64 v) {
+  // The sum over the CTA's threads, on every thread.
+  __device__ u64 block_sum(u64 v) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
     if (lane == 0) sts64(sm + Layout::warp + 8 * (threadIdx.x >> 5), v);
     __syncthreads();
-    if (threadIdx.x < 32) {
-      v = lane < kWarps ? lds64(sm + Layout::warp + 8 * lane) : 0;
+    v = lds64(sm + Layout::warp + 8 * (lane & (kWarps - 1)));
 #pragma unroll
-      for (int o = kWarps / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      v = __shfl_sync(0xffffffffu, v, 0);
-    }
-    const uint32_t slot = exchange(v);
+    for (int o = kWarps / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
+  __device__ u64 total(u64 v) {
+    const uint32_t slot = exchange(block_sum(v));
     v = 0;
     for (int c = 0; c < ctas; ++c) v += lds64(slot + 8 * c);
     return v;
@@ -253,13 +290,12 @@ struct Row {
     v = __reduce_max_sync(0xffffffffu, v);
     if (lane == 0) sts32(sm + Layout::warp + 8 * (threadIdx.x >> 5), v);
     __syncthreads();
-    if (threadIdx.x < 32) v = __reduce_max_sync(0xffffffffu, lane < kWarps ? lds32(sm + Layout::warp + 8 * lane) : 0);
+    v = __reduce_max_sync(0xffffffffu, lds32(sm + Layout::warp + 8 * (lane & (kWarps - 1))));
     const uint32_t slot = exchange(v);
     v = 0;
     for (int c = 0; c < ctas; ++c) v = max(v, lds32(slot + 8 * c));
     return v;
   }
-
   template <typename F>
   __device__ __forceinline__ void each(F &&f) const {  // f(logit, index in the slice), four a load
     const int n4 = (n + 3) / 4;  // logits behind n are -inf: no candidates
@@ -269,27 +305,30 @@ struct Row {
       f(__uint_as_float(v.z), 4 * i + 2), f(__uint_as_float(v.w), 4 * i + 3);
     }
   }
-
+  // Adds a place on a list of this CTA; one addition for the lanes that are here.
+  __device__ __forceinline__ uint32_t next_place() const {
+    const unsigned group = __activemask(), lane = threadIdx.x & 31, lead = __ffs(group) - 1;
+    uint32_t at = 0;
+    if (lane == lead) at = add32(sm + Layout::listed, __popc(group));
+    return __shfl_sync(group, at, lead) + __popc(group & ((1u << lane) - 1));
+  }
   // Brings the tokens of the row whose logits lie in [lo, hi] and that `take`
   // accepts onto the first CTA's list; returns their number.  More than kList
   // are only counted.  Each CTA lists its own, then moves them behind those of
   // the CTAs before it.  Ends with a cluster barrier.
   template <typename F>
   __device__ unsigned collect(float lo, float hi, F &&take) {
-    const uint32_t listed = sm + Layout::listed, list = sm + Layout::list;
-    if (threadIdx.x == 0) sts32(listed, 0);
+    const uint32_t list = sm + Layout::list;
+    if (threadIdx.x == 0) sts32(sm + Layout::listed, 0);
     __syncthreads();
     each([&](float x, int i) {
       if (x >= lo && x <= hi && take(x)) {
-        const unsigned group = __activemask(), lane = threadIdx.x & 31;  // one addition for the lanes that are here
-        uint32_t at = 0;
-        if (lane == __ffs(group) - 1) at = add32(listed, __popc(group));
-        at = __shfl_sync(group, at, __ffs(group) - 1) + __popc(group & ((1u << lane) - 1));
+        const uint32_t at = next_place();
         if (at < kList) sts64(list + 8 * at, (u64)~key_of(x) << 32 | (unsigned)(base + i));
       }
     });
     __syncthreads();
-    const unsigned own = lds32(listed);
+    const unsigned own = lds32(sm + Layout::listed);
     const uint32_t slot = exchange(own);
     unsigned all = 0, before = 0;
     for (int c = 0; c < ctas; ++c) {
@@ -299,39 +338,107 @@ struct Row {
     }
     if (rank && all <= kList) {
       const uint32_t to = in_cta(list, 0) + 8 * before;
-      for (unsigned i = threadIdx.x; i < own; i += kThreads) sts64(to + 8 * i, lds64(list + 8 * i));
+      for (unsigned i = threadIdx.x; i < own; i += kThreads) put_far64(to + 8 * i, lds64(list + 8 * i));
     }
     cluster_barrier();
     return all;
   }
 
-  __device__ __forceinline__ u64 listed_at(int i) const { return lds64(sm + Layout::list + 8 * i); }
-  __device__ __forceinline__ float logit_at(int i) const { return value_of((uint32_t)~(listed_at(i) >> 32)); }
-  __device__ __forceinline__ u64 run_at(int i) const { return lds64(sm + Layout::run + 8 * i); }
-  // Bitonic sort of the list, E neighbours per thread in registers: partners in
-  // the same thread or warp trade without shared memory.
+  // ---- bins
+  __device__ void clear_bins() {
+    for (int b = threadIdx.x; b < 2 * kBinRoom; b += kThreads) sts32(sm + Layout::lo + 4 * b, 0);  // lo and hi
+    __syncthreads();
+  }
+  __device__ __forceinline__ void add_to_bin(int b, uint32_t q) const {
+    red32(sm + Layout::lo + 4 * b, q & 0xffffu);
+    red32(sm + Layout::hi + 4 * b, q >> 16);
+  }
+  // Running sums over the bins: of this CTA, or (far) of the whole row, which
+  // every CTA forms for itself.  shift(b) < 0: counts.
+  template <bool far, typename S>
+  __device__ void run_bins(S &&shift) {
+    const uint32_t to = sm + (far ? Layout::bins : Layout::own_bins);
+    u64 before = 0;
+#pragma unroll
+    for (int i = 0; i < kBinRoom; i += kThreads) {
+      const int b = i + (int)threadIdx.x, s = shift(b);
+      u64 lo = 0, hi = 0;
+      if (far) {
+        for (int c = 0; c < ctas; ++c) {
+          lo += far32(in_cta(sm + Layout::lo + 4 * b, c));
+          if (s >= 0) hi += far32(in_cta(sm + Layout::hi + 4 * b, c));
+        }
+      } else {
+        lo = lds32(sm + Layout::lo + 4 * b), hi = lds32(sm + Layout::hi + 4 * b);
+      }
+      before = scan(s < 0 ? lo : ((hi << 16) + lo) << s, before, to + 8 * b);
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ u64 through_bin(int b, uint32_t of = Layout::bins) const {
+    return b < 0 ? 0 : lds64(sm + of + 8 * b);
+  }
+  // The first bin whose running sum reaches target (<= the last one).
+  __device__ int bin_of(u64 target, uint32_t of = Layout::bins) {
+    int c = 0;
+#pragma unroll
+    for (int b = 0; b < kBinRoom; b += kThreads) c += __syncthreads_count(through_bin(b + (int)threadIdx.x, of) < target);
+    return min(c, kBinRoom - 1);
+  }
+
+  // ---- in one CTA
+  // Running sum over the CTA's threads behind `before`, into `to`; returns the total.
+  __device__ u64 scan(u64 v, u64 before, uint32_t to) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    __syncthreads();  // the last call's sums have been read
+    if (lane == 31) sts64(sm + Layout::warp + 8 * (threadIdx.x >> 5), v);
+    __syncthreads();
+    u64 w = lds64(sm + Layout::warp + 8 * (lane & (kWarps - 1)));
+#pragma unroll
+    for (int o = 1; o < kWarps; o <<= 1) {
+      const u64 u = __shfl_up_sync(0xffffffffu, w, o, kWarps);
+      if ((lane & (kWarps - 1)) >= o) w += u;
+    }
+    const int mine = threadIdx.x >> 5;
+    const u64 prior = __shfl_sync(0xffffffffu, w, mine ? mine - 1 : 0);
+    sts64(to, before + (mine ? prior : 0) + v);
+    return before + __shfl_sync(0xffffffffu, w, kWarps - 1);
+  }
+  // Bitonic sort of m places of a list (padded to size), E neighbours per thread
+  // in registers: partners in the same thread or warp trade without shared memory.
   template <int E>
-  __device__ void sort_list(int m, int size) {
-    const uint32_t list = sm + Layout::list + 8 * E * threadIdx.x;
+  __device__ void sort_list(uint32_t list, int m, int size) {
     const int first = E * threadIdx.x;
+    const uint32_t mine = list + 8 * first;
+    const bool in = first < size;  // whole warps
     u64 v[E];
 #pragma unroll
-    for (int r = 0; r < E; ++r) v[r] = first + r < m ? lds64(list + 8 * r) : ~0ull;
+    for (int r = 0; r < E; ++r) v[r] = first + r < m ? lds64(mine + 8 * r) : ~0ull;
     for (int k = 2; k <= size; k <<= 1) {
       int j = k >> 1;
       for (; j >= 32 * E; j >>= 1) {  // partners in other warps
         __syncthreads();
+        if (in) {
 #pragma unroll
-        for (int r = 0; r < E; ++r) sts64(list + 8 * r, v[r]);
+          for (int r = 0; r < E; ++r) sts64(mine + 8 * r, v[r]);
+        }
         __syncthreads();
-        const bool small = ((first & j) == 0) == ((first & k) == 0);
-        const uint32_t other = sm + Layout::list + 8 * (first ^ j);
+        if (in) {
+          const bool small = ((first & j) == 0) == ((first & k) == 0);
+          const uint32_t other = list + 8 * (first ^ j);
 #pragma unroll
-        for (int r = 0; r < E; ++r) {
-          const u64 o = lds64(other + 8 * r);
-          v[r] = (o < v[r]) == small ? o : v[r];
+          for (int r = 0; r < E; ++r) {
+            const u64 o = lds64(other + 8 * r);
+            v[r] = (o < v[r]) == small ? o : v[r];
+          }
         }
       }
+      if (!in) continue;
       for (; j >= E; j >>= 1) {
         const bool small = ((first & j) == 0) == ((first & k) == 0);
 #pragma unroll
@@ -355,108 +462,164 @@ struct Row {
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < E; ++r) sts64(list + 8 * r, v[r]);
+    for (int r = 0; r < E; ++r)
+      if (first + r < m) sts64(mine + 8 * r, v[r]);
     __syncthreads();
   }
-  // Sorts the list's m tokens and sums their masses along it (one CTA).
+  __device__ __forceinline__ static float logit_of(u64 entry) { return value_of((uint32_t)~(entry >> 32)); }
+  // Sorts a list's m tokens and sums their masses along it.  All threads have
+  // seen the list's entries; they see the results.
   template <typename W>
-  __device__ void order_list(int m, const W &weigh) {
-    int size = 2;
+  __device__ void order(uint32_t list, uint32_t run, int m, const W &weigh) {
+    if (m <= 32) {  // one warp does it alone
+      if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        u64 v = lane < m ? lds64(list + 8 * lane) : ~0ull;
+        for (int k = 2; k <= 32 && k < 2 * m; k <<= 1)
+          for (int j = k >> 1; j; j >>= 1) {
+            const u64 o = __shfl_xor_sync(0xffffffffu, v, j);
+            const bool small = ((lane & j) == 0) == ((lane & k) == 0);
+            v = (o < v) == small ? o : v;
+          }
+        u64 w = lane < m ? weigh(logit_of(v)) : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 u = __shfl_up_sync(0xffffffffu, w, o);
+          if (lane >= o) w += u;
+        }
+        if (lane < m) {
+          sts64(list + 8 * lane, v);
+          sts64(run + 8 * lane, w);
+        }
+      }
+      __syncthreads();
+      return;
+    }
+    int size = 64;
     while (size < m) size <<= 1;
     if (size <= kThreads)
-      sort_list<1>(m, size);
+      sort_list<1>(list, m, size);
     else
-      sort_list<kList / kThreads>(m, size);
+      sort_list<kList / kThreads>(list, m, size);
     u64 before = 0;
     for (int i = 0; i < m; i += kThreads) {
       const int at = i + (int)threadIdx.x;
-      before = scan(at < m ? weigh(logit_at(at)) : 0, before, sm + Layout::run + 8 * at);
+      before = scan(at < m ? weigh(logit_of(lds64(list + 8 * at))) : 0, before, run + 8 * at);
     }
     __syncthreads();
   }
+};
 
-  // Running sum over the CTA's threads behind `before`, into `to`; returns the total.
-  __device__ u64 scan(u64 v, u64 before, uint32_t to) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
-    }
-    __syncthreads();  // the last call's sums have been read
-    if (lane == 31) sts64(sm + Layout::warp + 8 * (threadIdx.x >> 5), v);
-    __syncthreads();
-    u64 w = lane < kWarps ? lds64(sm + Layout::warp + 8 * lane) : 0;
-#pragma unroll
-    for (int o = 1; o < kWarps; o <<= 1) {
-      const u64 u = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += u;
-    }
-    const int mine = threadIdx.x >> 5;
-    const u64 prior = __shfl_sync(0xffffffffu, w, mine ? mine - 1 : 0);
-    sts64(to, before + (mine ? prior : 0) + v);
-    return before + __shfl_sync(0xffffffffu, w, kWarps - 1);
+// The first CTA's list of m tokens, all tokens of the order between two places;
+// `base` is the mass in front of it.  Finds places by mass: bin(logit) puts the
+// tokens into at most kBinRoom bins in their order, a bin's masses have `shift`.
+template <typename W, typename B, typename S>
+struct Head {
+  Row &row;
+  const W &weigh;
+  B bin;
+  S shift;
+  int m;
+  u64 base;
+  uint32_t list = 0, run = 0;  // what is sorted now: the whole list, or the tokens of bin `at`
+  int n = 0, at = -1;
+  u64 before = 0;  // the mass in front of what is sorted
+
+  __device__ __forceinline__ u64 entry(int i) const { return lds64(row.sm + Layout::list + 8 * i); }
+  __device__ void sort_all() {
+    list = row.sm + Layout::list, run = row.sm + Layout::run;
+    n = m, at = kBinRoom, before = base;
+    row.order(list, run, m, weigh);
   }
-
-  // How many of the first m places satisfy `is` (one CTA; every thread gets it).
-  template <typename F>
-  __device__ int count_places(int m, F &&is) {
+  __device__ void begin() {
+    if (m <= 32) return sort_all();
+    row.clear_bins();
+    for (int i = threadIdx.x; i < m; i += kThreads) {
+      const float x = Row::logit_of(entry(i));
+      const int b = bin(x);
+      row.add_to_bin(b, (uint32_t)(weigh(x) >> shift(b)));
+    }
+    __syncthreads();
+    row.template run_bins<false>(shift);
+  }
+  __device__ u64 mass() const { return at == kBinRoom ? lds64(run + 8 * (m - 1)) : row.through_bin(kBinRoom - 1, Layout::own_bins); }
+  __device__ void focus(int b) {
+    if (at == kBinRoom || at == b) return;
+    if (threadIdx.x == 0) sts32(row.sm + Layout::listed, 0);
+    __syncthreads();
+    list = row.sm + Layout::some, run = row.sm + Layout::some_run;
+    for (int i = threadIdx.x; i < m; i += kThreads) {
+      const u64 e = entry(i);
+      if (bin(Row::logit_of(e)) == b) {
+        const uint32_t p = row.next_place();
+        if (p < kSome) sts64(list + 8 * p, e);
+      }
+    }
+    __syncthreads();
+    n = (int)lds32(row.sm + Layout::listed);
+    if (n > kSome) return sort_all();
+    at = b, before = base + row.through_bin(b - 1, Layout::own_bins);
+    row.order(list, run, n, weigh);
+  }
+  __device__ Pick pick(int i) const {
+    const u64 e = lds64(list + 8 * i);
+    return Pick{before + lds64(run + 8 * i), (uint32_t)e, Row::logit_of(e)};
+  }
+  // The first place where the mass reaches `target`.
+  __device__ Pick by_mass(u64 target) {
+    if (at != kBinRoom) focus(row.bin_of(target - base, Layout::own_bins));
     int c = 0;
-    for (int i = 0; i < m; i += kThreads) c += __syncthreads_count(i + (int)threadIdx.x < m && is(i + threadIdx.x));
-    return c;
+    for (int i = 0; i < n; i += kThreads)
+      c += __syncthreads_count(i + (int)threadIdx.x < n && before + lds64(run + 8 * (i + threadIdx.x)) < target);
+    return pick(min(c, n - 1));
   }
+  // The place of the given rank (from 1), `in_front` of the list's tokens lying in the bins in front of its bin b.
+  __device__ Pick by_rank(int rank, int b, int in_front) {
+    focus(b);
+    return pick((at == kBinRoom ? rank : rank - in_front) - 1);
+  }
+};
+template <typename W, typename B, typename S>
+__device__ __forceinline__ Head<W, B, S> head_of(Row &row, const W &weigh, B bin, S shift, int m, u64 base) {
+  return Head<W, B, S>{row, weigh, bin, shift, m, base};
+}
 
-  __device__ void clear_bins() {
-    for (int b = threadIdx.x; b < 2 * kBinRoom; b += kThreads) sts32(sm + Layout::lo + 4 * b, 0);  // lo and hi
-    __syncthreads();
-  }
-  // Sums the bins of all CTAs into running masses (counts) over the bins: every CTA
-  // does it for itself.  Call between two cluster barriers.
-  __device__ void run_bins(bool counts) {
-    u64 before = 0;
-    for (int i = 0; i <= kBins; i += kThreads) {
-      const int b = i + (int)threadIdx.x;
-      u64 lo = 0, hi = 0;
-      if (b <= kBins)
-        for (int c = 0; c < ctas; ++c) {
-          lo += lds32(in_cta(sm + Layout::lo + 4 * b, c));
-          if (!counts) hi += lds32(in_cta(sm + Layout::hi + 4 * b, c));
-        }
-      before = scan(counts ? lo : ((hi << 16) + lo) << max(13 - (b >> 4), 0), before, sm + Layout::bins + 8 * b);
-    }
-    __syncthreads();
-  }
-  __device__ __forceinline__ u64 through_bin(int b) const { return lds64(sm + Layout::bins + 8 * b); }
-  // The first bin whose running sum reaches target (<= the last one).
-  __device__ int bin_of(u64 target) {
-    int c = 0;
-    for (int b = 0; b <= kBins; b += kThreads)
-      c += __syncthreads_count(b + (int)threadIdx.x <= kBins && through_bin(b + (int)threadIdx.x) < target);
-    return min(c, kBins);
-  }
+__device__ __forceinline__ u64 draw_target(float u, u64 mass) {
+  const u64 t = (u64)ceil((double)u * (double)mass);
+  return t < 1 ? 1 : (t > mass ? mass : t);
+}
 
-  // Step 5: the first place where the running count (or mass) reaches `target`,
-  // by digits of the key.  All CTAs take part and know the answer.
-  template <typename W>
-  __device__ Place descend(bool by_mass, u64 target, const W &weigh) {
-    const uint32_t mass = sm + Layout::run, count = mass + 8 * 256, sum_m = count + 8 * 256, sum_n = sum_m + 8 * 256;
+// Step 5, by digits of the key: all CTAs take part and know the answers.
+struct Descent {
+  Row row;
+  Weigher weigh;
+  bool inf;  // the largest logit is +inf: only its equals have mass
+
+  __device__ __forceinline__ u64 mass(float x) const { return inf ? (x == INFINITY ? kOne : 0) : weigh(x); }
+  __device__ __forceinline__ u64 through(const Place &a) const {
+    return a.key ? a.above + (u64)a.rank * mass(value_of(a.key)) : a.above;
+  }
+  // The first place where the running count (or mass) reaches `target`.
+  __device__ Place find(bool by_mass, u64 target) {
+    const uint32_t masses = row.sm + Layout::run, counts = masses + 8 * 256, sum_m = counts + 8 * 256,
+                   sum_n = sum_m + 8 * 256;
     Place at{0u, 1u, 0};
     u64 before_n = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
       cluster_barrier();
-      for (int i = threadIdx.x; i < 512; i += kThreads) sts64(mass + 8 * i, 0);
+      for (int i = threadIdx.x; i < 512; i += kThreads) sts64(masses + 8 * i, 0);
       __syncthreads();
-      each([&](float x, int) {
+      row.each([&](float x, int) {
         const uint32_t k = key_of(x);
         if (x > -INFINITY && (shift == 24 || (k >> (shift + 8)) == (at.key >> (shift + 8)))) {
-          red64(count + 8 * (k >> shift & 255), 1ull);
-          red64(mass + 8 * (k >> shift & 255), weigh(x));
+          red64(counts + 8 * (k >> shift & 255), 1ull);
+          red64(masses + 8 * (k >> shift & 255), mass(x));
         }
       });
       cluster_barrier();
       for (int i = threadIdx.x; i < 256; i += kThreads) {
         u64 m = 0, c = 0;
-        for (int r = 0; r < ctas; ++r) m += lds64(in_cta(mass + 8 * i, r)), c += lds64(in_cta(count + 8 * i, r));
+        for (int r = 0; r < row.ctas; ++r) m += far64(in_cta(masses + 8 * i, r)), c += far64(in_cta(counts + 8 * i, r));
         sts64(sum_m + 8 * i, m);
         sts64(sum_n + 8 * i, c);
       }
@@ -469,50 +632,91 @@ struct Row {
           if ((by_mass ? dm : dc) >= target) break;
           m = dm, c = dc;
         }
-        sts32(sm + Layout::found, d);
-        sts64(sm + Layout::before, m);
-        sts64(sm + Layout::before + 8, c);
+        sts32(row.sm + Layout::found, d);
+        sts64(row.sm + Layout::before, m);
+        sts64(row.sm + Layout::before + 8, c);
       }
       __syncthreads();
-      at.key |= lds32(sm + Layout::found) << shift;
-      at.above = lds64(sm + Layout::before), before_n = lds64(sm + Layout::before + 8);
+      at.key |= lds32(row.sm + Layout::found) << shift;
+      at.above = lds64(row.sm + Layout::before), before_n = lds64(row.sm + Layout::before + 8);
     }
     cluster_barrier();
     if (by_mass) {
-      const u64 w = weigh(value_of(at.key)), need = target - at.above;
+      const u64 w = mass(value_of(at.key)), need = target - at.above;
       at.rank = w ? (unsigned)((need + w - 1) / w) : 1u;
     } else {
       at.rank = (unsigned)(target - before_n);
     }
     return at;
   }
-
-  // The index of a place's token, on every thread of the CTA that holds it; -1 elsewhere.
-  __device__ int token_at(float logit, unsigned place) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per = (n + kWarps * 32 - 1) / (kWarps * 32) * 32, i0 = min(warp * per, n), i1 = min(i0 + per, n);
-    const uint32_t logits = sm + Layout::logits, found = sm + Layout::found;
-    auto is = [&](int i) { return i < i1 && __uint_as_float(lds32(logits + 4 * i)) == logit; };
-    unsigned have = 0;  // in this warp's stretch of the slice
-    for (int i = i0; i < i1; i += 32)
-      have += __popc(__ballot_sync(0xffffffffu, is(i + lane)));
-    if (threadIdx.x == 0) sts32(found, ~0u);
-    const u64 own = scan(lane ? 0 : have, 0, sm + Layout::run + 8 * threadIdx.x);  // of this CTA
-    __syncthreads();
-    const uint32_t slot = exchange(own);
-    u64 before = run_at(32 * warp) - have;
-    for (int c = 0; c < rank; ++c) before += lds64(slot + 8 * c);
-    if (before < place && place <= before + have)
-      for (int i = i0; i < i1; i += 32) {
-        const bool hit = is(i + lane);
-        const unsigned hits = __ballot_sync(0xffffffffu, hit);
-        if (hit && before + __popc(hits & ((2u << lane) - 1)) == place) sts32(found, base + i + lane);
-        before += __popc(hits);
-      }
-    __syncthreads();
-    return (int)lds32(found);
-  }
 };
+
+// The index of the place-th (from 1) token with that logit, on every thread of
+// the CTA that holds it; -1 elsewhere.
+__device__ int token_at(Row &row, float logit, unsigned place) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = (row.n + kWarps * 32 - 1) / (kWarps * 32) * 32;
+  const int i0 = min(warp * per, row.n), i1 = min(i0 + per, row.n);  // this warp's stretch of the slice
+  const uint32_t logits = row.sm + Layout::logits, found = row.sm + Layout::found;
+  auto is = [&](int i) { return i < i1 && __uint_as_float(lds32(logits + 4 * i)) == logit; };
+  unsigned have = 0;
+  for (int i = i0; i < i1; i += 32) have += __popc(__ballot_sync(0xffffffffu, is(i + lane)));
+  if (threadIdx.x == 0) sts32(found, ~0u);
+  const u64 own = row.scan(lane ? 0 : have, 0, row.sm + Layout::run + 8 * threadIdx.x);  // of this CTA
+  __syncthreads();
+  const uint32_t slot = row.exchange(own);
+  u64 before = lds64(row.sm + Layout::run + 8 * 32 * warp) - have;
+  for (int c = 0; c < row.rank; ++c) before += lds64(slot + 8 * c);
+  if (before < place && place <= before + have)
+    for (int i = i0; i < i1; i += 32) {
+      const bool hit = is(i + lane);
+      const unsigned hits = __ballot_sync(0xffffffffu, hit);
+      if (hit && before + __popc(hits & ((2u << lane) - 1)) == place) sts32(found, row.base + i + lane);
+      before += __popc(hits);
+    }
+  __syncthreads();
+  return (int)lds32(found);
+}
+
+struct Filters {
+  bool cut_k, cut_p, cut_m;
+  int top_k;
+  double share;  // top_p
+  u64 floor_m;   // min_p
+  float u;
+  __device__ __forceinline__ u64 over(u64 z) const { return (u64)floor(share * (double)z) + 1; }  // F > top_p Z
+};
+
+// Step 5 (kept out of line: it hardly ever runs, and would cost the rest registers).
+__device__ __noinline__ void descend(Row row, Weigher weigh, Filters f, int32_t *token, float *logprob) {
+  Descent d{row, weigh, weigh.top == INFINITY};
+  u64 z = 0, live = 0;
+  d.row.each([&](float x, int) { z += d.mass(x), live += x > -INFINITY; });
+  z = d.row.total(z);
+  live = d.row.total(live);
+  Place stop{0u, 1u, z};
+  if (f.cut_k && (u64)f.top_k < live) {
+    stop = d.find(false, (u64)f.top_k);
+    z = d.through(stop);
+  }
+  if (f.cut_p && f.over(z) <= z) stop = shorter(d.find(true, f.over(z)), stop);
+  if (f.cut_m) {
+    u64 m = 0;
+    d.row.each([&](float x, int) {
+      const u64 w = d.mass(x);
+      m += w >= f.floor_m ? w : 0;
+    });
+    stop = shorter(d.find(true, d.row.total(m)), stop);
+  }
+  const u64 mass = d.through(stop);
+  const Place at = shorter(d.find(true, draw_target(f.u, mass)), stop);
+  const float x = value_of(at.key);
+  const int t = token_at(d.row, x, at.rank);
+  if (t >= 0 && threadIdx.x == 0) {
+    *token = t;
+    if (logprob) *logprob = d.inf ? -logf((float)(mass >> 44)) : weigh.log_share(x, mass);
+  }
+}
 
 __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -529,6 +733,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
   const float pen = p.penalty ? p.penalty[r] : p.penalty_all;
   const int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
   const float u = fminf(fmaxf(p.uniforms[r], 0.0f), 0.99999994f);
+  if (tid < 16) sts64(sm + Layout::power + 8 * tid, (u64)__double_as_longlong(kPower[tid]));
 
   // the slice
   const bool penalise = p.ctx_len > 0 && pen != 1.0f;
@@ -608,7 +813,6 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
     scalar(4 * nv, [&](int i) { return l[i]; });
   }
   for (int i = n + tid; i < min(p.slice, (n + 3) & ~3); i += kThreads) sts32(logits + 4 * i, 0xff800000u);  // -inf
-  if (tid < 16) sts64(sm + Layout::power + 8 * tid, (u64)__double_as_longlong(exp2(44.0 - tid / 16.0)));
   __syncthreads();
 
   // 1. the maximum
@@ -622,156 +826,122 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
     return;
   }
   if (!(temp > 1e-4f)) {
-    const int t = row.token_at(top, 1);
+    const int t = token_at(row, top, 1);
     if (t >= 0 && tid == 0) write(t, 0.f);
     return;
   }
   const double c = 1.4426950408889634 / (double)fminf(temp, 1e36f);  // octaves of w per unit of a logit
   const Weigher weigh{top, (float)c, (double)top, c, sm + Layout::power};
+  Filters f;
+  f.cut_p = !(top_p >= 1.0f), f.cut_k = top_k > 0 && top_k < p.V, f.cut_m = min_p > 0.0f;
+  f.top_k = top_k, f.u = u;
+  f.share = f.cut_p ? (top_p > 0.f ? (double)top_p : 0.0) : 1.0;
+  f.floor_m = f.cut_m ? (u64)ceil(fmin((double)min_p, 1.0) * (double)kOne) : 1;
 
-  const bool cut_p = !(top_p >= 1.0f), cut_k = top_k > 0 && top_k < p.V, cut_m = min_p > 0.0f;
-  const double share = cut_p ? (top_p > 0.f ? (double)top_p : 0.0) : 1.0;
-  const u64 floor_m = cut_m ? (u64)ceil(fmin((double)min_p, 1.0) * (double)kOne) : 1;
   u64 z = 0;
-  if (top < INFINITY) {
-    int end = 0, m = 0;
-    if (cut_k) {
-      // 2. counts: the tokens through the bin that holds the k-th
-      row.clear_bins();
-      row.each([&](float x, int) {
-        if (x > -INFINITY) red32(sm + Layout::lo + 4 * weigh.bin(x), 1u);
-      });
-      cluster_barrier();
-      row.run_bins(true);
-      const int last = row.bin_of((u64)top_k);
-      m = (int)min(row.through_bin(last), (u64)(kList + 1));
-      if (m <= kList) {
-        m = (int)row.collect(last < kBins ? weigh.logit_below((last + 1) / 16.0) : -3.4028235e38f, INFINITY,
-                             [&](float x) { return weigh.bin(x) <= last; });
-        if (rank) return;
-        row.order_list(m, weigh);
-        end = min(top_k, m);
-        z = row.run_at(end - 1);
-      }
-    } else {
-      // 2. the sum of all masses, then the tokens that can still matter
-      u64 least = floor_m;
-      if (cut_p || !cut_m) {
-        row.each([&](float x, int) { z += weigh(x); });
-        z = row.total(z);
-        const double behind = (cut_p ? 1.0 - share : 1.0 - (double)u) * (double)z / (double)p.V;
-        const u64 t = behind > 2.0 ? (u64)behind - 1 : 1;
-        least = t > least ? t : least;
-      }
-      const float lowest = weigh.logit_below(44.0 - log2((double)least));
-      m = (int)row.collect(lowest, INFINITY, [&](float x) { return weigh(x) >= least; });
-      if (m <= kList) {
-        if (rank) return;
-        row.order_list(m, weigh);
-        end = m;
-        if (!cut_p && cut_m) z = row.run_at(m - 1);
-      } else {
-        // 4. masses by bins; the crossing of top_p and the draw each in one bin
-        row.clear_bins();
-        row.each([&](float x, int) {
-          if (x >= lowest && weigh.some(weigh.lead(x))) {
-            int k, shift;
-            const uint32_t q = weigh.bits(x, k, shift);
-            if (((u64)q << shift) >= least) {
-              red32(sm + Layout::lo + 4 * k, q & 0xffffu);
-              red32(sm + Layout::hi + 4 * k, q >> 16);
-            }
-          }
-        });
-        cluster_barrier();
-        row.run_bins(false);
-        const u64 held = row.through_bin(kBins);
-        u64 mass = cut_m ? held : z;  // of the kept tokens, unless top_p crosses before
-        const u64 over = (u64)floor(share * (double)z) + 1;
-        bool fits = true;
-        for (int pass = cut_p && over <= held ? 0 : 1; pass < 2 && fits; ++pass) {
-          u64 target = over;
-          if (pass) {
-            target = (u64)ceil((double)u * (double)mass);
-            target = target < 1 ? 1 : (target > mass ? mass : target);
-            target = target > held ? held : target;
-          }
-          const int b = row.bin_of(target);
-          const u64 before = b ? row.through_bin(b - 1) : 0;
-          const unsigned in_bin =
-              row.collect(weigh.logit_below((b + 0.5) / 16.0), weigh.logit_above((b - 0.5) / 16.0), [&](float x) {
-                int k = -1, shift;
-                const uint32_t q = weigh.some(weigh.lead(x)) ? weigh.bits(x, k, shift) : 0;
-                return k == b && ((u64)q << shift) >= least;
-              });
-          fits = in_bin <= kList;
-          if (fits && rank == 0) {
-            row.order_list((int)in_bin, weigh);
-            const int i = min(row.count_places((int)in_bin, [&](int j) { return before + row.run_at(j) < target; }),
-                              (int)in_bin - 1);
-            if (tid == 0) {
-              sts64(sm + Layout::before, before + row.run_at(i));
-              if (pass) write((int)(uint32_t)row.listed_at(i), weigh.log_share(row.logit_at(i), mass));
-            }
-          }
-          if (fits && pass) return;
-          cluster_barrier();
-          if (fits) mass = lds64(in_cta(sm + Layout::before, 0));
-        }
-      }
+  unsigned m = kList + 1;
+  int last = 0, in_front = 0;
+  float lowest = kLowest;
+  if (top == INFINITY) {
+    // step 5 alone knows what to do
+  } else if (f.cut_k) {
+    // 2. counts: the tokens through the bin that holds the k-th (tokens behind all bins have no mass)
+    row.clear_bins();
+    row.each([&](float x, int) {
+      const float t = weigh.lead(x);
+      if (weigh.some(t)) red32(sm + Layout::lo + 4 * weigh.sixteenths(t), 1u);
+    });
+    cluster_barrier();
+    row.run_bins<true>([](int) { return -1; });
+    const u64 all = row.through_bin(kBinRoom - 1);
+    last = row.bin_of(min((u64)top_k, all));
+    in_front = (int)row.through_bin(last - 1);
+    if (row.through_bin(last) <= kList)
+      m = row.collect(weigh.logit_below((last + 1) / 16.0), INFINITY, [&](float x) { return weigh.bin(x) <= last; });
+  } else {
+    // 2. the sum of all masses, then the tokens that can still matter
+    u64 least = f.floor_m;
+    if (f.cut_p || !f.cut_m) {
+      row.each([&](float x, int) { z += weigh(x); });
+      z = row.total(z);
+      const double behind = (f.cut_p ? 1.0 - f.share : 1.0 - (double)u) * (double)z / (double)p.V;
+      const u64 t = behind > 2.0 ? (u64)behind - 1 : 1;
+      least = t > least ? t : least;
     }
-    if (end) {
-      // 3. every place along the sorted list
-      if (cut_p) {
-        const u64 over = (u64)floor(share * (double)z) + 1;
-        end = min(end, 1 + row.count_places(end, [&](int i) { return row.run_at(i) < over; }));
-      }
-      if (cut_m)
-        end = min(end, max(1, row.count_places(end, [&](int i) {
-                return weigh(row.logit_at(i)) >= floor_m;
-              })));
-      // without a cut the list is the head of a longer row: the whole row's mass counts
-      const u64 mass = cut_k || cut_p || cut_m ? row.run_at(end - 1) : z;
-      u64 target = (u64)ceil((double)u * (double)mass);
-      target = target < 1 ? 1 : target;
-      const int i = min(row.count_places(end, [&](int j) { return row.run_at(j) < target; }), end - 1);
-      if (tid == 0) write((int)(uint32_t)row.listed_at(i), weigh.log_share(row.logit_at(i), mass));
-      return;
-    }
+    lowest = weigh.logit_below(44.0 - (double)log2f((float)least));
+    m = row.collect(lowest, INFINITY, [](float) { return true; });
   }
 
-  // 5. places by digits of the key
-  const bool inf = top == INFINITY;  // only its equals have mass
-  auto mass_of = [&](float x) { return inf ? (x == top ? kOne : 0ull) : weigh(x); };
-  z = 0;
-  u64 live = 0;
-  row.each([&](float x, int) { z += mass_of(x), live += x > -INFINITY; });
-  z = row.total(z);
-  live = row.total(live);
-  Place stop{0u, 1u, z};
-  auto through = [&](const Place &a) { return a.key ? a.above + (u64)a.rank * mass_of(value_of(a.key)) : a.above; };
-  if (cut_k && (u64)top_k < live) {
-    stop = row.descend(false, (u64)top_k, mass_of);
-    z = through(stop);
+  if (m <= kList) {
+    // 3. every place is on the first CTA's list
+    if (rank) return;
+    auto head = head_of(row, weigh, [&](float x) { return weigh.bin(x); }, [](int b) { return Weigher::shift(b); },
+                        (int)m, 0);
+    head.begin();
+    const u64 held = head.mass();
+    if (f.cut_k) z = (int)m > top_k ? head.by_rank(top_k, last, in_front).through : held;
+    u64 mass = f.cut_k || f.cut_p || !f.cut_m ? z : held;
+    if (f.cut_m) {
+      u64 v = 0;
+      for (int i = tid; i < (int)m; i += kThreads) {
+        const u64 w = weigh(Row::logit_of(head.entry(i)));
+        v += w >= f.floor_m ? w : 0;
+      }
+      mass = min(mass, row.block_sum(v));
+    }
+    if (f.cut_p && f.over(z) <= held) mass = min(mass, head.by_mass(f.over(z)).through);
+    const Pick t = head.by_mass(min(draw_target(u, mass), held));
+    if (tid == 0) write((int)t.token, weigh.log_share(t.logit, mass));
+    return;
   }
-  if (cut_p) {
-    const u64 over = (u64)floor(share * (double)z) + 1;
-    if (over <= z) stop = shorter(row.descend(true, over, mass_of), stop);
-  }
-  if (cut_m) {
+
+  if (!f.cut_k && top < INFINITY) {
+    // 4. masses by bins; the crossing of top_p and the draw each in one bin
+    row.clear_bins();
     u64 kept_m = 0;
     row.each([&](float x, int) {
-      const u64 w = mass_of(x);
-      kept_m += w >= floor_m ? w : 0;
+      if (x >= lowest) {
+        const float t = weigh.lead(x);
+        if (weigh.some(t)) {
+          const int b = weigh.sixteenths(t);
+          const uint32_t q = weigh.bits(x, b);
+          const u64 w = (u64)q << weigh.shift(b);
+          row.add_to_bin(b, q);
+          kept_m += w >= f.floor_m ? w : 0;
+        }
+      }
     });
-    stop = shorter(row.descend(true, row.total(kept_m), mass_of), stop);
+    cluster_barrier();
+    row.run_bins<true>([](int b) { return Weigher::shift(b); });
+    const u64 held = row.through_bin(kBinRoom - 1);
+    u64 mass = f.cut_p || !f.cut_m ? z : held;
+    if (f.cut_m) mass = min(mass, row.total(kept_m));
+    bool fits = true;
+    for (int pass = f.cut_p && f.over(z) <= held ? 0 : 1; pass < 2 && fits; ++pass) {
+      const u64 target = pass ? min(draw_target(u, mass), held) : f.over(z);
+      const int b = row.bin_of(target);
+      const u64 before = row.through_bin(b - 1);
+      const float lo = weigh.logit_below((b + 1) / 16.0), hi = weigh.logit_above(b / 16.0);
+      const unsigned in_bin = row.collect(lo, hi, [&](float x) { return x >= lowest && weigh.bin(x) == b; });
+      fits = in_bin <= kList;
+      if (fits && rank == 0) {
+        const uint32_t first = key_of(hi), span = first - key_of(lo);
+        const int s = max(0, 32 - __clz(span) - 10);  // span >> s < kBinRoom
+        auto head = head_of(row, weigh, [&](float x) { return (int)((first - key_of(x)) >> s); },
+                            [&](int) { return Weigher::shift(b); }, (int)in_bin, before);
+        head.begin();
+        const Pick t = head.by_mass(target);
+        if (tid == 0) {
+          sts64(sm + Layout::before, t.through);
+          if (pass) write((int)t.token, weigh.log_share(t.logit, mass));
+        }
+      }
+      if (fits && pass) return;
+      cluster_barrier();
+      if (fits) mass = min(mass, far64(in_cta(sm + Layout::before, 0)));
+    }
   }
-  const u64 mass = through(stop);
-  u64 target = (u64)ceil((double)u * (double)mass);
-  target = target < 1 ? 1 : (target > mass ? mass : target);
-  const Place at = shorter(row.descend(true, target, mass_of), stop);
-  const int t = row.token_at(value_of(at.key), at.rank);
-  if (t >= 0 && tid == 0) write(t, inf ? -logf((float)(mass >> 44)) : weigh.log_share(value_of(at.key), mass));
+  descend(row, weigh, f, p.token + r, p.logprob ? p.logprob + r : nullptr);
 }
 
 }  // namespace
