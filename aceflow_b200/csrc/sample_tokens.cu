@@ -46,6 +46,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCtas = 8;       // CTAs of a row's cluster
 constexpr int kList = 2048;       // tokens the first CTA takes over at once
 constexpr int kSome = 512;        // of them, those of one bin that are sorted at once
+constexpr int kAlone = 64;        // tokens that one warp sorts alone
 constexpr int kBins = 46 * 16;    // w down to 2^-46 in sixteenths of an octave; the rest behind them
 constexpr int kBinRoom = 2 * kThreads;
 constexpr u64 kOne = 1ull << 44;  // the mass of the largest logit
@@ -281,7 +282,8 @@ struct Row {
   __device__ u64 total(u64 v) {
     const uint32_t slot = exchange(block_sum(v));
     v = 0;
-    for (int c = 0; c < ctas; ++c) v += lds64(slot + 8 * c);
+#pragma unroll
+    for (int c = 0; c < kMaxCtas; ++c) v += c < ctas ? lds64(slot + 8 * c) : 0;
     return v;
   }
   // The largest key over all threads of the row.
@@ -293,7 +295,8 @@ struct Row {
     v = __reduce_max_sync(0xffffffffu, lds32(sm + Layout::warp + 8 * (lane & (kWarps - 1))));
     const uint32_t slot = exchange(v);
     v = 0;
-    for (int c = 0; c < ctas; ++c) v = max(v, lds32(slot + 8 * c));
+#pragma unroll
+    for (int c = 0; c < kMaxCtas; ++c) v = max(v, c < ctas ? lds32(slot + 8 * c) : 0);
     return v;
   }
   template <typename F>
@@ -305,40 +308,46 @@ struct Row {
       f(__uint_as_float(v.z), 4 * i + 2), f(__uint_as_float(v.w), 4 * i + 3);
     }
   }
-  // Adds a place on a list of this CTA; one addition for the lanes that are here.
-  __device__ __forceinline__ uint32_t next_place() const {
-    const unsigned group = __activemask(), lane = threadIdx.x & 31, lead = __ffs(group) - 1;
-    uint32_t at = 0;
-    if (lane == lead) at = add32(sm + Layout::listed, __popc(group));
-    return __shfl_sync(group, at, lead) + __popc(group & ((1u << lane) - 1));
-  }
   // Brings the tokens of the row whose logits lie in [lo, hi] and that `take`
-  // accepts onto the first CTA's list; returns their number.  More than kList
-  // are only counted.  Each CTA lists its own, then moves them behind those of
-  // the CTAs before it.  Ends with a cluster barrier.
+  // accepts onto the first CTA's list; returns their number, with nothing
+  // brought if it is above kList.  Threads count theirs first: the places follow
+  // from the counts, without atomics.  Ends with a cluster barrier.
   template <typename F>
   __device__ unsigned collect(float lo, float hi, F &&take) {
-    const uint32_t list = sm + Layout::list;
-    if (threadIdx.x == 0) sts32(sm + Layout::listed, 0);
-    __syncthreads();
-    each([&](float x, int i) {
-      if (x >= lo && x <= hi && take(x)) {
-        const uint32_t at = next_place();
-        if (at < kList) sts64(list + 8 * at, (u64)~key_of(x) << 32 | (unsigned)(base + i));
-      }
-    });
-    __syncthreads();
-    const unsigned own = lds32(sm + Layout::listed);
-    const uint32_t slot = exchange(own);
-    unsigned all = 0, before = 0;
-    for (int c = 0; c < ctas; ++c) {
-      const unsigned have = (unsigned)lds64(slot + 8 * c);
-      all += have;
-      before += c < rank ? have : 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned mine = 0;
+    each([&](float x, int) { mine += x >= lo && x <= hi && take(x); });
+    unsigned through = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned v = __shfl_up_sync(0xffffffffu, through, o);
+      if (lane >= o) through += v;
     }
-    if (rank && all <= kList) {
-      const uint32_t to = in_cta(list, 0) + 8 * before;
-      for (unsigned i = threadIdx.x; i < own; i += kThreads) put_far64(to + 8 * i, lds64(list + 8 * i));
+    __syncthreads();
+    if (lane == 31) sts32(sm + Layout::warp + 8 * warp, through);
+    __syncthreads();
+    unsigned warps = lds32(sm + Layout::warp + 8 * (lane & (kWarps - 1)));
+#pragma unroll
+    for (int o = 1; o < kWarps; o <<= 1) {
+      const unsigned v = __shfl_up_sync(0xffffffffu, warps, o, kWarps);
+      if ((lane & (kWarps - 1)) >= o) warps += v;
+    }
+    unsigned at = through - mine;
+    const unsigned prior = __shfl_sync(0xffffffffu, warps, warp ? warp - 1 : 0);
+    if (warp) at += prior;
+    const uint32_t slot = exchange(__shfl_sync(0xffffffffu, warps, kWarps - 1));
+    unsigned all = 0;
+#pragma unroll
+    for (int c = 0; c < kMaxCtas; ++c) {
+      const unsigned have = c < ctas ? (unsigned)lds64(slot + 8 * c) : 0;
+      all += have;
+      at += c < rank ? have : 0;
+    }
+    if (all <= kList && mine) {
+      const uint32_t list = in_cta(sm + Layout::list, 0);
+      each([&](float x, int i) {
+        if (x >= lo && x <= hi && take(x)) put_far64(list + 8 * at++, (u64)~key_of(x) << 32 | (unsigned)(base + i));
+      });
     }
     cluster_barrier();
     return all;
@@ -364,10 +373,14 @@ struct Row {
       const int b = i + (int)threadIdx.x, s = shift(b);
       u64 lo = 0, hi = 0;
       if (far) {
-        for (int c = 0; c < ctas; ++c) {
-          lo += far32(in_cta(sm + Layout::lo + 4 * b, c));
-          if (s >= 0) hi += far32(in_cta(sm + Layout::hi + 4 * b, c));
+        uint32_t l[kMaxCtas], h[kMaxCtas];  // all loads under way before the first is used
+#pragma unroll
+        for (int c = 0; c < kMaxCtas; ++c) {
+          l[c] = c < ctas ? far32(in_cta(sm + Layout::lo + 4 * b, c)) : 0;
+          h[c] = c < ctas && s >= 0 ? far32(in_cta(sm + Layout::hi + 4 * b, c)) : 0;
         }
+#pragma unroll
+        for (int c = 0; c < kMaxCtas; ++c) lo += l[c], hi += h[c];
       } else {
         lo = lds32(sm + Layout::lo + 4 * b), hi = lds32(sm + Layout::hi + 4 * b);
       }
@@ -467,35 +480,66 @@ struct Row {
     __syncthreads();
   }
   __device__ __forceinline__ static float logit_of(u64 entry) { return value_of((uint32_t)~(entry >> 32)); }
+  // The same for up to 32 E places in one warp, and the running mass.
+  template <int E, typename W>
+  __device__ __forceinline__ void order_alone(uint32_t list, uint32_t run, int m, const W &weigh) {
+    const int lane = threadIdx.x, first = E * lane;
+    u64 v[E], w[E];
+#pragma unroll
+    for (int r = 0; r < E; ++r) v[r] = first + r < m ? lds64(list + 8 * (first + r)) : ~0ull;
+#pragma unroll
+    for (int k = 2; k <= 32 * E; k <<= 1) {
+#pragma unroll
+      for (int j = k >> 1; j; j >>= 1) {
+        if (j >= E) {
+          const bool small = ((first & j) == 0) == ((first & k) == 0);
+#pragma unroll
+          for (int r = 0; r < E; ++r) {
+            const u64 o = __shfl_xor_sync(0xffffffffu, v[r], j / E);
+            v[r] = (o < v[r]) == small ? o : v[r];
+          }
+        } else {  // E is 2
+          const bool up = (first & k) == 0;
+          const u64 x = v[0], y = v[E - 1];
+          v[0] = (x < y) == up ? x : y;
+          v[E - 1] = (x < y) == up ? y : x;
+        }
+      }
+    }
+    u64 t = 0;
+#pragma unroll
+    for (int r = 0; r < E; ++r) {
+      t += first + r < m ? weigh(logit_of(v[r])) : 0;
+      w[r] = t;
+    }
+    u64 s = t;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+#pragma unroll
+    for (int r = 0; r < E; ++r)
+      if (first + r < m) {
+        sts64(list + 8 * (first + r), v[r]);
+        sts64(run + 8 * (first + r), s - t + w[r]);
+      }
+  }
   // Sorts a list's m tokens and sums their masses along it.  All threads have
   // seen the list's entries; they see the results.
   template <typename W>
   __device__ void order(uint32_t list, uint32_t run, int m, const W &weigh) {
-    if (m <= 32) {  // one warp does it alone
+    if (m <= kAlone) {  // one warp does it alone
       if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
-        u64 v = lane < m ? lds64(list + 8 * lane) : ~0ull;
-        for (int k = 2; k <= 32 && k < 2 * m; k <<= 1)
-          for (int j = k >> 1; j; j >>= 1) {
-            const u64 o = __shfl_xor_sync(0xffffffffu, v, j);
-            const bool small = ((lane & j) == 0) == ((lane & k) == 0);
-            v = (o < v) == small ? o : v;
-          }
-        u64 w = lane < m ? weigh(logit_of(v)) : 0;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const u64 u = __shfl_up_sync(0xffffffffu, w, o);
-          if (lane >= o) w += u;
-        }
-        if (lane < m) {
-          sts64(list + 8 * lane, v);
-          sts64(run + 8 * lane, w);
-        }
+        if (m <= 32)
+          order_alone<1>(list, run, m, weigh);
+        else
+          order_alone<2>(list, run, m, weigh);
       }
       __syncthreads();
       return;
     }
-    int size = 64;
+    int size = 2 * kAlone;
     while (size < m) size <<= 1;
     if (size <= kThreads)
       sort_list<1>(list, m, size);
@@ -532,7 +576,7 @@ struct Head {
     row.order(list, run, m, weigh);
   }
   __device__ void begin() {
-    if (m <= 32) return sort_all();
+    if (m <= kAlone) return sort_all();
     row.clear_bins();
     for (int i = threadIdx.x; i < m; i += kThreads) {
       const float x = Row::logit_of(entry(i));
@@ -551,7 +595,7 @@ struct Head {
     for (int i = threadIdx.x; i < m; i += kThreads) {
       const u64 e = entry(i);
       if (bin(Row::logit_of(e)) == b) {
-        const uint32_t p = row.next_place();
+        const uint32_t p = add32(row.sm + Layout::listed, 1);
         if (p < kSome) sts64(list + 8 * p, e);
       }
     }
