@@ -257,6 +257,8 @@ struct Row {
   int flip = 0;
 
   // ---- over the row
+  // The first CTA's value, on every CTA.
+  __device__ __forceinline__ u64 from_first(u64 v) { return lds64(exchange(v)); }
   // This CTA's value to every CTA of the row, then a cluster barrier.  The slots
   // alternate, so the next exchange cannot overtake a reader.
   __device__ __forceinline__ uint32_t exchange(u64 v) {
@@ -363,7 +365,8 @@ struct Row {
     red32(sm + Layout::hi + 4 * b, q >> 16);
   }
   // Running sums over the bins: of this CTA, or (far) of the whole row, which
-  // every CTA forms for itself.  shift(b) < 0: counts.
+  // the first CTA alone forms (all of them reading all others' bins took five
+  // times as long) and passes the answers on.  shift(b) < 0: counts.
   template <bool far, typename S>
   __device__ void run_bins(S &&shift) {
     const uint32_t to = sm + (far ? Layout::bins : Layout::own_bins);
@@ -896,11 +899,16 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
       if (weigh.some(t)) red32(sm + Layout::lo + 4 * weigh.sixteenths(t), 1u);
     });
     cluster_barrier();
-    row.run_bins<true>([](int) { return -1; });
-    const u64 all = row.through_bin(kBinRoom - 1);
-    last = row.bin_of(min((u64)top_k, all));
-    in_front = (int)row.through_bin(last - 1);
-    if (row.through_bin(last) <= kList)
+    u64 said = 0;  // the bin, and how many tokens lie through it
+    if (rank == 0) {
+      row.run_bins<true>([](int) { return -1; });
+      last = row.bin_of(min((u64)top_k, row.through_bin(kBinRoom - 1)));
+      in_front = (int)row.through_bin(last - 1);
+      said = (u64)last << 32 | row.through_bin(last);
+    }
+    said = row.from_first(said);
+    last = (int)(said >> 32);
+    if ((uint32_t)said <= kList)
       m = row.collect(weigh.logit_below((last + 1) / 16.0), INFINITY, [&](float x) { return weigh.bin(x) <= last; });
   } else {
     // 2. the sum of all masses, then the tokens that can still matter
@@ -955,34 +963,45 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
         }
       }
     });
-    cluster_barrier();
-    row.run_bins<true>([](int b) { return Weigher::shift(b); });
-    const u64 held = row.through_bin(kBinRoom - 1);
-    u64 mass = f.cut_p || !f.cut_m ? z : held;
-    if (f.cut_m) mass = min(mass, row.total(kept_m));
-    bool fits = true;
-    for (int pass = f.cut_p && f.over(z) <= held ? 0 : 1; pass < 2 && fits; ++pass) {
-      const u64 target = pass ? min(draw_target(u, mass), held) : f.over(z);
-      const int b = row.bin_of(target);
-      const u64 before = row.through_bin(b - 1);
+    u64 mass = f.cut_p || !f.cut_m ? z : ~0ull;
+    if (f.cut_m)
+      mass = min(mass, row.total(kept_m));
+    else
+      cluster_barrier();
+    // the first CTA decides and says in which bin the next place lies
+    u64 held = 0, target = 0;
+    bool crossing = false;  // the place is where top_p is crossed, else the draw's
+    int b = 0;
+    if (rank == 0) {
+      row.run_bins<true>([](int i) { return Weigher::shift(i); });
+      held = row.through_bin(kBinRoom - 1);
+      crossing = f.cut_p && f.over(z) <= held;
+      target = crossing ? f.over(z) : min(draw_target(u, mass), held);
+      b = row.bin_of(target);
+    }
+    for (;;) {
+      const u64 said = row.from_first((u64)b << 1 | crossing);
+      b = (int)(said >> 1), crossing = said & 1;
       const float lo = weigh.logit_below((b + 1) / 16.0), hi = weigh.logit_above(b / 16.0);
       const unsigned in_bin = row.collect(lo, hi, [&](float x) { return x >= lowest && weigh.bin(x) == b; });
-      fits = in_bin <= kList;
-      if (fits && rank == 0) {
+      if (in_bin > kList) break;
+      if (!crossing && rank) return;
+      if (rank == 0) {
         const uint32_t first = key_of(hi), span = first - key_of(lo);
         const int s = max(0, 32 - __clz(span) - 10);  // span >> s < kBinRoom
         auto head = head_of(row, weigh, [&](float x) { return (int)((first - key_of(x)) >> s); },
-                            [&](int) { return Weigher::shift(b); }, (int)in_bin, before);
+                            [&](int) { return Weigher::shift(b); }, (int)in_bin, row.through_bin(b - 1));
         head.begin();
         const Pick t = head.by_mass(target);
-        if (tid == 0) {
-          sts64(sm + Layout::before, t.through);
-          if (pass) write((int)t.token, weigh.log_share(t.logit, mass));
+        if (!crossing) {
+          if (tid == 0) write((int)t.token, weigh.log_share(t.logit, mass));
+          return;
         }
+        mass = min(mass, t.through);
+        target = min(draw_target(u, mass), held);
+        b = row.bin_of(target);
+        crossing = false;
       }
-      if (fits && pass) return;
-      cluster_barrier();
-      if (fits) mass = min(mass, far64(in_cta(sm + Layout::before, 0)));
     }
   }
   descend(row, weigh, f, p.token + r, p.logprob ? p.logprob + r : nullptr);
