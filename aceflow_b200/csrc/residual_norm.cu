@@ -29,6 +29,8 @@
 // atomics, the same bits every run.
 #include "common.cuh"
 
+#include <algorithm>
+
 namespace {
 
 struct SeamParams {
@@ -121,14 +123,13 @@ __device__ __forceinline__ void weights(const float *w, int col, float (&v)[VEC]
   }
 }
 
-__device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
+// The sigmoid with the hardware's exponential and reciprocal: 2^-21 of itself
+// off (4 times that at |g| = 16), against 2^-9 of a bf16 result; with expf and
+// an IEEE division the forward spent half its instructions here.
+__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
 // swish(g) = g sigmoid(g) and its derivative, with their limit 0 at -inf.
-__device__ __forceinline__ float swish(float g) {
-  const float sg = sigmoid(g);
-  return sg > 0.f || g != g ? g * sg : 0.f;
-}
-__device__ __forceinline__ float swish_slope(float g) {
-  const float sg = sigmoid(g);
+__device__ __forceinline__ float swish(float g, float sg) { return sg > 0.f || g != g ? g * sg : 0.f; }
+__device__ __forceinline__ float swish_slope(float g, float sg) {
   return sg > 0.f || g != g ? sg * (1.f + g * (1.f - sg)) : 0.f;
 }
 
@@ -156,143 +157,185 @@ __device__ __forceinline__ void row_sum(float (&v)[NV], bool one_warp, float *re
   }
 }
 
+// A type that the kernel was compiled for (0: fp32, 1: bf16) or that comes with the call (2).
+template <int T>
+__device__ __forceinline__ bool is16(int flag) {
+  return T == 2 ? flag != 0 : T == 1;
+}
+
 // Threads of a row: a warp (blockDim.y rows per block) or the whole block
 // (blockDim.y == 1).  Thread k of a row holds values (c * n + k) * VEC ..,
-// c < K, n the row's threads.
-template <int VEC, int K>
+// c < K, n the row's threads.  Where that is one vector, the weights stay in
+// registers while a block walks over rows, and a row's loads are under way
+// while the row before it is summed.
+template <int VEC, int K, int TX, int TH>
 __global__ void __launch_bounds__(512) seam_forward_kernel(SeamParams p) {
+  constexpr bool kAhead = VEC == 8 && K == 1;
   __shared__ float red[96];
   int flip = 0;
   const int n = blockDim.x;
-  const bool one_warp = n == 32;
-  const int row = blockIdx.x * blockDim.y + threadIdx.y;
-  if (row >= p.rows) return;  // whole warps where a warp has a row; never where the block has one
+  const bool one_warp = n == 32, x16 = is16<TX>(p.x16), h16 = is16<TH>(p.h16);
+  const int step = gridDim.x * blockDim.y;
   Raw<VEC> hr[K], gr[K], xr[K];
+  auto fetch = [&](int row) {
 #pragma unroll
-  for (int c = 0; c < K; ++c) {
-    const int col = (c * n + (int)threadIdx.x) * VEC;
-    if (col < p.d) {
-      hr[c].load(p.h, row * p.ldh + col, p.h16);
-      if (p.g) gr[c].load(p.g, row * p.ldg + col, p.h16);
-      xr[c].load(p.x, row * p.ldx + col, p.x16);
+    for (int c = 0; c < K; ++c) {
+      const int col = (c * n + (int)threadIdx.x) * VEC;
+      if (col < p.d) {
+        hr[c].load(p.h, row * p.ldh + col, h16);
+        if (p.g) gr[c].load(p.g, row * p.ldg + col, h16);
+        xr[c].load(p.x, row * p.ldx + col, x16);
+      }
     }
+  };
+  float kept[3][VEC];  // with kAhead: post_w scale (each 1 where not given), pre_w
+  if (kAhead && (int)threadIdx.x * VEC < p.d) {
+    const int col = (int)threadIdx.x * VEC;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) kept[0][i] = kept[1][i] = kept[2][i] = 1.f;
+    if (p.w1) weights<VEC>(p.w1, col, kept[0]);
+    if (p.s) weights<VEC>(p.s, col, kept[1]);
+    if (p.w2) weights<VEC>(p.w2, col, kept[2]);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) kept[0][i] *= kept[1][i];
   }
-  float z[K][VEC];
-  float r1 = 1.f;
-  if (p.w1) {
+  int row = blockIdx.x * blockDim.y + threadIdx.y;
+  if (kAhead && row < p.rows) fetch(row);
+  for (; row < p.rows; row += step) {  // a block's threads leave together where they share a row
+    if (!kAhead) fetch(row);
+    float z[K][VEC], x[K][VEC];
     float sq[1] = {0.f};
 #pragma unroll
     for (int c = 0; c < K; ++c) {
       const int col = (c * n + (int)threadIdx.x) * VEC;
       if (col < p.d) {
-        float v[VEC];
-        hr[c].get(v, p.h16);
+        hr[c].get(z[c], h16);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sq[0] = fmaf(v[i], v[i], sq[0]);
+        for (int i = 0; i < VEC; ++i) sq[0] = fmaf(z[c][i], z[c][i], sq[0]);
+        // all of n but r1
+        if (p.g) {
+          float v[VEC];
+          gr[c].get(v, h16);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) z[c][i] *= swish(v[i], sigmoid(v[i]));
+        }
+        if (kAhead) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) z[c][i] *= kept[0][i];
+        } else {
+          float v[VEC];
+          if (p.w1) {
+            weights<VEC>(p.w1, col, v);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) z[c][i] *= v[i];
+          }
+          if (p.s) {
+            weights<VEC>(p.s, col, v);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) z[c][i] *= v[i];
+          }
+        }
+        xr[c].get(x[c], x16);
       }
     }
-    row_sum(sq, one_warp, red, flip);
-    r1 = 1.0f / sqrtf(sq[0] * p.inv_d + p.eps);
-  }
-  float sz[1] = {0.f};
-#pragma unroll
-  for (int c = 0; c < K; ++c) {
-    const int col = (c * n + (int)threadIdx.x) * VEC;
-    if (col < p.d) {
-      float m[VEC], v[VEC];
-      hr[c].get(m, p.h16);
-      if (p.w1) {
-        weights<VEC>(p.w1, col, v);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) m[i] = m[i] * r1 * v[i];
-      }
-      if (p.g) {
-        gr[c].get(v, p.h16);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) m[i] *= swish(v[i]);
-      }
-      if (p.s) {
-        weights<VEC>(p.s, col, v);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) m[i] *= v[i];
-      }
-      xr[c].get(v, p.x16);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        z[c][i] = fmaf(p.alpha, v[i], m[i]);
-        sz[0] = fmaf(z[c][i], z[c][i], sz[0]);
-      }
-      put<VEC>(p.z, (int64_t)row * p.d + col, z[c], p.x16);
+    if (kAhead && row + step < p.rows) fetch(row + step);
+    float r1 = 1.f;
+    if (p.w1) {
+      row_sum(sq, one_warp, red, flip);
+      r1 = 1.0f / sqrtf(sq[0] * p.inv_d + p.eps);
     }
-  }
-  float r2 = 1.f;
-  if (p.w2) {
-    row_sum(sz, one_warp, red, flip);
-    r2 = 1.0f / sqrtf(sz[0] * p.inv_d + p.eps);
+    float sz[1] = {0.f};
 #pragma unroll
     for (int c = 0; c < K; ++c) {
       const int col = (c * n + (int)threadIdx.x) * VEC;
       if (col < p.d) {
-        float v[VEC];
-        weights<VEC>(p.w2, col, v);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = z[c][i] * r2 * v[i];
-        put<VEC>(p.y, (int64_t)row * p.d + col, v, p.y16);
+        for (int i = 0; i < VEC; ++i) {
+          z[c][i] = fmaf(p.alpha, x[c][i], z[c][i] * r1);
+          sz[0] = fmaf(z[c][i], z[c][i], sz[0]);
+        }
+        put<VEC>(p.z, (int64_t)row * p.d + col, z[c], x16);
       }
     }
-  }
-  if (p.stats && threadIdx.x == 0) {
-    p.stats[row] = r1;
-    p.stats[p.rows + row] = r2;
+    float r2 = 1.f;
+    if (p.w2) {
+      row_sum(sz, one_warp, red, flip);
+      r2 = 1.0f / sqrtf(sz[0] * p.inv_d + p.eps);
+#pragma unroll
+      for (int c = 0; c < K; ++c) {
+        const int col = (c * n + (int)threadIdx.x) * VEC;
+        if (col < p.d) {
+          float v[VEC];
+          if (!kAhead) weights<VEC>(p.w2, col, v);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[i] = z[c][i] * r2 * (kAhead ? kept[2][i] : v[i]);
+          put<VEC>(p.y, (int64_t)row * p.d + col, v, p.y16);
+        }
+      }
+    }
+    if (p.stats && threadIdx.x == 0) {
+      p.stats[row] = r1;
+      p.stats[p.rows + row] = r2;
+    }
   }
 }
 
-template <int VEC, int K>
-__global__ void __launch_bounds__(512) seam_backward_kernel(SeamParams p) {
+template <int VEC, int K, int TX, int TH>
+__global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
+  constexpr bool kAhead = VEC == 8 && K == 1;
   __shared__ float red[96];
   int flip = 0;
   const int n = blockDim.x;
-  const bool one_warp = n == 32;
+  const bool one_warp = n == 32, x16 = is16<TX>(p.x16), h16 = is16<TH>(p.h16);
   float a1[K][VEC], as[K][VEC], a2[K][VEC];  // this thread's columns of dw1, ds, dw2
 #pragma unroll
   for (int c = 0; c < K; ++c)
 #pragma unroll
     for (int i = 0; i < VEC; ++i) a1[c][i] = as[c][i] = a2[c][i] = 0.f;
-  const int part = blockIdx.x * blockDim.y + threadIdx.y;  // also this row group's place among all
-  for (int row = part; row < p.rows; row += p.parts) {
-    Raw<VEC> hr[K], gr[K], xr[K], dzr[K], dyr[K];
+  Raw<VEC> hr[K], gr[K], xr[K], dzr[K], dyr[K];
+  auto fetch = [&](int row) {
 #pragma unroll
     for (int c = 0; c < K; ++c) {
       const int col = (c * n + (int)threadIdx.x) * VEC;
       if (col < p.d) {
-        hr[c].load(p.h, row * p.ldh + col, p.h16);
-        if (p.g) gr[c].load(p.g, row * p.ldg + col, p.h16);
-        if (p.dz) dzr[c].load(p.dz, row * p.lddz + col, p.x16);
+        hr[c].load(p.h, row * p.ldh + col, h16);
+        if (p.g) gr[c].load(p.g, row * p.ldg + col, h16);
+        if (p.dz) dzr[c].load(p.dz, row * p.lddz + col, x16);
         if (p.dy) {
           dyr[c].load(p.dy, row * p.lddy + col, p.y16);
-          xr[c].load(p.x, row * p.ldx + col, p.x16);
+          xr[c].load(p.x, row * p.ldx + col, x16);
         }
       }
     }
+  };
+  const int part = blockIdx.x * blockDim.y + threadIdx.y;  // also this row group's place among all
+  if (kAhead && part < p.rows) fetch(part);
+  for (int row = part; row < p.rows; row += p.parts) {
+    if (!kAhead) fetch(row);
     const float r1 = p.w1 ? p.stats[row] : 1.f, r2 = p.w2 ? p.stats[p.rows + row] : 1.f;
-    // q = d z / d n * w1 * hh, t = dy w2, zh = z r2 and the three sums
-    float sum[3] = {0.f, 0.f, 0.f};  // t zh, (dz + r2 t) q, zh q
-    float zh[K][VEC], e[K][VEC];     // e = dz + r2 t
+    // hh (h without post_w), the gate, q = s swish w1 hh, zh, e = dz + r2 t and the three sums
+    float sum[3] = {0.f, 0.f, 0.f};  // t zh, e q, zh q
+    float hh[K][VEC], g[K][VEC], sg[K][VEC], zh[K][VEC], e[K][VEC];
 #pragma unroll
     for (int c = 0; c < K; ++c) {
       const int col = (c * n + (int)threadIdx.x) * VEC;
       if (col < p.d) {
         float q[VEC], v[VEC];
-        hr[c].get(q, p.h16);
+        hr[c].get(hh[c], h16);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) q[i] = hh[c][i] *= r1;
         if (p.w1) {
           weights<VEC>(p.w1, col, v);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) q[i] = q[i] * r1 * v[i];
+          for (int i = 0; i < VEC; ++i) q[i] *= v[i];
         }
         if (p.g) {
-          gr[c].get(v, p.h16);
+          gr[c].get(g[c], h16);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) q[i] *= swish(v[i]);
+          for (int i = 0; i < VEC; ++i) {
+            sg[c][i] = sigmoid(g[c][i]);
+            q[i] *= swish(g[c][i], sg[c][i]);
+          }
         }
         if (p.s) {
           weights<VEC>(p.s, col, v);
@@ -300,14 +343,14 @@ __global__ void __launch_bounds__(512) seam_backward_kernel(SeamParams p) {
           for (int i = 0; i < VEC; ++i) q[i] *= v[i];
         }
         if (p.dz) {
-          dzr[c].get(e[c], p.x16);
+          dzr[c].get(e[c], x16);
         } else {
 #pragma unroll
           for (int i = 0; i < VEC; ++i) e[c][i] = 0.f;
         }
         if (p.dy) {
           float w[VEC], dy[VEC];
-          xr[c].get(v, p.x16);
+          xr[c].get(v, x16);
           weights<VEC>(p.w2, col, w);
           dyr[c].get(dy, p.y16);
 #pragma unroll
@@ -324,6 +367,7 @@ __global__ void __launch_bounds__(512) seam_backward_kernel(SeamParams p) {
         for (int i = 0; i < VEC; ++i) sum[1] = fmaf(e[c][i], q[i], sum[1]);
       }
     }
+    if (kAhead && row + p.parts < p.rows) fetch(row + p.parts);
     if (p.w1 || p.dy) row_sum(sum, one_warp, red, flip);
     const float m2 = p.dy ? r2 * (sum[0] * p.inv_d) : 0.f;  // r2 mean(t zh)
     const float m1 = (sum[1] - m2 * sum[2]) * p.inv_d;       // mean(N w1 hh)
@@ -332,57 +376,35 @@ __global__ void __launch_bounds__(512) seam_backward_kernel(SeamParams p) {
       const int col = (c * n + (int)threadIdx.x) * VEC;
       if (col < p.d) {
         const int64_t at = (int64_t)row * p.d + col;
-        float o[VEC], nn[VEC], v[VEC];
+        float o[VEC], v[VEC], w[VEC];
         if (p.dy) {
 #pragma unroll
           for (int i = 0; i < VEC; ++i) e[c][i] = fmaf(-m2, zh[c][i], e[c][i]);  // Z
         }
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[i] = p.alpha * e[c][i];
-        put<VEC>(p.dx, at, o, p.x16);
-        // n, hh
-        float hh[VEC], w1[VEC];
-        hr[c].get(hh, p.h16);
+        put<VEC>(p.dx, at, o, x16);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) w1[i] = 1.f;
-        if (p.w1) {
-          weights<VEC>(p.w1, col, w1);
+        for (int i = 0; i < VEC; ++i) w[i] = 1.f, v[i] = 1.f;
+        if (p.w1) weights<VEC>(p.w1, col, w);
+        if (p.s) weights<VEC>(p.s, col, v);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) hh[i] *= r1;
+        for (int i = 0; i < VEC; ++i) {
+          const float nn = hh[c][i] * w[i], en = e[c][i] * nn;
+          const float sw = p.g ? swish(g[c][i], sg[c][i]) : 1.f;
+          as[c][i] = fmaf(en, sw, as[c][i]);
+          o[i] = p.g ? en * v[i] * swish_slope(g[c][i], sg[c][i]) : 0.f;
+          v[i] *= e[c][i] * sw;
         }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) nn[i] = hh[i] * w1[i];
-        float s[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) s[i] = 1.f;
-        if (p.s) weights<VEC>(p.s, col, s);
-        if (p.g) {
-          float gv[VEC];
-          gr[c].get(gv, p.h16);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float sw = swish(gv[i]);
-            as[c][i] = fmaf(e[c][i] * sw, nn[i], as[c][i]);
-            const float zs = e[c][i] * s[i];
-            o[i] = zs * nn[i] * swish_slope(gv[i]);
-            v[i] = zs * sw;
-          }
-          put<VEC>(p.dg, at, o, p.h16);
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            as[c][i] = fmaf(e[c][i], nn[i], as[c][i]);
-            v[i] = e[c][i] * s[i];
-          }
-        }
+        if (p.g) put<VEC>(p.dg, at, o, h16);
         if (p.w1) {
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
-            a1[c][i] = fmaf(v[i], hh[i], a1[c][i]);
-            v[i] = r1 * (v[i] * w1[i] - hh[i] * m1);
+            a1[c][i] = fmaf(v[i], hh[c][i], a1[c][i]);
+            v[i] = r1 * (v[i] * w[i] - hh[c][i] * m1);
           }
         }
-        put<VEC>(p.dh, at, v, p.h16);
+        put<VEC>(p.dh, at, v, h16);
       }
     }
   }
@@ -395,6 +417,132 @@ __global__ void __launch_bounds__(512) seam_backward_kernel(SeamParams p) {
       if (p.w1) put<VEC>(p.part, at, a1[c], false);
       if (p.s) put<VEC>(p.part, plane + at, as[c], false);
       if (p.w2) put<VEC>(p.part, 2 * plane + at, a2[c], false);
+    }
+  }
+}
+
+// Rows too wide for a thread's registers: the same in two passes over the row,
+// the second from the caches, with the column sums in shared memory, [3][d],
+// where every thread alone touches its columns.
+template <int VEC, int TX, int TH>
+__global__ void __launch_bounds__(512, 1) seam_backward_wide_kernel(SeamParams p) {
+  extern __shared__ __align__(16) float acc[];
+  __shared__ float red[96];
+  int flip = 0;
+  const int n = blockDim.x;
+  const bool x16 = is16<TX>(p.x16), h16 = is16<TH>(p.h16);
+  float *a1 = acc, *as = acc + p.d, *a2 = acc + 2 * p.d;
+  for (int col = threadIdx.x * VEC; col < p.d; col += n * VEC)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) a1[col + i] = as[col + i] = a2[col + i] = 0.f;
+  // hh, the gate's sigmoid, q and zh, e of VEC values
+  struct Values {
+    float hh[VEC], g[VEC], sg[VEC], q[VEC], zh[VEC], e[VEC], dy[VEC], t[VEC];
+  };
+  auto values = [&](int row, int col, float r1, float r2, Values &s) {
+    Raw<VEC> hr, gr, xr, dzr, dyr;
+    hr.load(p.h, row * p.ldh + col, h16);
+    if (p.g) gr.load(p.g, row * p.ldg + col, h16);
+    if (p.dz) dzr.load(p.dz, row * p.lddz + col, x16);
+    if (p.dy) {
+      dyr.load(p.dy, row * p.lddy + col, p.y16);
+      xr.load(p.x, row * p.ldx + col, x16);
+    }
+    float v[VEC];
+    hr.get(s.hh, h16);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s.q[i] = s.hh[i] *= r1;
+    if (p.w1) {
+      weights<VEC>(p.w1, col, v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s.q[i] *= v[i];
+    }
+    if (p.g) {
+      gr.get(s.g, h16);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        s.sg[i] = sigmoid(s.g[i]);
+        s.q[i] *= swish(s.g[i], s.sg[i]);
+      }
+    }
+    if (p.s) {
+      weights<VEC>(p.s, col, v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s.q[i] *= v[i];
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s.e[i] = s.zh[i] = s.t[i] = s.dy[i] = 0.f;
+    if (p.dz) dzr.get(s.e, x16);
+    if (p.dy) {
+      float w[VEC];
+      xr.get(v, x16);
+      weights<VEC>(p.w2, col, w);
+      dyr.get(s.dy, p.y16);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        s.zh[i] = fmaf(p.alpha, v[i], s.q[i]) * r2;
+        s.t[i] = s.dy[i] * w[i];
+        s.e[i] = fmaf(r2, s.t[i], s.e[i]);
+      }
+    }
+  };
+  for (int row = blockIdx.x; row < p.rows; row += p.parts) {
+    const float r1 = p.w1 ? p.stats[row] : 1.f, r2 = p.w2 ? p.stats[p.rows + row] : 1.f;
+    float sum[3] = {0.f, 0.f, 0.f};  // t zh, e q, zh q
+    for (int col = threadIdx.x * VEC; col < p.d; col += n * VEC) {
+      Values s;
+      values(row, col, r1, r2, s);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        sum[0] = fmaf(s.t[i], s.zh[i], sum[0]);
+        sum[1] = fmaf(s.e[i], s.q[i], sum[1]);
+        sum[2] = fmaf(s.zh[i], s.q[i], sum[2]);
+      }
+    }
+    row_sum(sum, false, red, flip);
+    const float m2 = r2 * (sum[0] * p.inv_d), m1 = (sum[1] - m2 * sum[2]) * p.inv_d;
+    for (int col = threadIdx.x * VEC; col < p.d; col += n * VEC) {
+      const int64_t at = (int64_t)row * p.d + col;
+      Values s;
+      values(row, col, r1, r2, s);
+      float o[VEC], v[VEC], w[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        s.e[i] = fmaf(-m2, s.zh[i], s.e[i]);  // Z
+        o[i] = p.alpha * s.e[i];
+        w[i] = v[i] = 1.f;
+      }
+      put<VEC>(p.dx, at, o, x16);
+      if (p.w1) weights<VEC>(p.w1, col, w);
+      if (p.s) weights<VEC>(p.s, col, v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float en = s.e[i] * (s.hh[i] * w[i]);
+        const float sw = p.g ? swish(s.g[i], s.sg[i]) : 1.f;
+        as[col + i] = fmaf(en, sw, as[col + i]);
+        a2[col + i] = fmaf(s.dy[i], s.zh[i], a2[col + i]);
+        o[i] = p.g ? en * v[i] * swish_slope(s.g[i], s.sg[i]) : 0.f;
+        v[i] *= s.e[i] * sw;
+      }
+      if (p.g) put<VEC>(p.dg, at, o, h16);
+      if (p.w1) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          a1[col + i] = fmaf(v[i], s.hh[i], a1[col + i]);
+          v[i] = r1 * (v[i] * w[i] - s.hh[i] * m1);
+        }
+      }
+      put<VEC>(p.dh, at, v, h16);
+    }
+  }
+  const int64_t plane = (int64_t)p.parts * p.d;
+  for (int col = threadIdx.x * VEC; col < p.d; col += n * VEC) {
+    const int64_t at = (int64_t)blockIdx.x * p.d + col;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      if (p.w1) p.part[at + i] = a1[col + i];
+      if (p.s) p.part[plane + at + i] = as[col + i];
+      if (p.w2) p.part[2 * plane + at + i] = a2[col + i];
     }
   }
 }
@@ -421,47 +569,45 @@ __global__ void __launch_bounds__(256) seam_columns_kernel(const float *part, in
 
 constexpr int kMaxWidth = 16384;
 
-// Threads of a row and values per thread for rows of d values.
+// Threads of a row and values per thread for rows of d values: one vector a
+// thread while 512 threads suffice.
 struct Shape {
   int vec, k, threads, rows_per_block;
 };
-Shape shape_of(int d, bool vec8, bool backward) {
+Shape shape_of(int d, bool vec8) {
   if (vec8) {
     const int ch = d / 8;  // 16-byte (bf16) or 32-byte (fp32) chunks
     if (ch <= 32) return {8, 1, 32, 4};
-    if (backward) {  // five tensors and three column sums per value held: one chunk per thread while it lasts
-      if (ch <= 64) return {8, 1, 64, 1};
-      if (ch <= 128) return {8, 1, 128, 1};
-      if (ch <= 256) return {8, 1, 256, 1};
-      if (ch <= 512) return {8, 1, 512, 1};
-    }
-    if (ch <= 64) return {8, 2, 32, 4};
-    if (ch <= 128) return {8, 1, 128, 1};
-    if (ch <= 256) return {8, 2, 128, 1};
-    if (ch <= 512) return {8, 2, 256, 1};
+    if (ch <= 512) return {8, 1, (ch + 31) / 32 * 32, 1};
     if (ch <= 1024) return {8, 2, 512, 1};
     return {8, 4, 512, 1};
   }
   if (d <= 128) return {1, 4, 32, 4};
-  if (d <= 512) return {1, 4, 128, 1};
-  if (d <= 1024) return {1, 8, 128, 1};
-  if (d <= 2048) return {1, 8, 256, 1};
-  if (d <= 4096) return {1, 8, 512, 1};
+  if (d <= 2048) return {1, 4, (d + 127) / 128 * 32, 1};
+  if (d <= 4096) return {1, 8, (d + 255) / 256 * 32, 1};
   if (d <= 8192) return {1, 16, 512, 1};
   return {1, 32, 512, 1};
 }
 
-template <typename F>
-void with_kernel(const Shape &s, F &&f) {
+// A backward of this shape holds its row in registers (else: two passes).
+bool held_backward(const Shape &s) { return s.k == 1 || (s.vec == 1 && s.k <= 8); }
+
+using SeamKernel = void (*)(SeamParams);
+template <int TX, int TH>
+SeamKernel vector_kernel(int k, bool backward) {
+  if (backward) return k == 1 ? seam_backward_kernel<8, 1, TX, TH> : seam_backward_wide_kernel<8, TX, TH>;
+  return k == 1 ? seam_forward_kernel<8, 1, TX, TH>
+                : k == 2 ? seam_forward_kernel<8, 2, TX, TH> : seam_forward_kernel<8, 4, TX, TH>;
+}
+SeamKernel kernel_of(const Shape &s, bool x16, bool h16, bool backward) {
   if (s.vec == 8) {
-    if (s.k == 1) return f(seam_forward_kernel<8, 1>, seam_backward_kernel<8, 1>);
-    if (s.k == 2) return f(seam_forward_kernel<8, 2>, seam_backward_kernel<8, 2>);
-    return f(seam_forward_kernel<8, 4>, seam_backward_kernel<8, 4>);
+    if (x16) return h16 ? vector_kernel<1, 1>(s.k, backward) : vector_kernel<1, 0>(s.k, backward);
+    return h16 ? vector_kernel<0, 1>(s.k, backward) : vector_kernel<0, 0>(s.k, backward);
   }
-  if (s.k == 4) return f(seam_forward_kernel<1, 4>, seam_backward_kernel<1, 4>);
-  if (s.k == 8) return f(seam_forward_kernel<1, 8>, seam_backward_kernel<1, 8>);
-  if (s.k == 16) return f(seam_forward_kernel<1, 16>, seam_backward_kernel<1, 16>);
-  return f(seam_forward_kernel<1, 32>, seam_backward_kernel<1, 32>);
+  if (s.k == 4) return backward ? seam_backward_kernel<1, 4, 2, 2> : seam_forward_kernel<1, 4, 2, 2>;
+  if (s.k == 8) return backward ? seam_backward_kernel<1, 8, 2, 2> : seam_forward_kernel<1, 8, 2, 2>;
+  if (backward) return seam_backward_wide_kernel<1, 2, 2>;
+  return s.k == 16 ? seam_forward_kernel<1, 16, 2, 2> : seam_forward_kernel<1, 32, 2, 2>;
 }
 
 // 16-byte accesses of 8 values need rows that start on 16 bytes (bf16; fp32
@@ -470,8 +616,9 @@ bool rows_aligned(const void *p, int64_t ld, int is16) {
   return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % (is16 ? 8 : 4) == 0);
 }
 
-// Row groups that share the rows of a backward: enough to fill the GPU, few
-// enough that their partial rows stay small beside the data.
+// Row groups that share the rows of a backward: about 512 threads an SM, as
+// many as its registers hold; few enough that their partial rows stay small
+// beside the data.
 int parts_of(int num_sms, int rows, const Shape &s) {
   const int per_sm = 512 / (s.threads * s.rows_per_block), blocks = num_sms * (per_sm < 1 ? 1 : per_sm);
   const int need = (rows + s.rows_per_block - 1) / s.rows_per_block;
@@ -501,11 +648,14 @@ int af_residual_norm(af_ctx *ctx, const void *x, int64_t ldx, int x_bf16, const 
   const bool vec = d % 8 == 0 && rows_aligned(x, ldx, x_bf16) && rows_aligned(h, ldh, h_bf16) &&
                    rows_aligned(gate, ldg, h_bf16) && rows_aligned(post_w, 8, 0) && rows_aligned(scale, 8, 0) &&
                    rows_aligned(pre_w, 8, 0) && rows_aligned(z, d, x_bf16) && rows_aligned(y, d, y_bf16);
-  const Shape s = shape_of(d, vec, false);
-  with_kernel(s, [&](auto fwd, auto) {
-    fwd<<<(unsigned)((rows + s.rows_per_block - 1) / s.rows_per_block), dim3(s.threads, s.rows_per_block), 0,
-          af::stream_of(stream)>>>(p);
-  });
+  const Shape s = shape_of(d, vec);
+  int64_t blocks = (rows + s.rows_per_block - 1) / s.rows_per_block;
+  if (s.vec == 8 && s.k == 1) {  // blocks that walk: 1024 threads an SM, what its registers hold
+    const int per_sm = 1024 / (s.threads * s.rows_per_block);
+    blocks = std::min<int64_t>(blocks, (int64_t)ctx->num_sms * (per_sm < 1 ? 1 : per_sm));
+  }
+  kernel_of(s, p.x16, p.h16, false)<<<(unsigned)blocks, dim3(s.threads, s.rows_per_block), 0,
+                                      af::stream_of(stream)>>>(p);
   return af::launched(ctx, fn);
 }
 
@@ -515,8 +665,8 @@ int af_residual_norm_scratch(af_ctx *ctx, int64_t rows, int d, int64_t *floats) 
   AF_ENTER(ctx, fn);
   AF_REQUIRE(floats && rows >= 0 && rows < (1ll << 31) && d > 0 && d <= kMaxWidth, "af_residual_norm_scratch",
              "bad sizes");
-  const int a = parts_of(ctx->num_sms, (int)rows, shape_of(d, false, true));
-  const int b = d % 8 == 0 ? parts_of(ctx->num_sms, (int)rows, shape_of(d, true, true)) : 0;
+  const int a = parts_of(ctx->num_sms, (int)rows, shape_of(d, false));
+  const int b = d % 8 == 0 ? parts_of(ctx->num_sms, (int)rows, shape_of(d, true)) : 0;
   *floats = 3ll * (a > b ? a : b) * d;
   return AF_OK;
 }
@@ -555,14 +705,22 @@ int af_residual_norm_backward(af_ctx *ctx, const void *dz, int64_t lddz, const v
                    rows_aligned(pre_w, 8, 0) && rows_aligned(dz, lddz, x_bf16) && rows_aligned(dy, lddy, y_bf16) &&
                    rows_aligned(dx, d, x_bf16) && rows_aligned(dh, d, h_bf16) && rows_aligned(dgate, d, h_bf16) &&
                    rows_aligned(scratch, 8, 0);
-  const Shape s = shape_of(d, vec, true);
+  const Shape s = shape_of(d, vec);
   p.parts = parts_of(ctx->num_sms, (int)rows, s);
   const bool sums = post_w || scale || pre_w;
   AF_REQUIRE(!sums || (scratch && scratch_floats >= 3ll * p.parts * d), "af_residual_norm_backward",
              "scratch of %lld floats, %lld are needed", (long long)scratch_floats, 3ll * p.parts * d);
-  with_kernel(s, [&](auto, auto bwd) {
-    bwd<<<(unsigned)(p.parts / s.rows_per_block), dim3(s.threads, s.rows_per_block), 0, st>>>(p);
-  });
+  const SeamKernel kernel = kernel_of(s, p.x16, p.h16, true);
+  size_t smem = 0;
+  if (!held_backward(s)) {
+    smem = (size_t)3 * d * sizeof(float);
+    static std::atomic<unsigned long long> attr_devices[5];
+    const int which = s.vec == 1 ? 4 : p.x16 * 2 + p.h16;
+    if (int rc = af::smem_attr(ctx, reinterpret_cast<const void *>(kernel), (size_t)3 * kMaxWidth * sizeof(float),
+                               attr_devices[which], fn))
+      return rc;
+  }
+  kernel<<<(unsigned)(p.parts / s.rows_per_block), dim3(s.threads, s.rows_per_block), smem, st>>>(p);
   if (int rc = af::launched(ctx, fn)) return rc;
   if (!sums) return AF_OK;
   seam_columns_kernel<<<dim3((unsigned)((d + 31) / 32), 3), dim3(32, 8), 0, st>>>(

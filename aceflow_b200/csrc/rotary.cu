@@ -12,24 +12,40 @@
 // reduced to [-1/2, 1/2] there, and only the remainder goes to sincospif
 // (2^-26 turns off, 1e-7 rad).
 //
-// Bound: HBM, each value read once and written once.  An angle costs two
-// 64-bit multiplies and a sincospif (about 40 instructions), so a thread keeps
-// the angles of its few pairs in registers and uses them for several heads.
+// Bound: HBM, each value read once and written once: 84 us for q and k of 8 x
+// 4096 tokens (16 heads of 256, bf16, 0.54 GB), 0.97 of the measured copy rate.
+// An angle costs two 64-bit multiplies and a sincospif (about 40
+// instructions), so a thread keeps the angles of its few pairs in registers
+// for up to 16 heads, whose first loads are under way while they are formed.
+// bf16 values are taken apart and put together two at a time: one by one the
+// conversions alone made the same call 100 us.
 #include "common.cuh"
 
+#include <algorithm>
+
 namespace {
+
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery 1994): 2^s >= d,
+// m = floor(2^32 (2^s - d) / d) + 1.
+struct Div {
+  uint32_t d, m, s;
+  void set(uint32_t by) {
+    d = by, s = 0;
+    while ((1ull << s) < by) ++s;
+    m = (uint32_t)(((1ull << 32) * ((1ull << s) - by)) / by + 1);
+  }
+  __device__ __forceinline__ uint32_t of(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
+};
 
 struct RotaryParams {
   const void *x;
   void *out;
   int64_t xb, xt, xh, ob, ot, oh;  // strides in elements: stream, token, head
-  int T, heads, dim, rot;
-  unsigned tokens;   // streams * T
-  unsigned cols;     // column groups per head
-  unsigned items;    // (head slot, column group) pairs per token
-  int per_thread;    // heads a thread turns
-  unsigned slots;    // ceil(heads / per_thread)
-  unsigned block_tokens;
+  int heads, dim, rot;
+  unsigned tokens;        // streams * T
+  Div T, cols, items;     // tokens of a stream, column groups of a head, (heads' slot, column group) items of a token
+  unsigned block_tokens;  // tokens of a block
+  int slot_heads;         // heads of a slot
   const float *inv_freq;
   const void *pos;  // int32 or int64, or NULL: start + t
   int pos64;
@@ -38,21 +54,47 @@ struct RotaryParams {
   int inverse;
 };
 
+// W values of one access, and as fp32.
 template <typename T, int W>
 struct alignas(sizeof(T) * W) Pack {
   T v[W];
 };
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f(float v);
-template <>
-__device__ __forceinline__ float from_f<float>(float v) {
-  return v;
+template <int W>
+__device__ __forceinline__ void unpack(const Pack<float, W> &p, float (&f)[W]) {
+#pragma unroll
+  for (int i = 0; i < W; ++i) f[i] = p.v[i];
 }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
-  return __float2bfloat16(v);
+template <int W>
+__device__ __forceinline__ void unpack(const Pack<__nv_bfloat16, W> &p, float (&f)[W]) {
+  if constexpr (W == 1) {
+    f[0] = __bfloat162float(p.v[0]);
+  } else {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&p);
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+template <int W>
+__device__ __forceinline__ Pack<float, W> packed(const float (&f)[W], float) {
+  Pack<float, W> p;
+#pragma unroll
+  for (int i = 0; i < W; ++i) p.v[i] = f[i];
+  return p;
+}
+template <int W>
+__device__ __forceinline__ Pack<__nv_bfloat16, W> packed(const float (&f)[W], __nv_bfloat16) {
+  Pack<__nv_bfloat16, W> p;
+  if constexpr (W == 1) {
+    p.v[0] = __float2bfloat16(f[0]);
+  } else {
+    __nv_bfloat162 *w = reinterpret_cast<__nv_bfloat162 *>(&p);
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) w[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+  }
+  return p;
 }
 
 __device__ __forceinline__ double position_of(const RotaryParams &p, unsigned b, unsigned t) {
@@ -62,112 +104,124 @@ __device__ __forceinline__ double position_of(const RotaryParams &p, unsigned b,
 }
 
 // cos and sin (times the scale) of pair i at this position.
-__device__ __forceinline__ void angle(const RotaryParams &p, double pos, int i, float &c, float &s) {
+__device__ __forceinline__ float2 angle(const RotaryParams &p, double pos, int i) {
   const double turns = pos * ((double)p.inv_freq[i] * 0.15915494309189535);
   const float r = (float)(turns - rint(turns));
+  float c, s;
   sincospif(2.0f * r, &s, &c);
-  c *= p.scale;
-  s *= p.inverse ? -p.scale : p.scale;
+  return make_float2(c * p.scale, s * (p.inverse ? -p.scale : p.scale));
 }
 
 constexpr int kThreads = 256;
-constexpr int kFlight = 4;  // heads whose loads a thread has in flight
+constexpr int kHeads = 16;  // heads that share one thread's angles at most
 
 // W: values per access.  HALF: pairs (i, i + rot/2), a column group is W
 // pairs, then groups of W values behind the turned part; else pairs
 // (2i, 2i + 1), a column group is max(W, 2) values of the head.
 template <typename T, int W, bool HALF>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
+__global__ void __launch_bounds__(kThreads, 3) rotary_kernel(RotaryParams p) {
   constexpr int G = HALF ? W : (W < 2 ? 2 : W);  // values of one access group
   constexpr int N = HALF ? W : G / 2;            // pairs a thread turns
   constexpr int A = G / W;                       // accesses per group (2 for scalar interleaved pairs)
+  constexpr int kFlight = HALF ? 2 : 4;        // heads whose loads (two each with HALF) a thread has in flight
   using V = Pack<T, W>;
   const unsigned token0 = blockIdx.x * p.block_tokens;
   const unsigned ntok = min(p.block_tokens, p.tokens - token0);
-  const T *xin = static_cast<const T *>(p.x);
+  const T *x = static_cast<const T *>(p.x);
   T *out = static_cast<T *>(p.out);
   const int half = p.rot / 2;
-  for (unsigned it = threadIdx.x; it < ntok * p.items; it += kThreads) {
-    const unsigned tl = it / p.items, rem = it - tl * p.items;
-    const unsigned slot = rem / p.cols, col = rem - slot * p.cols;
-    const unsigned token = token0 + tl, b = token / (unsigned)p.T, t = token - b * (unsigned)p.T;
-    const T *xr = xin + (int64_t)b * p.xb + (int64_t)t * p.xt;
-    T *orow = out + (int64_t)b * p.ob + (int64_t)t * p.ot;
-    // where the group lies in a head, and the angles of its pairs
-    int first, second = 0, turned;
+  for (unsigned it = blockIdx.y * kThreads + threadIdx.x; it < ntok * p.items.d; it += gridDim.y * kThreads) {
+    const unsigned tl = p.items.of(it), rem = it - tl * p.items.d, slot = p.cols.of(rem);
+    const int col = (int)(rem - slot * p.cols.d);
+    const unsigned token = token0 + tl, b = p.T.of(token), t = token - b * p.T.d;
+    // where the group lies in a head, and how many of its pairs turn
+    int first, turned;
     if (HALF) {
       const int groups = half / W;
-      turned = (int)col < groups ? N : 0;
-      first = turned ? (int)col * W : p.rot + ((int)col - groups) * W;
-      second = first + half;
+      turned = col < groups ? N : 0;
+      first = col < groups ? col * W : p.rot + (col - groups) * W;
     } else {
-      first = (int)col * G;
+      first = col * G;
       turned = min(max((p.rot - first) / 2, 0), N);
     }
-    float c[N], s[N];
-    if (turned) {
-      const double pos = position_of(p, b, t);
-      const int i0 = HALF ? first : first / 2;
+    int h = (int)slot * p.slot_heads;
+    const int h_end = min(h + p.slot_heads, p.heads);
+    const T *src = x + ((int64_t)b * p.xb + (int64_t)t * p.xt + (int64_t)h * p.xh + first);
+    T *dst = out + ((int64_t)b * p.ob + (int64_t)t * p.ot + (int64_t)h * p.oh + first);
+    V va[kFlight][A], vb[kFlight];
+    auto fetch = [&]() {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (i < turned) angle(p, pos, i0 + i, c[i], s[i]);
-    }
-    const int h_end = min((int)(slot + 1) * p.per_thread, p.heads);
-    for (int h0 = (int)slot * p.per_thread; h0 < h_end; h0 += kFlight) {
-      V va[kFlight][A], vb[kFlight];
-#pragma unroll
-      for (int j = 0; j < kFlight; ++j) {
-        if (h0 + j < h_end) {
-          const T *src = xr + (int64_t)(h0 + j) * p.xh;
+      for (int j = 0; j < kFlight; ++j)
+        if (h + j < h_end) {
+          const T *s = src + (int64_t)j * p.xh;
 #pragma unroll
           for (int a = 0; a < A; ++a)
-            if (first + a * W < p.dim) va[j][a] = *reinterpret_cast<const V *>(src + first + a * W);
-          if (HALF && turned) vb[j] = *reinterpret_cast<const V *>(src + second);
+            if (W > 1 || first + a < p.dim) va[j][a] = *reinterpret_cast<const V *>(s + a * W);
+          if (HALF && turned) vb[j] = *reinterpret_cast<const V *>(s + half);
         }
-      }
+    };
+    fetch();  // under way while the angles are formed
+    float2 cs[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) cs[i] = make_float2(1.f, 0.f);
+    if (turned) {
+      const double pos = position_of(p, b, t);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < turned) cs[i] = angle(p, pos, (HALF ? first : first / 2) + i);
+    }
+    for (;;) {
 #pragma unroll
       for (int j = 0; j < kFlight; ++j) {
-        if (h0 + j < h_end) {
-          T *dst = orow + (int64_t)(h0 + j) * p.oh;
-          if (HALF) {
-            if (turned) {
+        if (h + j < h_end) {
+          T *d = dst + (int64_t)j * p.oh;
+          if (HALF && turned) {
+            float a[W], bb[W], u[W], v[W];
+            unpack(va[j][0], a);
+            unpack(vb[j], bb);
 #pragma unroll
-              for (int i = 0; i < N; ++i) {
-                const float a = to_f(va[j][0].v[i]), bb = to_f(vb[j].v[i]);
-                va[j][0].v[i] = from_f<T>(a * c[i] - bb * s[i]);
-                vb[j].v[i] = from_f<T>(a * s[i] + bb * c[i]);
-              }
-              *reinterpret_cast<V *>(dst + second) = vb[j];
+            for (int i = 0; i < W; ++i) {
+              u[i] = a[i] * cs[i].x - bb[i] * cs[i].y;
+              v[i] = a[i] * cs[i].y + bb[i] * cs[i].x;
             }
-            *reinterpret_cast<V *>(dst + first) = va[j][0];
-          } else {
+            va[j][0] = packed(u, T());
+            *reinterpret_cast<V *>(d + half) = packed(v, T());
+          } else if (!HALF && turned) {
+            float f[A][W];
+#pragma unroll
+            for (int a = 0; a < A; ++a) unpack(va[j][a], f[a]);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-              T &ra = va[j][(2 * i) / W].v[(2 * i) % W];
-              T &rb = va[j][(2 * i + 1) / W].v[(2 * i + 1) % W];
-              if (i < turned) {
-                const float a = to_f(ra), bb = to_f(rb);
-                ra = from_f<T>(a * c[i] - bb * s[i]);
-                rb = from_f<T>(a * s[i] + bb * c[i]);
+              float &ra = f[(2 * i) / W][(2 * i) % W], &rb = f[(2 * i + 1) / W][(2 * i + 1) % W];
+              const float a = ra, bb = rb;
+              if (N == 1 || i < turned) {  // behind the turned part values are copied
+                ra = a * cs[i].x - bb * cs[i].y;
+                rb = a * cs[i].y + bb * cs[i].x;
               }
             }
 #pragma unroll
-            for (int a = 0; a < A; ++a)
-              if (first + a * W < p.dim) *reinterpret_cast<V *>(dst + first + a * W) = va[j][a];
+            for (int a = 0; a < A; ++a) va[j][a] = packed(f[a], T());
           }
+#pragma unroll
+          for (int a = 0; a < A; ++a)
+            if (W > 1 || first + a < p.dim) *reinterpret_cast<V *>(d + a * W) = va[j][a];
         }
       }
+      h += kFlight;
+      if (h >= h_end) break;
+      src += kFlight * p.xh;
+      dst += kFlight * p.oh;
+      fetch();
     }
   }
 }
 
 template <typename T, int W>
-cudaError_t launch(const RotaryParams &p, bool half, unsigned blocks, cudaStream_t st) {
+void launch(const RotaryParams &p, bool half, dim3 grid, cudaStream_t st) {
   if (half)
-    rotary_kernel<T, W, true><<<blocks, kThreads, 0, st>>>(p);
+    rotary_kernel<T, W, true><<<grid, kThreads, 0, st>>>(p);
   else
-    rotary_kernel<T, W, false><<<blocks, kThreads, 0, st>>>(p);
-  return cudaSuccess;
+    rotary_kernel<T, W, false><<<grid, kThreads, 0, st>>>(p);
 }
 
 }  // namespace
@@ -201,35 +255,38 @@ extern "C" int af_rotary(af_ctx *ctx, const void *x, void *out, int is_bf16, con
   p.x = x, p.out = out;
   p.xb = x_strides[0], p.xt = x_strides[1], p.xh = x_strides[2];
   p.ob = out_strides[0], p.ot = out_strides[1], p.oh = out_strides[2];
-  p.T = T, p.heads = heads, p.dim = head_dim, p.rot = rot_dim;
+  p.heads = heads, p.dim = head_dim, p.rot = rot_dim;
   p.tokens = (unsigned)((int64_t)batch * T);
   const int G = interleaved && W < 2 ? 2 : W;
-  p.cols = interleaved ? (unsigned)((head_dim + G - 1) / G) : (unsigned)(rot_dim / 2 / W + (head_dim - rot_dim) / W);
-  // Heads per thread: 8 share one thread's angles once that still leaves every
-  // SM a full set of threads; a short call rather spreads over the SMs.
+  const int cols = interleaved ? (head_dim + G - 1) / G : rot_dim / 2 / W + (head_dim - rot_dim) / W;
+  // Heads per thread: up to 16 share one thread's angles, fewer while that
+  // leaves an SM less than a full set of threads (8 x 4096 tokens of 16 heads of
+  // 256: 84 us with 16, 90 with 8); then evenly over the threads of a token.
   const int64_t fill = (int64_t)ctx->num_sms * 2048;
-  p.per_thread = 8;
-  while (p.per_thread > 1 && (int64_t)p.tokens * p.cols * ((heads + p.per_thread - 1) / p.per_thread) < fill)
-    p.per_thread /= 2;
-  p.slots = (unsigned)((heads + p.per_thread - 1) / p.per_thread);
-  AF_REQUIRE((int64_t)p.slots * p.cols < (1 << 24), "af_rotary", "heads * head_dim is too large");
-  p.items = p.slots * p.cols;
-  p.block_tokens = p.items >= kThreads ? 1 : kThreads / p.items;
+  int share = kHeads;
+  while (share > 1 && (int64_t)p.tokens * cols * ((heads + share - 1) / share) < fill) share /= 2;
+  const int slots = (heads + share - 1) / share;
+  p.slot_heads = (heads + slots - 1) / slots;
+  AF_REQUIRE((int64_t)slots * cols < (1 << 24), "af_rotary", "heads * head_dim is too large");
+  p.block_tokens = slots * cols >= kThreads ? 1 : kThreads / (slots * cols);
+  p.T.set((uint32_t)T), p.cols.set((uint32_t)cols), p.items.set((uint32_t)(slots * cols));
   p.inv_freq = inv_freq, p.pos = positions, p.pos64 = positions_i64;
   p.pb = positions ? pos_strides[0] : 0, p.pt = positions ? pos_strides[1] : 0;
   p.start = start, p.scale = scale, p.inverse = inverse;
-  const unsigned blocks = (p.tokens + p.block_tokens - 1) / p.block_tokens;
-  cudaStream_t st = af::stream_of(stream);
+  const dim3 grid((p.tokens + p.block_tokens - 1) / p.block_tokens,
+                  std::min((slots * cols + kThreads - 1) / kThreads, 65535));
+  const cudaStream_t st = af::stream_of(stream);
+  const bool half = !interleaved;
   if (is_bf16) {
     using B16 = __nv_bfloat16;
-    W == 8   ? launch<B16, 8>(p, !interleaved, blocks, st)
-    : W == 4 ? launch<B16, 4>(p, !interleaved, blocks, st)
-    : W == 2 ? launch<B16, 2>(p, !interleaved, blocks, st)
-             : launch<B16, 1>(p, !interleaved, blocks, st);
+    W == 8   ? launch<B16, 8>(p, half, grid, st)
+    : W == 4 ? launch<B16, 4>(p, half, grid, st)
+    : W == 2 ? launch<B16, 2>(p, half, grid, st)
+             : launch<B16, 1>(p, half, grid, st);
   } else {
-    W == 4   ? launch<float, 4>(p, !interleaved, blocks, st)
-    : W == 2 ? launch<float, 2>(p, !interleaved, blocks, st)
-             : launch<float, 1>(p, !interleaved, blocks, st);
+    W == 4   ? launch<float, 4>(p, half, grid, st)
+    : W == 2 ? launch<float, 2>(p, half, grid, st)
+             : launch<float, 1>(p, half, grid, st);
   }
   return af::launched(ctx, fn);
 }
