@@ -126,16 +126,22 @@ __device__ __forceinline__ void weights(const float *w, int col, float (&v)[VEC]
 // The sigmoid with the hardware's exponential and reciprocal: 2^-21 of itself
 // off (4 times that at |g| = 16), against 2^-9 of a bf16 result; with expf and
 // an IEEE division the forward spent half its instructions here.
-__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
-// swish(g) = g sigmoid(g) and its derivative, with their limit 0 at -inf.
-__device__ __forceinline__ float swish(float g, float sg) { return sg > 0.f || g != g ? g * sg : 0.f; }
+__device__ __forceinline__ float sigmoid(float g) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
+}
+// swish(g) = g sigmoid(g) and its derivative; at -inf (where sg is 0) their limit 0.
+__device__ __forceinline__ float swish(float g, float sg) { return fmaxf(g, -3.0e38f) * sg; }
 __device__ __forceinline__ float swish_slope(float g, float sg) {
-  return sg > 0.f || g != g ? sg * (1.f + g * (1.f - sg)) : 0.f;
+  return fmaf(swish(g, sg), 1.f - sg, sg);
 }
 
+constexpr int kRed = 2 * 3 * 16;
 // Sums of n values over the row's threads: a warp (one_warp) or the block.
-// `red` holds 2 x 3 x 16 floats; `flip` alternates its halves, so one barrier
-// per sum is enough.
+// `red` holds 2 x 3 x 16 floats, those of absent warps 0; `flip` alternates its
+// halves, so one barrier per sum is enough.
 template <int NV>
 __device__ __forceinline__ void row_sum(float (&v)[NV], bool one_warp, float *red, int &flip) {
 #pragma unroll
@@ -143,18 +149,27 @@ __device__ __forceinline__ void row_sum(float (&v)[NV], bool one_warp, float *re
   if (one_warp) return;
   float *r = red + flip * 48;
   flip ^= 1;
-  const int nw = blockDim.x >> 5, w = threadIdx.x >> 5;
   if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) r[i * 16 + w] = v[i];
+    for (int i = 0; i < NV; ++i) r[i * 16 + (threadIdx.x >> 5)] = v[i];
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    float t = 0.f;
-    for (int k = 0; k < nw; ++k) t += r[i * 16 + k];
-    v[i] = t;
+    const float4 *q = reinterpret_cast<const float4 *>(r + i * 16);
+    float4 a = q[0], b = q[1];
+    if (blockDim.x > 256) {
+      const float4 c = q[2], d = q[3];
+      a.x += c.x, a.y += c.y, a.z += c.z, a.w += c.w;
+      b.x += d.x, b.y += d.y, b.z += d.z, b.w += d.w;
+    }
+    v[i] = ((a.x + b.x) + (a.y + b.y)) + ((a.z + b.z) + (a.w + b.w));
   }
+}
+__device__ __forceinline__ void clear_red(float *red) {
+  const int t = threadIdx.y * blockDim.x + threadIdx.x;
+  for (int i = t; i < kRed; i += blockDim.x * blockDim.y) red[i] = 0.f;
+  __syncthreads();
 }
 
 // A type that the kernel was compiled for (0: fp32, 1: bf16) or that comes with the call (2).
@@ -169,10 +184,11 @@ __device__ __forceinline__ bool is16(int flag) {
 // registers while a block walks over rows, and a row's loads are under way
 // while the row before it is summed.
 template <int VEC, int K, int TX, int TH>
-__global__ void __launch_bounds__(512) seam_forward_kernel(SeamParams p) {
+__global__ void __launch_bounds__(512, VEC == 8 && K == 1 ? 2 : 1) seam_forward_kernel(SeamParams p) {
   constexpr bool kAhead = VEC == 8 && K == 1;
-  __shared__ float red[96];
+  __shared__ __align__(16) float red[kRed];
   int flip = 0;
+  clear_red(red);
   const int n = blockDim.x;
   const bool one_warp = n == 32, x16 = is16<TX>(p.x16), h16 = is16<TH>(p.h16);
   const int step = gridDim.x * blockDim.y;
@@ -283,8 +299,9 @@ __global__ void __launch_bounds__(512) seam_forward_kernel(SeamParams p) {
 template <int VEC, int K, int TX, int TH>
 __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
   constexpr bool kAhead = VEC == 8 && K == 1;
-  __shared__ float red[96];
+  __shared__ __align__(16) float red[kRed];
   int flip = 0;
+  clear_red(red);
   const int n = blockDim.x;
   const bool one_warp = n == 32, x16 = is16<TX>(p.x16), h16 = is16<TH>(p.h16);
   float a1[K][VEC], as[K][VEC], a2[K][VEC];  // this thread's columns of dw1, ds, dw2
@@ -427,8 +444,9 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
 template <int VEC, int TX, int TH>
 __global__ void __launch_bounds__(512, 1) seam_backward_wide_kernel(SeamParams p) {
   extern __shared__ __align__(16) float acc[];
-  __shared__ float red[96];
+  __shared__ __align__(16) float red[kRed];
   int flip = 0;
+  clear_red(red);
   const int n = blockDim.x;
   const bool x16 = is16<TX>(p.x16), h16 = is16<TH>(p.h16);
   float *a1 = acc, *as = acc + p.d, *a2 = acc + 2 * p.d;
