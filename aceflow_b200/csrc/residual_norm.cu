@@ -123,6 +123,82 @@ __device__ __forceinline__ void weights(const float *w, int col, float (&v)[VEC]
   }
 }
 
+// Arithmetic on VEC values: eight go two to an instruction (fma.rn.f32x2), which
+// halves what the kernels, bound by issue before it, spend on sums and products.
+__device__ __forceinline__ void mul_pair(float &ox, float &oy, float ax, float ay, float bx, float by) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(ox), "=f"(oy)
+      : "f"(ax), "f"(ay), "f"(bx), "f"(by));
+}
+__device__ __forceinline__ void fma_pair(float &ox, float &oy, float ax, float ay, float bx, float by, float cx,
+                                         float cy) {
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(ox), "=f"(oy)
+      : "f"(ax), "f"(ay), "f"(bx), "f"(by), "f"(cx), "f"(cy));
+}
+// o = a b
+template <int VEC>
+__device__ __forceinline__ void mul(float (&o)[VEC], const float (&a)[VEC], const float (&b)[VEC]) {
+  if constexpr (VEC == 1) {
+    o[0] = a[0] * b[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) mul_pair(o[i], o[i + 1], a[i], a[i + 1], b[i], b[i + 1]);
+  }
+}
+// o = a s
+template <int VEC>
+__device__ __forceinline__ void mul(float (&o)[VEC], const float (&a)[VEC], float s) {
+  if constexpr (VEC == 1) {
+    o[0] = a[0] * s;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) mul_pair(o[i], o[i + 1], a[i], a[i + 1], s, s);
+  }
+}
+// o = a b + c
+template <int VEC>
+__device__ __forceinline__ void fma(float (&o)[VEC], const float (&a)[VEC], const float (&b)[VEC],
+                                    const float (&c)[VEC]) {
+  if constexpr (VEC == 1) {
+    o[0] = fmaf(a[0], b[0], c[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) fma_pair(o[i], o[i + 1], a[i], a[i + 1], b[i], b[i + 1], c[i], c[i + 1]);
+  }
+}
+// o = a s + c
+template <int VEC>
+__device__ __forceinline__ void fma(float (&o)[VEC], const float (&a)[VEC], float s, const float (&c)[VEC]) {
+  if constexpr (VEC == 1) {
+    o[0] = fmaf(a[0], s, c[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) fma_pair(o[i], o[i + 1], a[i], a[i + 1], s, s, c[i], c[i + 1]);
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void fill(float (&o)[VEC], float s) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) o[i] = s;
+}
+// A running sum of products, in two halves.
+struct Dot {
+  float x = 0.f, y = 0.f;
+  template <int VEC>
+  __device__ __forceinline__ void add(const float (&a)[VEC], const float (&b)[VEC]) {
+    if constexpr (VEC == 1) {
+      x = fmaf(a[0], b[0], x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; i += 2) fma_pair(x, y, a[i], a[i + 1], b[i], b[i + 1], x, y);
+    }
+  }
+  __device__ __forceinline__ float sum() const { return x + y; }
+};
+
 // The sigmoid with the hardware's exponential and reciprocal: 2^-21 of itself
 // off (4 times that at |g| = 16), against 2^-9 of a bf16 result; with expf and
 // an IEEE division the forward spent half its instructions here.
@@ -136,6 +212,19 @@ __device__ __forceinline__ float sigmoid(float g) {
 __device__ __forceinline__ float swish(float g, float sg) { return fmaxf(g, -3.0e38f) * sg; }
 __device__ __forceinline__ float swish_slope(float g, float sg) {
   return fmaf(swish(g, sg), 1.f - sg, sg);
+}
+
+// sg = sigmoid(g), o = o swish(g)
+template <int VEC>
+__device__ __forceinline__ void gate_by(float (&o)[VEC], const float (&g)[VEC], float (&sg)[VEC]) {
+  float w[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    sg[i] = sigmoid(g[i]);
+    w[i] = fmaxf(g[i], -3.0e38f);
+  }
+  mul(w, w, sg);
+  mul(o, o, w);
 }
 
 constexpr int kRed = 2 * 3 * 16;
@@ -220,72 +309,71 @@ __global__ void __launch_bounds__(512, VEC == 8 && K == 1 ? 2 : 1) seam_forward_
   for (; row < p.rows; row += step) {  // a block's threads leave together where they share a row
     if (!kAhead) fetch(row);
     float z[K][VEC], x[K][VEC];
-    float sq[1] = {0.f};
+    Dot dot;
 #pragma unroll
     for (int c = 0; c < K; ++c) {
       const int col = (c * n + (int)threadIdx.x) * VEC;
       if (col < p.d) {
         hr[c].get(z[c], h16);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) sq[0] = fmaf(z[c][i], z[c][i], sq[0]);
+        dot.add(z[c], z[c]);
         // all of n but r1
         if (p.g) {
-          float v[VEC];
+          float v[VEC], sg[VEC];
           gr[c].get(v, h16);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) z[c][i] *= swish(v[i], sigmoid(v[i]));
+          gate_by(z[c], v, sg);
         }
         if (kAhead) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) z[c][i] *= kept[0][i];
+          mul(z[c], z[c], kept[0]);
         } else {
           float v[VEC];
           if (p.w1) {
             weights<VEC>(p.w1, col, v);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) z[c][i] *= v[i];
+            mul(z[c], z[c], v);
           }
           if (p.s) {
             weights<VEC>(p.s, col, v);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) z[c][i] *= v[i];
+            mul(z[c], z[c], v);
           }
         }
         xr[c].get(x[c], x16);
+        mul(x[c], x[c], p.alpha);
       }
     }
     if (kAhead && row + step < p.rows) fetch(row + step);
     float r1 = 1.f;
     if (p.w1) {
+      float sq[1] = {dot.sum()};
       row_sum(sq, one_warp, red, flip);
       r1 = 1.0f / sqrtf(sq[0] * p.inv_d + p.eps);
     }
-    float sz[1] = {0.f};
+    Dot dz;
 #pragma unroll
     for (int c = 0; c < K; ++c) {
       const int col = (c * n + (int)threadIdx.x) * VEC;
       if (col < p.d) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          z[c][i] = fmaf(p.alpha, x[c][i], z[c][i] * r1);
-          sz[0] = fmaf(z[c][i], z[c][i], sz[0]);
-        }
+        fma(z[c], z[c], r1, x[c]);
+        dz.add(z[c], z[c]);
         put<VEC>(p.z, (int64_t)row * p.d + col, z[c], x16);
       }
     }
     float r2 = 1.f;
     if (p.w2) {
+      float sz[1] = {dz.sum()};
       row_sum(sz, one_warp, red, flip);
       r2 = 1.0f / sqrtf(sz[0] * p.inv_d + p.eps);
 #pragma unroll
       for (int c = 0; c < K; ++c) {
         const int col = (c * n + (int)threadIdx.x) * VEC;
         if (col < p.d) {
-          float v[VEC];
-          if (!kAhead) weights<VEC>(p.w2, col, v);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) v[i] = z[c][i] * r2 * (kAhead ? kept[2][i] : v[i]);
-          put<VEC>(p.y, (int64_t)row * p.d + col, v, p.y16);
+          mul(z[c], z[c], r2);
+          if (kAhead) {
+            mul(z[c], z[c], kept[2]);
+          } else {
+            float v[VEC];
+            weights<VEC>(p.w2, col, v);
+            mul(z[c], z[c], v);
+          }
+          put<VEC>(p.y, (int64_t)row * p.d + col, z[c], p.y16);
         }
       }
     }
@@ -331,7 +419,7 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
     if (!kAhead) fetch(row);
     const float r1 = p.w1 ? p.stats[row] : 1.f, r2 = p.w2 ? p.stats[p.rows + row] : 1.f;
     // hh (h without post_w), the gate, q = s swish w1 hh, zh, e = dz + r2 t and the three sums
-    float sum[3] = {0.f, 0.f, 0.f};  // t zh, e q, zh q
+    Dot tz, eq, zq;  // t zh, e q, zh q
     float hh[K][VEC], g[K][VEC], sg[K][VEC], zh[K][VEC], e[K][VEC];
 #pragma unroll
     for (int c = 0; c < K; ++c) {
@@ -339,52 +427,42 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
       if (col < p.d) {
         float q[VEC], v[VEC];
         hr[c].get(hh[c], h16);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) q[i] = hh[c][i] *= r1;
-        if (p.w1) {
+        mul(hh[c], hh[c], r1);
+        if (p.w1)
           weights<VEC>(p.w1, col, v);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) q[i] *= v[i];
-        }
+        else
+          fill(v, 1.f);
+        mul(q, hh[c], v);
         if (p.g) {
           gr[c].get(g[c], h16);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            sg[c][i] = sigmoid(g[c][i]);
-            q[i] *= swish(g[c][i], sg[c][i]);
-          }
+          gate_by(q, g[c], sg[c]);
         }
         if (p.s) {
           weights<VEC>(p.s, col, v);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) q[i] *= v[i];
+          mul(q, q, v);
         }
-        if (p.dz) {
+        if (p.dz)
           dzr[c].get(e[c], x16);
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) e[c][i] = 0.f;
-        }
+        else
+          fill(e[c], 0.f);
         if (p.dy) {
           float w[VEC], dy[VEC];
           xr[c].get(v, x16);
           weights<VEC>(p.w2, col, w);
           dyr[c].get(dy, p.y16);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            zh[c][i] = fmaf(p.alpha, v[i], q[i]) * r2;
-            a2[c][i] = fmaf(dy[i], zh[c][i], a2[c][i]);
-            const float t = dy[i] * w[i];
-            sum[0] = fmaf(t, zh[c][i], sum[0]);
-            e[c][i] = fmaf(r2, t, e[c][i]);
-            sum[2] = fmaf(zh[c][i], q[i], sum[2]);
-          }
+          fma(zh[c], v, p.alpha, q);
+          mul(zh[c], zh[c], r2);
+          fma(a2[c], dy, zh[c], a2[c]);
+          mul(dy, dy, w);  // t
+          tz.add(dy, zh[c]);
+          fma(e[c], dy, r2, e[c]);
+          zq.add(zh[c], q);
         }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) sum[1] = fmaf(e[c][i], q[i], sum[1]);
+        eq.add(e[c], q);
       }
     }
     if (kAhead && row + p.parts < p.rows) fetch(row + p.parts);
+    float sum[3] = {tz.sum(), eq.sum(), zq.sum()};
     if (p.w1 || p.dy) row_sum(sum, one_warp, red, flip);
     const float m2 = p.dy ? r2 * (sum[0] * p.inv_d) : 0.f;  // r2 mean(t zh)
     const float m1 = (sum[1] - m2 * sum[2]) * p.inv_d;       // mean(N w1 hh)
@@ -394,32 +472,47 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
       if (col < p.d) {
         const int64_t at = (int64_t)row * p.d + col;
         float o[VEC], v[VEC], w[VEC];
-        if (p.dy) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) e[c][i] = fmaf(-m2, zh[c][i], e[c][i]);  // Z
-        }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = p.alpha * e[c][i];
+        if (p.dy) fma(e[c], zh[c], -m2, e[c]);  // Z
+        mul(o, e[c], p.alpha);
         put<VEC>(p.dx, at, o, x16);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) w[i] = 1.f, v[i] = 1.f;
-        if (p.w1) weights<VEC>(p.w1, col, w);
-        if (p.s) weights<VEC>(p.s, col, v);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float nn = hh[c][i] * w[i], en = e[c][i] * nn;
-          const float sw = p.g ? swish(g[c][i], sg[c][i]) : 1.f;
-          as[c][i] = fmaf(en, sw, as[c][i]);
-          o[i] = p.g ? en * v[i] * swish_slope(g[c][i], sg[c][i]) : 0.f;
-          v[i] *= e[c][i] * sw;
-        }
-        if (p.g) put<VEC>(p.dg, at, o, h16);
-        if (p.w1) {
+        if (p.s)
+          weights<VEC>(p.s, col, v);
+        else
+          fill(v, 1.f);
+        if (p.w1)
+          weights<VEC>(p.w1, col, w);
+        else
+          fill(w, 1.f);
+        mul(o, e[c], hh[c]);
+        mul(o, o, w);  // Z n
+        mul(v, v, e[c]);  // Z s
+        if (p.g) {
+          float sw[VEC], sl[VEC];
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
-            a1[c][i] = fmaf(v[i], hh[c][i], a1[c][i]);
-            v[i] = r1 * (v[i] * w[i] - hh[c][i] * m1);
+            sw[i] = fmaxf(g[c][i], -3.0e38f);
+            sl[i] = 1.f - sg[c][i];
           }
+          mul(sw, sw, sg[c]);
+          fma(as[c], o, sw, as[c]);
+          fma(sl, sw, sl, sg[c]);  // swish'
+          if (p.s) {
+            float s[VEC];
+            weights<VEC>(p.s, col, s);
+            mul(o, o, s);
+          }
+          mul(o, o, sl);
+          put<VEC>(p.dg, at, o, h16);
+          mul(v, v, sw);  // N
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) as[c][i] += o[i];
+        }
+        if (p.w1) {
+          fma(a1[c], v, hh[c], a1[c]);
+          mul(v, v, w);
+          fma(v, hh[c], -m1, v);
+          mul(v, v, r1);
         }
         put<VEC>(p.dh, at, v, h16);
       }
