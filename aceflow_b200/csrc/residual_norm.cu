@@ -13,7 +13,7 @@
 // Backward, from dz and dy: with zh = z r2, hh = h r1, t = dy w2,
 //     Z  = dz + r2 (t - zh mean(t zh))                  dx = alpha Z
 //     dw2 = sum dy zh,  ds = sum Z swish(g) n,  dg = Z s n swish'(g)
-//     N  = Z s swish(g),  dw1 = sum N hh
+//     N  = Z s swish(g),  dw1 = sum N hh  (= s A,  ds = w1 A,  A = sum Z swish(g) hh)
 //     dh = r1 (N w1 - hh mean(N w1 hh))
 // mean(N w1 hh) needs Z, which needs the other mean.  Both come from one
 // reduction of three sums: with q = s swish(g) w1 hh,
@@ -45,7 +45,7 @@ struct SeamParams {
   const void *dz, *dy;  // either may be NULL (zero)
   int64_t lddz, lddy;
   void *dx, *dh, *dg;
-  float *part;  // [3][parts][d]: dw1, ds, dw2
+  float *part;  // [2][parts][d]: sum Z swish(g) hh, sum dy zh
   int parts;
 };
 
@@ -384,6 +384,18 @@ __global__ void __launch_bounds__(512, VEC == 8 && K == 1 ? 2 : 1) seam_forward_
   }
 }
 
+// post_w scale (what is not given counts as 1) of VEC columns.
+template <int VEC>
+__device__ __forceinline__ void both_weights(const SeamParams &p, int col, float (&v)[VEC]) {
+  fill(v, 1.f);
+  if (p.w1) weights<VEC>(p.w1, col, v);
+  if (p.s) {
+    float s[VEC];
+    weights<VEC>(p.s, col, s);
+    mul(v, v, s);
+  }
+}
+
 template <int VEC, int K, int TX, int TH>
 __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
   constexpr bool kAhead = VEC == 8 && K == 1;
@@ -392,11 +404,15 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
   clear_red(red);
   const int n = blockDim.x;
   const bool one_warp = n == 32, x16 = is16<TX>(p.x16), h16 = is16<TH>(p.h16);
-  float a1[K][VEC], as[K][VEC], a2[K][VEC];  // this thread's columns of dw1, ds, dw2
+  float a1[K][VEC], a2[K][VEC];  // this thread's columns of sum Z swish hh and of dw2
 #pragma unroll
-  for (int c = 0; c < K; ++c)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) a1[c][i] = as[c][i] = a2[c][i] = 0.f;
+  for (int c = 0; c < K; ++c) fill(a1[c], 0.f), fill(a2[c], 0.f);
+  float kept1[VEC], kept2[VEC];  // with kAhead: post_w scale, pre_w
+  if (kAhead && (int)threadIdx.x * VEC < p.d) {
+    both_weights<VEC>(p, (int)threadIdx.x * VEC, kept1);
+    fill(kept2, 0.f);
+    if (p.w2) weights<VEC>(p.w2, (int)threadIdx.x * VEC, kept2);
+  }
   Raw<VEC> hr[K], gr[K], xr[K], dzr[K], dyr[K];
   auto fetch = [&](int row) {
 #pragma unroll
@@ -418,42 +434,43 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
   for (int row = part; row < p.rows; row += p.parts) {
     if (!kAhead) fetch(row);
     const float r1 = p.w1 ? p.stats[row] : 1.f, r2 = p.w2 ? p.stats[p.rows + row] : 1.f;
-    // hh (h without post_w), the gate, q = s swish w1 hh, zh, e = dz + r2 t and the three sums
     Dot tz, eq, zq;  // t zh, e q, zh q
+    // hh (h without post_w), the gate and its sigmoid, zh, e = dz + r2 t; q is what z has of n
     float hh[K][VEC], g[K][VEC], sg[K][VEC], zh[K][VEC], e[K][VEC];
 #pragma unroll
     for (int c = 0; c < K; ++c) {
       const int col = (c * n + (int)threadIdx.x) * VEC;
       if (col < p.d) {
-        float q[VEC], v[VEC];
+        float q[VEC], v[VEC], w[VEC];
         hr[c].get(hh[c], h16);
         mul(hh[c], hh[c], r1);
-        if (p.w1)
-          weights<VEC>(p.w1, col, v);
-        else
-          fill(v, 1.f);
-        mul(q, hh[c], v);
+        if (kAhead) {
+          mul(q, hh[c], kept1);
+        } else {
+          both_weights<VEC>(p, col, w);
+          mul(q, hh[c], w);
+        }
         if (p.g) {
           gr[c].get(g[c], h16);
           gate_by(q, g[c], sg[c]);
-        }
-        if (p.s) {
-          weights<VEC>(p.s, col, v);
-          mul(q, q, v);
         }
         if (p.dz)
           dzr[c].get(e[c], x16);
         else
           fill(e[c], 0.f);
         if (p.dy) {
-          float w[VEC], dy[VEC];
+          float dy[VEC];
           xr[c].get(v, x16);
-          weights<VEC>(p.w2, col, w);
           dyr[c].get(dy, p.y16);
           fma(zh[c], v, p.alpha, q);
           mul(zh[c], zh[c], r2);
           fma(a2[c], dy, zh[c], a2[c]);
-          mul(dy, dy, w);  // t
+          if (kAhead) {
+            mul(dy, dy, kept2);  // t
+          } else {
+            weights<VEC>(p.w2, col, w);
+            mul(dy, dy, w);
+          }
           tz.add(dy, zh[c]);
           fma(e[c], dy, r2, e[c]);
           zq.add(zh[c], q);
@@ -475,17 +492,12 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
         if (p.dy) fma(e[c], zh[c], -m2, e[c]);  // Z
         mul(o, e[c], p.alpha);
         put<VEC>(p.dx, at, o, x16);
-        if (p.s)
-          weights<VEC>(p.s, col, v);
-        else
-          fill(v, 1.f);
-        if (p.w1)
-          weights<VEC>(p.w1, col, w);
-        else
-          fill(w, 1.f);
+        if (!kAhead) both_weights<VEC>(p, col, w);
         mul(o, e[c], hh[c]);
-        mul(o, o, w);  // Z n
-        mul(v, v, e[c]);  // Z s
+        if (kAhead)
+          mul(v, e[c], kept1);
+        else
+          mul(v, e[c], w);
         if (p.g) {
           float sw[VEC], sl[VEC];
 #pragma unroll
@@ -494,23 +506,17 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
             sl[i] = 1.f - sg[c][i];
           }
           mul(sw, sw, sg[c]);
-          fma(as[c], o, sw, as[c]);
+          fma(a1[c], o, sw, a1[c]);
           fma(sl, sw, sl, sg[c]);  // swish'
-          if (p.s) {
-            float s[VEC];
-            weights<VEC>(p.s, col, s);
-            mul(o, o, s);
-          }
+          mul(o, v, hh[c]);
           mul(o, o, sl);
           put<VEC>(p.dg, at, o, h16);
-          mul(v, v, sw);  // N
+          mul(v, v, sw);
         } else {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) as[c][i] += o[i];
+          for (int i = 0; i < VEC; ++i) a1[c][i] += o[i];
         }
-        if (p.w1) {
-          fma(a1[c], v, hh[c], a1[c]);
-          mul(v, v, w);
+        if (p.w1) {  // v = N w1
           fma(v, hh[c], -m1, v);
           mul(v, v, r1);
         }
@@ -524,15 +530,14 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
     const int col = (c * n + (int)threadIdx.x) * VEC;
     if (col < p.d) {
       const int64_t at = (int64_t)part * p.d + col;
-      if (p.w1) put<VEC>(p.part, at, a1[c], false);
-      if (p.s) put<VEC>(p.part, plane + at, as[c], false);
-      if (p.w2) put<VEC>(p.part, 2 * plane + at, a2[c], false);
+      if (p.w1 || p.s) put<VEC>(p.part, at, a1[c], false);
+      if (p.w2) put<VEC>(p.part, plane + at, a2[c], false);
     }
   }
 }
 
 // Rows too wide for a thread's registers: the same in two passes over the row,
-// the second from the caches, with the column sums in shared memory, [3][d],
+// the second from the caches, with the column sums in shared memory, [2][d],
 // where every thread alone touches its columns.
 template <int VEC, int TX, int TH>
 __global__ void __launch_bounds__(512, 1) seam_backward_wide_kernel(SeamParams p) {
@@ -542,13 +547,12 @@ __global__ void __launch_bounds__(512, 1) seam_backward_wide_kernel(SeamParams p
   clear_red(red);
   const int n = blockDim.x;
   const bool x16 = is16<TX>(p.x16), h16 = is16<TH>(p.h16);
-  float *a1 = acc, *as = acc + p.d, *a2 = acc + 2 * p.d;
+  float *a1 = acc, *a2 = acc + p.d;
   for (int col = threadIdx.x * VEC; col < p.d; col += n * VEC)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) a1[col + i] = as[col + i] = a2[col + i] = 0.f;
-  // hh, the gate's sigmoid, q and zh, e of VEC values
+    for (int i = 0; i < VEC; ++i) a1[col + i] = a2[col + i] = 0.f;
   struct Values {
-    float hh[VEC], g[VEC], sg[VEC], q[VEC], zh[VEC], e[VEC], dy[VEC], t[VEC];
+    float hh[VEC], g[VEC], sg[VEC], w[VEC], q[VEC], zh[VEC], e[VEC], dy[VEC], t[VEC];
   };
   auto values = [&](int row, int col, float r1, float r2, Values &s) {
     Raw<VEC> hr, gr, xr, dzr, dyr;
@@ -559,89 +563,73 @@ __global__ void __launch_bounds__(512, 1) seam_backward_wide_kernel(SeamParams p
       dyr.load(p.dy, row * p.lddy + col, p.y16);
       xr.load(p.x, row * p.ldx + col, x16);
     }
-    float v[VEC];
+    both_weights<VEC>(p, col, s.w);
     hr.get(s.hh, h16);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) s.q[i] = s.hh[i] *= r1;
-    if (p.w1) {
-      weights<VEC>(p.w1, col, v);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) s.q[i] *= v[i];
-    }
+    mul(s.hh, s.hh, r1);
+    mul(s.q, s.hh, s.w);
     if (p.g) {
       gr.get(s.g, h16);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        s.sg[i] = sigmoid(s.g[i]);
-        s.q[i] *= swish(s.g[i], s.sg[i]);
-      }
+      gate_by(s.q, s.g, s.sg);
     }
-    if (p.s) {
-      weights<VEC>(p.s, col, v);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) s.q[i] *= v[i];
-    }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) s.e[i] = s.zh[i] = s.t[i] = s.dy[i] = 0.f;
+    fill(s.e, 0.f), fill(s.zh, 0.f), fill(s.t, 0.f), fill(s.dy, 0.f);
     if (p.dz) dzr.get(s.e, x16);
     if (p.dy) {
-      float w[VEC];
+      float v[VEC];
       xr.get(v, x16);
-      weights<VEC>(p.w2, col, w);
       dyr.get(s.dy, p.y16);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        s.zh[i] = fmaf(p.alpha, v[i], s.q[i]) * r2;
-        s.t[i] = s.dy[i] * w[i];
-        s.e[i] = fmaf(r2, s.t[i], s.e[i]);
-      }
+      fma(s.zh, v, p.alpha, s.q);
+      mul(s.zh, s.zh, r2);
+      weights<VEC>(p.w2, col, v);
+      mul(s.t, s.dy, v);
+      fma(s.e, s.t, r2, s.e);
     }
   };
   for (int row = blockIdx.x; row < p.rows; row += p.parts) {
     const float r1 = p.w1 ? p.stats[row] : 1.f, r2 = p.w2 ? p.stats[p.rows + row] : 1.f;
-    float sum[3] = {0.f, 0.f, 0.f};  // t zh, e q, zh q
+    Dot tz, eq, zq;
     for (int col = threadIdx.x * VEC; col < p.d; col += n * VEC) {
       Values s;
       values(row, col, r1, r2, s);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        sum[0] = fmaf(s.t[i], s.zh[i], sum[0]);
-        sum[1] = fmaf(s.e[i], s.q[i], sum[1]);
-        sum[2] = fmaf(s.zh[i], s.q[i], sum[2]);
-      }
+      tz.add(s.t, s.zh);
+      eq.add(s.e, s.q);
+      zq.add(s.zh, s.q);
     }
+    float sum[3] = {tz.sum(), eq.sum(), zq.sum()};
     row_sum(sum, false, red, flip);
     const float m2 = r2 * (sum[0] * p.inv_d), m1 = (sum[1] - m2 * sum[2]) * p.inv_d;
     for (int col = threadIdx.x * VEC; col < p.d; col += n * VEC) {
       const int64_t at = (int64_t)row * p.d + col;
       Values s;
       values(row, col, r1, r2, s);
-      float o[VEC], v[VEC], w[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        s.e[i] = fmaf(-m2, s.zh[i], s.e[i]);  // Z
-        o[i] = p.alpha * s.e[i];
-        w[i] = v[i] = 1.f;
-      }
+      float o[VEC], v[VEC];
+      fma(s.e, s.zh, -m2, s.e);  // Z
+      mul(o, s.e, p.alpha);
       put<VEC>(p.dx, at, o, x16);
-      if (p.w1) weights<VEC>(p.w1, col, w);
-      if (p.s) weights<VEC>(p.s, col, v);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float en = s.e[i] * (s.hh[i] * w[i]);
-        const float sw = p.g ? swish(s.g[i], s.sg[i]) : 1.f;
-        as[col + i] = fmaf(en, sw, as[col + i]);
-        a2[col + i] = fmaf(s.dy[i], s.zh[i], a2[col + i]);
-        o[i] = p.g ? en * v[i] * swish_slope(s.g[i], s.sg[i]) : 0.f;
-        v[i] *= s.e[i] * sw;
-      }
-      if (p.g) put<VEC>(p.dg, at, o, h16);
-      if (p.w1) {
+      mul(o, s.e, s.hh);
+      mul(v, s.e, s.w);
+      if (p.g) {
+        float sw[VEC], sl[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          a1[col + i] = fmaf(v[i], s.hh[i], a1[col + i]);
-          v[i] = r1 * (v[i] * w[i] - s.hh[i] * m1);
+          sw[i] = fmaxf(s.g[i], -3.0e38f);
+          sl[i] = 1.f - s.sg[i];
         }
+        mul(sw, sw, s.sg);
+        fma(sl, sw, sl, s.sg);  // swish'
+        mul(o, o, sw);
+        mul(sl, sl, s.hh);
+        mul(sl, sl, v);
+        put<VEC>(p.dg, at, sl, h16);
+        mul(v, v, sw);
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        a1[col + i] += o[i];
+        a2[col + i] = fmaf(s.dy[i], s.zh[i], a2[col + i]);
+      }
+      if (p.w1) {
+        fma(v, s.hh, -m1, v);
+        mul(v, v, r1);
       }
       put<VEC>(p.dh, at, v, h16);
     }
@@ -651,30 +639,36 @@ __global__ void __launch_bounds__(512, 1) seam_backward_wide_kernel(SeamParams p
     const int64_t at = (int64_t)blockIdx.x * p.d + col;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      if (p.w1) p.part[at + i] = a1[col + i];
-      if (p.s) p.part[plane + at + i] = as[col + i];
-      if (p.w2) p.part[2 * plane + at + i] = a2[col + i];
+      if (p.w1 || p.s) p.part[at + i] = a1[col + i];
+      if (p.w2) p.part[plane + at + i] = a2[col + i];
     }
   }
 }
 
-// Column sums of up to three [parts][d] planes (blockIdx.y picks the plane):
-// 8 warps share a block of 32 columns, each adds every eighth part in order.
-__global__ void __launch_bounds__(256) seam_columns_kernel(const float *part, int parts, int d, float *o1, float *o2,
-                                                           float *o3) {
-  __shared__ float red[8][32];
-  float *out = blockIdx.y == 0 ? o1 : blockIdx.y == 1 ? o2 : o3;
-  if (!out) return;
+// Column sums of the [parts][d] planes (blockIdx.y: which): 16 warps share a
+// block of 32 columns, each adds every sixteenth part in order.  The first
+// plane's sum times scale is dw1, times post_w it is ds.
+__global__ void __launch_bounds__(512) seam_columns_kernel(const float *part, int parts, int d, const float *w1,
+                                                           const float *s, float *dw1, float *ds, float *dw2) {
+  __shared__ float red[16][32];
+  if (blockIdx.y ? !dw2 : !(dw1 || ds)) return;
   const int col = blockIdx.x * 32 + threadIdx.x;
   const float *src = part + (int64_t)blockIdx.y * parts * d + col;
   float t = 0.f;
-  if (col < d)
-    for (int k = threadIdx.y; k < parts; k += 8) t += src[(int64_t)k * d];
+  if (col < d) {
+#pragma unroll 4
+    for (int k = threadIdx.y; k < parts; k += 16) t += src[(int64_t)k * d];
+  }
   red[threadIdx.y][threadIdx.x] = t;
   __syncthreads();
   if (threadIdx.y == 0 && col < d) {
-    for (int k = 1; k < 8; ++k) t += red[k][threadIdx.x];
-    out[col] = t;
+    for (int k = 1; k < 16; ++k) t += red[k][threadIdx.x];
+    if (blockIdx.y) {
+      dw2[col] = t;
+    } else {
+      if (dw1) dw1[col] = s ? t * s[col] : t;
+      if (ds) ds[col] = w1 ? t * w1[col] : t;
+    }
   }
 }
 
@@ -778,7 +772,7 @@ int af_residual_norm_scratch(af_ctx *ctx, int64_t rows, int d, int64_t *floats) 
              "bad sizes");
   const int a = parts_of(ctx->num_sms, (int)rows, shape_of(d, false));
   const int b = d % 8 == 0 ? parts_of(ctx->num_sms, (int)rows, shape_of(d, true)) : 0;
-  *floats = 3ll * (a > b ? a : b) * d;
+  *floats = 2ll * (a > b ? a : b) * d;
   return AF_OK;
 }
 
@@ -819,23 +813,24 @@ int af_residual_norm_backward(af_ctx *ctx, const void *dz, int64_t lddz, const v
   const Shape s = shape_of(d, vec);
   p.parts = parts_of(ctx->num_sms, (int)rows, s);
   const bool sums = post_w || scale || pre_w;
-  AF_REQUIRE(!sums || (scratch && scratch_floats >= 3ll * p.parts * d), "af_residual_norm_backward",
-             "scratch of %lld floats, %lld are needed", (long long)scratch_floats, 3ll * p.parts * d);
+  AF_REQUIRE(!sums || (scratch && scratch_floats >= 2ll * p.parts * d), "af_residual_norm_backward",
+             "scratch of %lld floats, %lld are needed", (long long)scratch_floats, 2ll * p.parts * d);
   const SeamKernel kernel = kernel_of(s, p.x16, p.h16, true);
   size_t smem = 0;
   if (!held_backward(s)) {
-    smem = (size_t)3 * d * sizeof(float);
+    smem = (size_t)2 * d * sizeof(float);
     static std::atomic<unsigned long long> attr_devices[5];
     const int which = s.vec == 1 ? 4 : p.x16 * 2 + p.h16;
-    if (int rc = af::smem_attr(ctx, reinterpret_cast<const void *>(kernel), (size_t)3 * kMaxWidth * sizeof(float),
+    if (int rc = af::smem_attr(ctx, reinterpret_cast<const void *>(kernel), (size_t)2 * kMaxWidth * sizeof(float),
                                attr_devices[which], fn))
       return rc;
   }
   kernel<<<(unsigned)(p.parts / s.rows_per_block), dim3(s.threads, s.rows_per_block), smem, st>>>(p);
   if (int rc = af::launched(ctx, fn)) return rc;
   if (!sums) return AF_OK;
-  seam_columns_kernel<<<dim3((unsigned)((d + 31) / 32), 3), dim3(32, 8), 0, st>>>(
-      scratch, p.parts, d, post_w ? dpost_w : nullptr, scale ? dscale : nullptr, pre_w ? dpre_w : nullptr);
+  seam_columns_kernel<<<dim3((unsigned)((d + 31) / 32), 2), dim3(32, 16), 0, st>>>(
+      scratch, p.parts, d, post_w, scale, post_w ? dpost_w : nullptr, scale ? dscale : nullptr,
+      pre_w ? dpre_w : nullptr);
   return af::launched(ctx, fn);
 }
 
