@@ -81,11 +81,11 @@ struct Raw<1> {
   uint32_t a;
   __device__ __forceinline__ void load(const void *p, int64_t i, bool b16) {
     if (b16)
-      a = (uint32_t)__ldcs(static_cast<const unsigned short *>(p) + i) << 16;
+      a = __ldcs(static_cast<const unsigned short *>(p) + i);
     else
       a = __ldcs(static_cast<const unsigned int *>(p) + i);
   }
-  __device__ __forceinline__ void get(float (&v)[1], bool) const { v[0] = __uint_as_float(a); }
+  __device__ __forceinline__ void get(float (&v)[1], bool b16) const { v[0] = __uint_as_float(b16 ? a << 16 : a); }
 };
 
 template <int VEC>
@@ -267,14 +267,40 @@ __device__ __forceinline__ bool is16(int flag) {
   return T == 2 ? flag != 0 : T == 1;
 }
 
+// post_w scale (what is not given counts as 1) of VEC columns.
+template <int VEC>
+__device__ __forceinline__ void both_weights(const SeamParams &p, int col, float (&v)[VEC]) {
+  fill(v, 1.f);
+  if (p.w1) weights<VEC>(p.w1, col, v);
+  if (p.s) {
+    float s[VEC];
+    weights<VEC>(p.s, col, s);
+    mul(v, v, s);
+  }
+}
+
+// Those and pre_w of all of a thread's columns.
+template <int VEC, int K>
+__device__ __forceinline__ void keep_weights(const SeamParams &p, int n, float (&w1)[K][VEC], float (&w2)[K][VEC]) {
+#pragma unroll
+  for (int c = 0; c < K; ++c) {
+    const int col = (c * n + (int)threadIdx.x) * VEC;
+    fill(w1[c], 0.f), fill(w2[c], 0.f);
+    if (col < p.d) {
+      both_weights<VEC>(p, col, w1[c]);
+      if (p.w2) weights<VEC>(p.w2, col, w2[c]);
+    }
+  }
+}
+
 // Threads of a row: a warp (blockDim.y rows per block) or the whole block
 // (blockDim.y == 1).  Thread k of a row holds values (c * n + k) * VEC ..,
-// c < K, n the row's threads.  Where that is one vector, the weights stay in
+// c < K, n the row's threads.  Where those are few, the weights stay in
 // registers while a block walks over rows, and a row's loads are under way
 // while the row before it is summed.
 template <int VEC, int K, int TX, int TH>
-__global__ void __launch_bounds__(512, VEC == 8 && K == 1 ? 2 : 1) seam_forward_kernel(SeamParams p) {
-  constexpr bool kAhead = VEC == 8 && K == 1;
+__global__ void __launch_bounds__(512, VEC * K <= 8 && K <= 4 ? 2 : 1) seam_forward_kernel(SeamParams p) {
+  constexpr bool kAhead = VEC * K <= 8 && K <= 4;
   __shared__ __align__(16) float red[kRed];
   int flip = 0;
   clear_red(red);
@@ -293,17 +319,8 @@ __global__ void __launch_bounds__(512, VEC == 8 && K == 1 ? 2 : 1) seam_forward_
       }
     }
   };
-  float kept[3][VEC];  // with kAhead: post_w scale (each 1 where not given), pre_w
-  if (kAhead && (int)threadIdx.x * VEC < p.d) {
-    const int col = (int)threadIdx.x * VEC;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) kept[0][i] = kept[1][i] = kept[2][i] = 1.f;
-    if (p.w1) weights<VEC>(p.w1, col, kept[0]);
-    if (p.s) weights<VEC>(p.s, col, kept[1]);
-    if (p.w2) weights<VEC>(p.w2, col, kept[2]);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) kept[0][i] *= kept[1][i];
-  }
+  float kept1[K][VEC], kept2[K][VEC];  // with kAhead: post_w scale, pre_w
+  if (kAhead) keep_weights<VEC, K>(p, n, kept1, kept2);
   int row = blockIdx.x * blockDim.y + threadIdx.y;
   if (kAhead && row < p.rows) fetch(row);
   for (; row < p.rows; row += step) {  // a block's threads leave together where they share a row
@@ -323,17 +340,11 @@ __global__ void __launch_bounds__(512, VEC == 8 && K == 1 ? 2 : 1) seam_forward_
           gate_by(z[c], v, sg);
         }
         if (kAhead) {
-          mul(z[c], z[c], kept[0]);
+          mul(z[c], z[c], kept1[c]);
         } else {
           float v[VEC];
-          if (p.w1) {
-            weights<VEC>(p.w1, col, v);
-            mul(z[c], z[c], v);
-          }
-          if (p.s) {
-            weights<VEC>(p.s, col, v);
-            mul(z[c], z[c], v);
-          }
+          both_weights<VEC>(p, col, v);
+          mul(z[c], z[c], v);
         }
         xr[c].get(x[c], x16);
         mul(x[c], x[c], p.alpha);
@@ -367,7 +378,7 @@ __global__ void __launch_bounds__(512, VEC == 8 && K == 1 ? 2 : 1) seam_forward_
         if (col < p.d) {
           mul(z[c], z[c], r2);
           if (kAhead) {
-            mul(z[c], z[c], kept[2]);
+            mul(z[c], z[c], kept2[c]);
           } else {
             float v[VEC];
             weights<VEC>(p.w2, col, v);
@@ -384,21 +395,9 @@ __global__ void __launch_bounds__(512, VEC == 8 && K == 1 ? 2 : 1) seam_forward_
   }
 }
 
-// post_w scale (what is not given counts as 1) of VEC columns.
-template <int VEC>
-__device__ __forceinline__ void both_weights(const SeamParams &p, int col, float (&v)[VEC]) {
-  fill(v, 1.f);
-  if (p.w1) weights<VEC>(p.w1, col, v);
-  if (p.s) {
-    float s[VEC];
-    weights<VEC>(p.s, col, s);
-    mul(v, v, s);
-  }
-}
-
 template <int VEC, int K, int TX, int TH>
 __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
-  constexpr bool kAhead = VEC == 8 && K == 1;
+  constexpr bool kAhead = VEC * K <= 8 && K <= 4;
   __shared__ __align__(16) float red[kRed];
   int flip = 0;
   clear_red(red);
@@ -407,12 +406,8 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
   float a1[K][VEC], a2[K][VEC];  // this thread's columns of sum Z swish hh and of dw2
 #pragma unroll
   for (int c = 0; c < K; ++c) fill(a1[c], 0.f), fill(a2[c], 0.f);
-  float kept1[VEC], kept2[VEC];  // with kAhead: post_w scale, pre_w
-  if (kAhead && (int)threadIdx.x * VEC < p.d) {
-    both_weights<VEC>(p, (int)threadIdx.x * VEC, kept1);
-    fill(kept2, 0.f);
-    if (p.w2) weights<VEC>(p.w2, (int)threadIdx.x * VEC, kept2);
-  }
+  float kept1[K][VEC], kept2[K][VEC];  // with kAhead: post_w scale, pre_w
+  if (kAhead) keep_weights<VEC, K>(p, n, kept1, kept2);
   Raw<VEC> hr[K], gr[K], xr[K], dzr[K], dyr[K];
   auto fetch = [&](int row) {
 #pragma unroll
@@ -445,7 +440,7 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
         hr[c].get(hh[c], h16);
         mul(hh[c], hh[c], r1);
         if (kAhead) {
-          mul(q, hh[c], kept1);
+          mul(q, hh[c], kept1[c]);
         } else {
           both_weights<VEC>(p, col, w);
           mul(q, hh[c], w);
@@ -466,7 +461,7 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
           mul(zh[c], zh[c], r2);
           fma(a2[c], dy, zh[c], a2[c]);
           if (kAhead) {
-            mul(dy, dy, kept2);  // t
+            mul(dy, dy, kept2[c]);  // t
           } else {
             weights<VEC>(p.w2, col, w);
             mul(dy, dy, w);
@@ -495,7 +490,7 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
         if (!kAhead) both_weights<VEC>(p, col, w);
         mul(o, e[c], hh[c]);
         if (kAhead)
-          mul(v, e[c], kept1);
+          mul(v, e[c], kept1[c]);
         else
           mul(v, e[c], w);
         if (p.g) {
@@ -755,7 +750,7 @@ int af_residual_norm(af_ctx *ctx, const void *x, int64_t ldx, int x_bf16, const 
                    rows_aligned(pre_w, 8, 0) && rows_aligned(z, d, x_bf16) && rows_aligned(y, d, y_bf16);
   const Shape s = shape_of(d, vec);
   int64_t blocks = (rows + s.rows_per_block - 1) / s.rows_per_block;
-  if (s.vec == 8 && s.k == 1) {  // blocks that walk: 1024 threads an SM, what its registers hold
+  if (s.vec * s.k <= 8 && s.k <= 4) {  // blocks that walk: 1024 threads an SM, what its registers hold
     const int per_sm = 1024 / (s.threads * s.rows_per_block);
     blocks = std::min<int64_t>(blocks, (int64_t)ctx->num_sms * (per_sm < 1 ? 1 : per_sm));
   }
