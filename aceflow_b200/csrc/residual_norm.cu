@@ -30,6 +30,7 @@
 #include "common.cuh"
 
 #include <algorithm>
+#include <initializer_list>
 
 namespace {
 
@@ -77,6 +78,22 @@ struct Raw<8> {
   }
 };
 template <>
+struct Raw<2> {
+  uint32_t a, b;
+  __device__ __forceinline__ void load(const void *p, int64_t i, bool b16) {
+    if (b16) {
+      a = __ldcs(reinterpret_cast<const unsigned int *>(static_cast<const char *>(p) + 2 * i));
+    } else {
+      const uint2 q = __ldcs(reinterpret_cast<const uint2 *>(static_cast<const char *>(p) + 4 * i));
+      a = q.x, b = q.y;
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[2], bool b16) const {
+    v[0] = __uint_as_float(b16 ? a << 16 : a);
+    v[1] = __uint_as_float(b16 ? a & 0xffff0000u : b);
+  }
+};
+template <>
 struct Raw<1> {
   uint32_t a;
   __device__ __forceinline__ void load(const void *p, int64_t i, bool b16) {
@@ -105,6 +122,13 @@ __device__ __forceinline__ void put<8>(void *p, int64_t i, const float (&v)[8], 
   }
 }
 template <>
+__device__ __forceinline__ void put<2>(void *p, int64_t i, const float (&v)[2], bool b16) {
+  if (b16)
+    *reinterpret_cast<__nv_bfloat162 *>(static_cast<__nv_bfloat16 *>(p) + i) = __floats2bfloat162_rn(v[0], v[1]);
+  else
+    *reinterpret_cast<float2 *>(static_cast<float *>(p) + i) = make_float2(v[0], v[1]);
+}
+template <>
 __device__ __forceinline__ void put<1>(void *p, int64_t i, const float (&v)[1], bool b16) {
   if (b16)
     static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16(v[0]);
@@ -118,6 +142,9 @@ __device__ __forceinline__ void weights(const float *w, int col, float (&v)[VEC]
     const float4 a = __ldg(reinterpret_cast<const float4 *>(w + col)),
                  b = __ldg(reinterpret_cast<const float4 *>(w + col) + 1);
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else if constexpr (VEC == 2) {
+    const float2 a = __ldg(reinterpret_cast<const float2 *>(w + col));
+    v[0] = a.x, v[1] = a.y;
   } else {
     v[0] = __ldg(w + col);
   }
@@ -227,31 +254,33 @@ __device__ __forceinline__ void gate_by(float (&o)[VEC], const float (&g)[VEC], 
   mul(o, o, w);
 }
 
-constexpr int kRed = 2 * 3 * 16;
+constexpr int kRed = 2 * 3 * 32;
 // Sums of n values over the row's threads: a warp (one_warp) or the block.
-// `red` holds 2 x 3 x 16 floats, those of absent warps 0; `flip` alternates its
+// `red` holds 2 x 3 x 32 floats, those of absent warps 0; `flip` alternates its
 // halves, so one barrier per sum is enough.
 template <int NV>
 __device__ __forceinline__ void row_sum(float (&v)[NV], bool one_warp, float *red, int &flip) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) v[i] = warp_sum(v[i]);
   if (one_warp) return;
-  float *r = red + flip * 48;
+  float *r = red + flip * 96;
   flip ^= 1;
   if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) r[i * 16 + (threadIdx.x >> 5)] = v[i];
+    for (int i = 0; i < NV; ++i) r[i * 32 + (threadIdx.x >> 5)] = v[i];
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const float4 *q = reinterpret_cast<const float4 *>(r + i * 16);
+    const float4 *q = reinterpret_cast<const float4 *>(r + i * 32);
     float4 a = q[0], b = q[1];
-    if (blockDim.x > 256) {
-      const float4 c = q[2], d = q[3];
-      a.x += c.x, a.y += c.y, a.z += c.z, a.w += c.w;
-      b.x += d.x, b.y += d.y, b.z += d.z, b.w += d.w;
-    }
+#pragma unroll
+    for (int k = 2; k < 8; k += 2)
+      if ((int)blockDim.x > 128 * k) {  // more than 4 k warps
+        const float4 c = q[k], d = q[k + 1];
+        a.x += c.x, a.y += c.y, a.z += c.z, a.w += c.w;
+        b.x += d.x, b.y += d.y, b.z += d.z, b.w += d.w;
+      }
     v[i] = ((a.x + b.x) + (a.y + b.y)) + ((a.z + b.z) + (a.w + b.w));
   }
 }
@@ -259,12 +288,6 @@ __device__ __forceinline__ void clear_red(float *red) {
   const int t = threadIdx.y * blockDim.x + threadIdx.x;
   for (int i = t; i < kRed; i += blockDim.x * blockDim.y) red[i] = 0.f;
   __syncthreads();
-}
-
-// A type that the kernel was compiled for (0: fp32, 1: bf16) or that comes with the call (2).
-template <int T>
-__device__ __forceinline__ bool is16(int flag) {
-  return T == 2 ? flag != 0 : T == 1;
 }
 
 // post_w scale (what is not given counts as 1) of VEC columns.
@@ -299,13 +322,13 @@ __device__ __forceinline__ void keep_weights(const SeamParams &p, int n, float (
 // registers while a block walks over rows, and a row's loads are under way
 // while the row before it is summed.
 template <int VEC, int K, int TX, int TH>
-__global__ void __launch_bounds__(512, VEC * K <= 8 && K <= 4 ? 2 : 1) seam_forward_kernel(SeamParams p) {
+__global__ void __launch_bounds__(VEC == 8 && K == 1 ? 1024 : 512, VEC == 8 ? 1 : 2) seam_forward_kernel(SeamParams p) {
   constexpr bool kAhead = VEC * K <= 8 && K <= 4;
   __shared__ __align__(16) float red[kRed];
   int flip = 0;
   clear_red(red);
   const int n = blockDim.x;
-  const bool one_warp = n == 32, x16 = is16<TX>(p.x16), h16 = is16<TH>(p.h16);
+  const bool one_warp = n == 32, x16 = TX == 1, h16 = TH == 1;
   const int step = gridDim.x * blockDim.y;
   Raw<VEC> hr[K], gr[K], xr[K];
   auto fetch = [&](int row) {
@@ -402,7 +425,7 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
   int flip = 0;
   clear_red(red);
   const int n = blockDim.x;
-  const bool one_warp = n == 32, x16 = is16<TX>(p.x16), h16 = is16<TH>(p.h16);
+  const bool one_warp = n == 32, x16 = TX == 1, h16 = TH == 1;
   float a1[K][VEC], a2[K][VEC];  // this thread's columns of sum Z swish hh and of dw2
 #pragma unroll
   for (int c = 0; c < K; ++c) fill(a1[c], 0.f), fill(a2[c], 0.f);
@@ -541,7 +564,7 @@ __global__ void __launch_bounds__(512, 1) seam_backward_wide_kernel(SeamParams p
   int flip = 0;
   clear_red(red);
   const int n = blockDim.x;
-  const bool x16 = is16<TX>(p.x16), h16 = is16<TH>(p.h16);
+  const bool x16 = TX == 1, h16 = TH == 1;
   float *a1 = acc, *a2 = acc + p.d;
   for (int col = threadIdx.x * VEC; col < p.d; col += n * VEC)
 #pragma unroll
@@ -669,51 +692,72 @@ __global__ void __launch_bounds__(512) seam_columns_kernel(const float *part, in
 
 constexpr int kMaxWidth = 16384;
 
-// Threads of a row and values per thread for rows of d values: one vector a
-// thread while 512 threads suffice.
+// Threads of a row and values per thread for rows of d values.  A block's
+// registers allow 512 threads (1024 in the vectorised forward); while they
+// suffice, few values a thread, so that much is under way.
 struct Shape {
   int vec, k, threads, rows_per_block;
 };
-Shape shape_of(int d, bool vec8) {
-  if (vec8) {
-    const int ch = d / 8;  // 16-byte (bf16) or 32-byte (fp32) chunks
-    if (ch <= 32) return {8, 1, 32, 4};
-    if (ch <= 512) return {8, 1, (ch + 31) / 32 * 32, 1};
-    if (ch <= 1024) return {8, 2, 512, 1};
-    return {8, 4, 512, 1};
+Shape shape_of(int d, int vec, bool backward) {
+  auto threads = [&](int per) { return (d + per * 32 - 1) / (per * 32) * 32; };  // whole warps that hold d values
+  if (vec == 8) {
+    if (d <= 256) return {8, 1, 32, 4};
+    if (d <= (backward ? 4096 : 8192)) return {8, 1, threads(8), 1};
+    return {8, backward ? 0 : 4, 512, 1};
   }
   if (d <= 128) return {1, 4, 32, 4};
-  if (d <= 2048) return {1, 4, (d + 127) / 128 * 32, 1};
-  if (d <= 4096) return {1, 8, (d + 255) / 256 * 32, 1};
-  if (d <= 8192) return {1, 16, 512, 1};
-  return {1, 32, 512, 1};
+  if (vec == 2) {
+    if (d <= 2048) return {2, 2, threads(4), 1};
+    if (d <= 4096) return {2, 4, threads(8), 1};
+    return backward ? Shape{2, 0, 512, 1} : Shape{2, 16, 512, 1};
+  }
+  if (d <= 2048) return {1, 4, threads(4), 1};
+  if (d <= 4096) return {1, 8, threads(8), 1};
+  if (backward) return {1, 0, 512, 1};
+  return d <= 8192 ? Shape{1, 16, 512, 1} : Shape{1, 32, 512, 1};
 }
+bool walks(const Shape &s) { return s.vec * s.k <= 8 && s.k > 0 && s.k <= 4; }  // the kernels' kAhead
 
-// A backward of this shape holds its row in registers (else: two passes).
-bool held_backward(const Shape &s) { return s.k == 1 || (s.vec == 1 && s.k <= 8); }
-
+// The kernel of a shape (k 0: the two-pass backward).
 using SeamKernel = void (*)(SeamParams);
 template <int TX, int TH>
-SeamKernel vector_kernel(int k, bool backward) {
-  if (backward) return k == 1 ? seam_backward_kernel<8, 1, TX, TH> : seam_backward_wide_kernel<8, TX, TH>;
-  return k == 1 ? seam_forward_kernel<8, 1, TX, TH>
-                : k == 2 ? seam_forward_kernel<8, 2, TX, TH> : seam_forward_kernel<8, 4, TX, TH>;
+SeamKernel typed_kernel(const Shape &s, bool backward) {
+  if (backward) {
+    if (s.vec == 8) return s.k == 1 ? seam_backward_kernel<8, 1, TX, TH> : seam_backward_wide_kernel<8, TX, TH>;
+    if (s.vec == 2)
+      return s.k == 2   ? seam_backward_kernel<2, 2, TX, TH>
+             : s.k == 4 ? seam_backward_kernel<2, 4, TX, TH>
+                        : seam_backward_wide_kernel<2, TX, TH>;
+    return s.k == 4   ? seam_backward_kernel<1, 4, TX, TH>
+           : s.k == 8 ? seam_backward_kernel<1, 8, TX, TH>
+                      : seam_backward_wide_kernel<1, TX, TH>;
+  }
+  if (s.vec == 8) return s.k == 1 ? seam_forward_kernel<8, 1, TX, TH> : seam_forward_kernel<8, 4, TX, TH>;
+  if (s.vec == 2)
+    return s.k == 2   ? seam_forward_kernel<2, 2, TX, TH>
+           : s.k == 4 ? seam_forward_kernel<2, 4, TX, TH>
+                      : seam_forward_kernel<2, 16, TX, TH>;
+  return s.k == 4    ? seam_forward_kernel<1, 4, TX, TH>
+         : s.k == 8  ? seam_forward_kernel<1, 8, TX, TH>
+         : s.k == 16 ? seam_forward_kernel<1, 16, TX, TH>
+                     : seam_forward_kernel<1, 32, TX, TH>;
 }
 SeamKernel kernel_of(const Shape &s, bool x16, bool h16, bool backward) {
-  if (s.vec == 8) {
-    if (x16) return h16 ? vector_kernel<1, 1>(s.k, backward) : vector_kernel<1, 0>(s.k, backward);
-    return h16 ? vector_kernel<0, 1>(s.k, backward) : vector_kernel<0, 0>(s.k, backward);
-  }
-  if (s.k == 4) return backward ? seam_backward_kernel<1, 4, 2, 2> : seam_forward_kernel<1, 4, 2, 2>;
-  if (s.k == 8) return backward ? seam_backward_kernel<1, 8, 2, 2> : seam_forward_kernel<1, 8, 2, 2>;
-  if (backward) return seam_backward_wide_kernel<1, 2, 2>;
-  return s.k == 16 ? seam_forward_kernel<1, 16, 2, 2> : seam_forward_kernel<1, 32, 2, 2>;
+  if (x16) return h16 ? typed_kernel<1, 1>(s, backward) : typed_kernel<1, 0>(s, backward);
+  return h16 ? typed_kernel<0, 1>(s, backward) : typed_kernel<0, 0>(s, backward);
 }
 
-// 16-byte accesses of 8 values need rows that start on 16 bytes (bf16; fp32
-// rows are then aligned too).
-bool rows_aligned(const void *p, int64_t ld, int is16) {
-  return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % (is16 ? 8 : 4) == 0);
+// Values an access may take where rows lie at p, ld elements apart: 8 need 16
+// bytes (of fp32 rows, which are then aligned too, every half), 2 the pair's size.
+int access_of(const void *p, int64_t ld, int is16) {
+  if (!p) return 8;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  if (a % 16 == 0 && ld % (is16 ? 8 : 4) == 0) return 8;
+  return a % (is16 ? 4 : 8) == 0 && ld % 2 == 0 ? 2 : 1;
+}
+int least_access(int d, std::initializer_list<int> all) {
+  const int v = std::min(all);
+  return d % v == 0 ? v : d % 2 == 0 && v >= 2 ? 2 : 1;
 }
 
 // Row groups that share the rows of a backward: about 512 threads an SM, as
@@ -745,12 +789,12 @@ int af_residual_norm(af_ctx *ctx, const void *x, int64_t ldx, int x_bf16, const 
   p.x16 = x_bf16 != 0, p.h16 = h_bf16 != 0, p.y16 = y_bf16 != 0;
   p.w1 = post_w, p.s = scale, p.w2 = pre_w, p.alpha = alpha, p.eps = eps, p.inv_d = 1.0f / (float)d;
   p.rows = (int)rows, p.d = d, p.z = z, p.y = y, p.stats = stats;
-  const bool vec = d % 8 == 0 && rows_aligned(x, ldx, x_bf16) && rows_aligned(h, ldh, h_bf16) &&
-                   rows_aligned(gate, ldg, h_bf16) && rows_aligned(post_w, 8, 0) && rows_aligned(scale, 8, 0) &&
-                   rows_aligned(pre_w, 8, 0) && rows_aligned(z, d, x_bf16) && rows_aligned(y, d, y_bf16);
-  const Shape s = shape_of(d, vec);
+  const int vec = least_access(
+      d, {access_of(x, ldx, x_bf16), access_of(h, ldh, h_bf16), access_of(gate, ldg, h_bf16), access_of(post_w, 8, 0),
+          access_of(scale, 8, 0), access_of(pre_w, 8, 0), access_of(z, d, x_bf16), access_of(y, d, y_bf16)});
+  const Shape s = shape_of(d, vec, false);
   int64_t blocks = (rows + s.rows_per_block - 1) / s.rows_per_block;
-  if (s.vec * s.k <= 8 && s.k <= 4) {  // blocks that walk: 1024 threads an SM, what its registers hold
+  if (walks(s)) {  // blocks that walk: 1024 threads an SM, what its registers hold
     const int per_sm = 1024 / (s.threads * s.rows_per_block);
     blocks = std::min<int64_t>(blocks, (int64_t)ctx->num_sms * (per_sm < 1 ? 1 : per_sm));
   }
@@ -765,9 +809,10 @@ int af_residual_norm_scratch(af_ctx *ctx, int64_t rows, int d, int64_t *floats) 
   AF_ENTER(ctx, fn);
   AF_REQUIRE(floats && rows >= 0 && rows < (1ll << 31) && d > 0 && d <= kMaxWidth, "af_residual_norm_scratch",
              "bad sizes");
-  const int a = parts_of(ctx->num_sms, (int)rows, shape_of(d, false));
-  const int b = d % 8 == 0 ? parts_of(ctx->num_sms, (int)rows, shape_of(d, true)) : 0;
-  *floats = 2ll * (a > b ? a : b) * d;
+  int most = 0;  // whatever accesses the call's tensors will allow
+  for (int vec : {1, 2, 8})
+    if (d % vec == 0) most = std::max(most, parts_of(ctx->num_sms, (int)rows, shape_of(d, vec, true)));
+  *floats = 2ll * most * d;
   return AF_OK;
 }
 
@@ -800,24 +845,22 @@ int af_residual_norm_backward(af_ctx *ctx, const void *dz, int64_t lddz, const v
   p.w1 = post_w, p.s = scale, p.w2 = pre_w, p.alpha = alpha, p.inv_d = 1.0f / (float)d;
   p.rows = (int)rows, p.d = d, p.stats = const_cast<float *>(stats);
   p.dz = dz, p.dy = dy, p.lddz = lddz, p.lddy = lddy, p.dx = dx, p.dh = dh, p.dg = dgate, p.part = scratch;
-  const bool vec = d % 8 == 0 && rows_aligned(x, ldx, x_bf16) && rows_aligned(h, ldh, h_bf16) &&
-                   rows_aligned(gate, ldg, h_bf16) && rows_aligned(post_w, 8, 0) && rows_aligned(scale, 8, 0) &&
-                   rows_aligned(pre_w, 8, 0) && rows_aligned(dz, lddz, x_bf16) && rows_aligned(dy, lddy, y_bf16) &&
-                   rows_aligned(dx, d, x_bf16) && rows_aligned(dh, d, h_bf16) && rows_aligned(dgate, d, h_bf16) &&
-                   rows_aligned(scratch, 8, 0);
-  const Shape s = shape_of(d, vec);
+  const int vec = least_access(
+      d, {access_of(x, ldx, x_bf16), access_of(h, ldh, h_bf16), access_of(gate, ldg, h_bf16), access_of(post_w, 8, 0),
+          access_of(scale, 8, 0), access_of(pre_w, 8, 0), access_of(dz, lddz, x_bf16), access_of(dy, lddy, y_bf16),
+          access_of(dx, d, x_bf16), access_of(dh, d, h_bf16), access_of(dgate, d, h_bf16), access_of(scratch, 8, 0)});
+  const Shape s = shape_of(d, vec, true);
   p.parts = parts_of(ctx->num_sms, (int)rows, s);
   const bool sums = post_w || scale || pre_w;
   AF_REQUIRE(!sums || (scratch && scratch_floats >= 2ll * p.parts * d), "af_residual_norm_backward",
              "scratch of %lld floats, %lld are needed", (long long)scratch_floats, 2ll * p.parts * d);
   const SeamKernel kernel = kernel_of(s, p.x16, p.h16, true);
   size_t smem = 0;
-  if (!held_backward(s)) {
+  if (s.k == 0) {
     smem = (size_t)2 * d * sizeof(float);
-    static std::atomic<unsigned long long> attr_devices[5];
-    const int which = s.vec == 1 ? 4 : p.x16 * 2 + p.h16;
+    static std::atomic<unsigned long long> attr_devices[3][4];
     if (int rc = af::smem_attr(ctx, reinterpret_cast<const void *>(kernel), (size_t)2 * kMaxWidth * sizeof(float),
-                               attr_devices[which], fn))
+                               attr_devices[s.vec == 8 ? 2 : s.vec - 1][p.x16 * 2 + p.h16], fn))
       return rc;
   }
   kernel<<<(unsigned)(p.parts / s.rows_per_block), dim3(s.threads, s.rows_per_block), smem, st>>>(p);
