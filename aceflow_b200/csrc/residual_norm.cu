@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(VEC == 8 && K == 1 ? 1024 : 512, VEC == 8 ? 1 
     if (p.w1) {
       float sq[1] = {dot.sum()};
       row_sum(sq, one_warp, red, flip);
-      r1 = 1.0f / sqrtf(sq[0] * p.inv_d + p.eps);
+      r1 = rsqrtf(fmaf(sq[0], p.inv_d, p.eps));
     }
     Dot dz;
 #pragma unroll
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(VEC == 8 && K == 1 ? 1024 : 512, VEC == 8 ? 1 
     if (p.w2) {
       float sz[1] = {dz.sum()};
       row_sum(sz, one_warp, red, flip);
-      r2 = 1.0f / sqrtf(sz[0] * p.inv_d + p.eps);
+      r2 = rsqrtf(fmaf(sz[0], p.inv_d, p.eps));
 #pragma unroll
       for (int c = 0; c < K; ++c) {
         const int col = (c * n + (int)threadIdx.x) * VEC;
