@@ -7,6 +7,7 @@ makes exactly one ABI call on the tensor's current stream.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -35,6 +36,12 @@ def _ctx(t: torch.Tensor) -> int:
 
 def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _device_call(name: str, dev: int, *args) -> None:
+    """ABI call on device `dev`'s context and its current stream (`args` is
+    what stands between them)."""
+    _lib.call(name, _lib.context(dev), *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
 def _p(t):
@@ -644,26 +651,29 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: str | No
 
 
 def _same_device(x: torch.Tensor, **others) -> None:
+    dev = x.get_device()  # -1 on the CPU
     for n, t in others.items():
-        if t is not None and t.device != x.device:
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"{n} is on {t.device}, expected {x.device}")
+
+
+_Strides = _lib.ctypes.c_int64 * 3
+_PosStrides = _lib.ctypes.c_int64 * 2
 
 
 def _rotary_dims(x: torch.Tensor):
     """(B, T, heads, dim, strides) of x [B, T, heads, dim] or [rows, heads, dim]."""
     if x.dtype not in (F32, BF16):
         raise ValueError(f"x: expected float32 or bfloat16, got {x.dtype}")
-    if x.dim() == 3:
-        B, (T, H, D) = 1, x.shape
-        st = (0, x.stride(0), x.stride(1))
-    elif x.dim() == 4:
-        B, T, H, D = x.shape
-        st = x.stride()[:3]
-    else:
+    shape, st = x.shape, x.stride()
+    if len(shape) == 3:
+        shape, st = (1, *shape), (0, *st)
+    elif len(shape) != 4:
         raise ValueError("x must be [B, T, heads, head_dim] or [rows, heads, head_dim]")
-    if D == 0 or (x.stride(-1) != 1 and D > 1):
+    B, T, H, D = shape
+    if D == 0 or (st[3] != 1 and D > 1):
         raise ValueError("x: heads must have unit stride")
-    return B, T, H, D, st
+    return B, T, H, D, st[:3]
 
 
 def rotary(x: torch.Tensor, inv_freq: torch.Tensor, positions=0, *, layout: str = "interleaved", scale: float = 1.0,
@@ -688,9 +698,9 @@ def rotary(x: torch.Tensor, inv_freq: torch.Tensor, positions=0, *, layout: str 
         pos = positions
         if pos.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"positions: expected int32 or int64, got {pos.dtype}")
-        if tuple(pos.shape) == (T,):
+        if pos.shape == (T,):
             pst = (0, pos.stride(0))
-        elif x.dim() == 4 and tuple(pos.shape) == (B, T):
+        elif x.dim() == 4 and pos.shape == (B, T):
             pst = pos.stride()
         else:
             raise ValueError(f"positions of shape {tuple(pos.shape)} do not match x {tuple(x.shape)}")
@@ -709,11 +719,9 @@ def rotary(x: torch.Tensor, inv_freq: torch.Tensor, positions=0, *, layout: str 
     else:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         ost = (T * H * D, H * D, D)
-    arr = _lib.ctypes.c_int64 * 3
-    _lib.call("af_rotary", _lib.context(dev), _p(x), _p(out), int(x.dtype == BF16), arr(*st), arr(*ost), B, T, H, D,
-              _p(inv_freq), rot, _p(pos), int(pos is not None and pos.dtype == torch.int64),
-              (_lib.ctypes.c_int64 * 2)(*pst), start, int(layout == "interleaved"), float(scale), int(inverse),
-              _stream(x))
+    _device_call("af_rotary", dev, x.data_ptr(), out.data_ptr(), x.dtype == BF16, _Strides(*st), _Strides(*ost), B, T, H,
+                 D, inv_freq.data_ptr(), rot, _p(pos), pos is not None and pos.dtype == torch.int64,
+                 _PosStrides(*pst), start, layout == "interleaved", scale, inverse)
     return out
 
 
@@ -759,15 +767,15 @@ class ResidualNormGrads(NamedTuple):
 def _rows_of(t: torch.Tensor, name: str, shape) -> tuple:
     """(t, row stride) of rows [..., d] with one stride between them (a copy
     where the leading dimensions have no common one)."""
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype not in (F32, BF16):
         raise ValueError(f"{name}: expected float32 or bfloat16, got {t.dtype}")
-    if t.dim() == 2 and t.stride(1) == 1:
-        return t, t.stride(0)
-    d = t.shape[-1]
+    d = shape[-1]
     if t.is_contiguous():
         return t, d
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t, t.stride(0)
     want = None  # stride that the rows would have as one dimension
     ok = t.stride(-1) == 1 or d == 1
     for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
@@ -784,12 +792,13 @@ def _rows_of(t: torch.Tensor, name: str, shape) -> tuple:
 
 
 def _seam_args(x, h, gate, post_w, scale, pre_w):
-    if x.dim() < 1 or x.shape[-1] == 0:
+    shape = x.shape
+    if not shape or shape[-1] == 0:
         raise ValueError("x must have a non-empty last dimension")
-    d = x.shape[-1]
-    xt, ldx = _rows_of(x, "x", x.shape)
-    ht, ldh = _rows_of(h, "h", x.shape)
-    gt, ldg = (None, 0) if gate is None else _rows_of(gate, "gate", x.shape)
+    d = shape[-1]
+    xt, ldx = _rows_of(x, "x", shape)
+    ht, ldh = _rows_of(h, "h", shape)
+    gt, ldg = (None, 0) if gate is None else _rows_of(gate, "gate", shape)
     if gate is not None and gate.dtype != h.dtype:
         raise ValueError(f"gate: expected {h.dtype} as h, got {gate.dtype}")
     for n, w in (("post_w", post_w), ("scale", scale), ("pre_w", pre_w)):
@@ -819,13 +828,12 @@ def residual_norm(x: torch.Tensor, h: torch.Tensor, *, gate: torch.Tensor | None
     out_dtype = h.dtype if out_dtype is None else out_dtype
     if out_dtype not in (F32, BF16):
         raise ValueError("out_dtype must be float32 or bfloat16")
-    ctx = _ctx(x)
+    dev = _dev(x)
     z = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     y = None if pre_w is None else torch.empty(x.shape, dtype=out_dtype, device=x.device)
     stats = torch.empty(2, rows, dtype=F32, device=x.device) if want_stats else None
-    _lib.call("af_residual_norm", ctx, _p(xt), ldx, int(x.dtype == BF16), _p(ht), ldh, int(h.dtype == BF16), _p(gt),
-              ldg, _p(post_w), _p(scale), _p(pre_w), float(alpha), float(eps), rows, d, _p(z), _p(y),
-              int(out_dtype == BF16), _p(stats), _stream(x))
+    _device_call("af_residual_norm", dev, _p(xt), ldx, x.dtype == BF16, _p(ht), ldh, h.dtype == BF16, _p(gt), ldg,
+                 _p(post_w), _p(scale), _p(pre_w), alpha, eps, rows, d, _p(z), _p(y), out_dtype == BF16, _p(stats))
     return (z, y, stats) if want_stats else (z, y)
 
 
@@ -839,7 +847,7 @@ def residual_norm_backward(dz: torch.Tensor | None, dy: torch.Tensor | None, x: 
     every call, so it can be captured into any number of CUDA graphs."""
     d, rows, xt, ldx, ht, ldh, gt, ldg = _seam_args(x, h, gate, post_w, scale, pre_w)
     _need(stats, F32, "stats")
-    if tuple(stats.shape) != (2, rows):
+    if stats.shape != (2, rows):
         raise ValueError(f"stats must be [2, {rows}]")
     if dy is not None and pre_w is None:
         raise ValueError("dy without pre_w: the forward made no y")
@@ -848,19 +856,26 @@ def residual_norm_backward(dz: torch.Tensor | None, dy: torch.Tensor | None, x: 
     if dz is not None and dz.dtype != x.dtype:
         raise ValueError(f"dz: expected {x.dtype} as x, got {dz.dtype}")
     _same_device(x, stats=stats, dz=dz, dy=dy)
-    ctx = _ctx(x)
+    dev = _dev(x)
     new = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
     g = ResidualNormGrads(new(x), new(h), new(gate), new(post_w), new(scale), new(pre_w))
-    n = _lib.ctypes.c_int64()
-    scratch = None
+    floats, scratch = 0, None
     if not (post_w is None and scale is None and pre_w is None):
-        _lib.call("af_residual_norm_scratch", ctx, rows, d, _lib.ctypes.byref(n))
-        scratch = torch.empty(n.value, dtype=F32, device=x.device)
-    _lib.call("af_residual_norm_backward", ctx, _p(dzt), lddz, _p(dyt), lddy, _p(xt), ldx, int(x.dtype == BF16),
-              _p(ht), ldh, int(h.dtype == BF16), _p(gt), ldg, int(dy is not None and dy.dtype == BF16), _p(post_w),
-              _p(scale), _p(pre_w), float(alpha), rows, d, _p(stats), _p(g.x), _p(g.h), _p(g.gate), _p(g.post_w),
-              _p(g.scale), _p(g.pre_w), _p(scratch), n.value, _stream(x))
+        floats = _seam_scratch(dev, rows, d)
+        scratch = torch.empty(floats, dtype=F32, device=x.device)
+    _device_call("af_residual_norm_backward", dev, _p(dzt), lddz, _p(dyt), lddy, _p(xt), ldx, x.dtype == BF16, _p(ht),
+                 ldh, h.dtype == BF16, _p(gt), ldg, dy is not None and dy.dtype == BF16, _p(post_w), _p(scale),
+                 _p(pre_w), alpha, rows, d, _p(stats), _p(g.x), _p(g.h), _p(g.gate), _p(g.post_w), _p(g.scale),
+                 _p(g.pre_w), _p(scratch), floats)
     return g
+
+
+@functools.lru_cache(maxsize=1024)
+def _seam_scratch(dev: int, rows: int, d: int) -> int:
+    """Floats of scratch that residual_norm_backward needs for these sizes."""
+    n = _lib.ctypes.c_int64()
+    _lib.call("af_residual_norm_scratch", _lib.context(dev), rows, d, _lib.ctypes.byref(n))
+    return n.value
 
 
 class _ResidualNorm(torch.autograd.Function):
@@ -937,10 +952,10 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1
                 context.stride(1) != 1 and context.shape[1] > 1):
             raise ValueError("context must be an int32 [rows, L] tensor with unit column stride")
         c_ptr, c_stride, c_len = _p(context), context.stride(0), context.shape[1]
-    ctx = _ctx(logits)
+    index = _dev(logits)
     token = torch.empty(rows, dtype=torch.int32, device=dev)
     logp = torch.empty(rows, dtype=F32, device=dev) if return_logprobs else None
-    _lib.call("af_sample_tokens", ctx, _p(logits), int(logits.dtype == BF16), logits.stride(0), rows, V, c_ptr,
-              c_stride, c_len, t_ptr, float(t_all), k_ptr, int(k_all), p_ptr, float(p_all), m_ptr, float(m_all), r_ptr,
-              float(r_all), _p(uniforms), _p(token), _p(logp), _stream(logits))
+    _device_call("af_sample_tokens", index, logits.data_ptr(), logits.dtype == BF16, logits.stride(0), rows, V, c_ptr,
+                 c_stride, c_len, t_ptr, t_all, k_ptr, int(k_all), p_ptr, p_all, m_ptr, m_all, r_ptr, r_all,
+                 uniforms.data_ptr(), token.data_ptr(), _p(logp))
     return (token, logp) if return_logprobs else token
