@@ -19,6 +19,10 @@ LIB_PATH = os.environ.get("ACEFLOW_CUDA_LIB", os.path.join(_HERE, "lib", "libace
 
 AF_OK, AF_ERR_ARG, AF_ERR_CUDA, AF_ERR_NCCL, AF_ERR_TIMEOUT, AF_ERR_STATE = range(6)
 
+# include/aceflow_cuda.h
+AF_SAMPLE_MAX_VOCAB = 50000
+AF_SAMPLE_TOKENS_MAX_VOCAB = 327680
+
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64

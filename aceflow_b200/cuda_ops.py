@@ -521,15 +521,17 @@ def gemm_bf16(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor, row_sumsq: to
     a: bf16 2-D view with unit column stride.  Plain (a_kblock == 0): a is
     [M, K].  K-blocked: a is [K/a_kblock * M, a_kblock], the K/a_kblock
     blocks [M, a_kblock] stacked (an all-gather of column slices).
-    b: bf16 [N, K] view; out: fp32 [M, N] view.  rowscale from row_sumsq
+    b: bf16 [N, K] view; out: fp32 or bf16 [M, N] view.  rowscale from row_sumsq
     ([M, P] or, with parts_block, P/parts_block stacked blocks [M, parts_block])
     as 1/sqrt(sum/d + eps) when given; bias [N] fp32 and residual (an fp32
     [M, N] view, may be `out` itself) are added after the scale."""
     for n, t in (("a", a), ("b", b)):
         if t.dtype != BF16 or t.dim() != 2 or t.stride(1) != 1:
             raise ValueError(f"{n}: expected a 2-D bf16 view with unit column stride")
-    if out.dtype != F32 or out.dim() != 2 or out.stride(1) != 1:
-        raise ValueError("out: expected a 2-D fp32 view with unit column stride")
+    if out.dtype not in (F32, BF16) or out.dim() != 2 or out.stride(1) != 1:
+        raise ValueError("out: expected a 2-D fp32 or bf16 view with unit column stride")
+    if out.dtype == BF16 and accumulate:
+        raise ValueError("accumulate adds into an fp32 out")
     N, K = b.shape
     M = out.shape[0]
     if a_kblock:
@@ -551,7 +553,7 @@ def gemm_bf16(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor, row_sumsq: to
     if bias is not None:
         _need(bias, F32, "bias")
     _lib.call("af_gemm_bf16", _ctx(a), _p(a), a.stride(0), int(a_kblock), _p(b), b.stride(0), M, N, K, _p(out),
-              out.stride(0), 0, _p(bias), _p(residual), ldr, _p(row_sumsq), P, int(parts_block), float(inv_d),
+              out.stride(0), int(out.dtype == BF16), _p(bias), _p(residual), ldr, _p(row_sumsq), P, int(parts_block), float(inv_d),
               float(eps), int(accumulate), _stream(a))
     return out
 

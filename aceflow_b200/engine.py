@@ -333,20 +333,26 @@ class AceEngine:
         return float(np.random.random()) if uniform is None else float(uniform)
 
     def sample_token_from_logits(self, logits, context_tokens, temperature: float = 0.7, top_k: int = 40,
-                                 top_p: float = 0.9, repetition_penalty: float = 1.2, uniform=None) -> int:
+                                 top_p: float = 0.9, repetition_penalty: float = 1.2, uniform=None,
+                                 min_p: float = 0.0) -> int:
         """AceEngine.sample_token_from_logits (cpu/mod.rs:404-420, sampler.rs:104-180)
         on the GPU.  `uniform` in [0, 1) is the random draw (the reference
         takes it from a clock-seeded generator); None draws one from numpy's
-        global generator."""
+        global generator.  min_p (not in the reference): tokens less than min_p
+        times as likely as the likeliest are left out."""
         lt = torch.as_tensor(_f32(logits).reshape(1, -1)).to(self.device)
         ctx = np.asarray(list(context_tokens), np.int64)
         ctx = np.where((ctx >= 0) & (ctx < lt.shape[1]), ctx, -1).astype(np.int32).reshape(1, -1)
         ct = torch.as_tensor(ctx).to(self.device) if ctx.size else None
         u = torch.tensor([self._uniform(uniform)], dtype=torch.float32, device=self.device)
+        if min_p > 0.0 or lt.shape[1] > _lib.AF_SAMPLE_MAX_VOCAB:
+            return int(cuda_ops.sample_tokens(lt, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p,
+                                              repetition_penalty=repetition_penalty, context=ct).cpu()[0])
         return int(cuda_ops.sample_rows(lt, u, ct, temperature, top_k, top_p, repetition_penalty).cpu()[0])
 
     def sample_next_token(self, hidden_state, context_tokens, temperature: float = 0.7, top_k: int = 40,
-                          top_p: float = 0.9, repetition_penalty: float = 1.2, uniform=None) -> int:
+                          top_p: float = 0.9, repetition_penalty: float = 1.2, uniform=None,
+                          min_p: float = 0.0) -> int:
         """AceEngine.sample_next_token (cpu/mod.rs:349-394): final RMSNorm,
         LM head (the tied embedding unless one was loaded), then
         sample_token_from_logits."""
@@ -356,7 +362,7 @@ class AceEngine:
             raise ValueError(f"hidden_state length {h.size} must match d_model {self._d}")
         logits = self._logits(torch.as_tensor(h.reshape(1, -1)).to(self.device))
         return self.sample_token_from_logits(logits.cpu().numpy()[0], context_tokens, temperature, top_k, top_p,
-                                             repetition_penalty, uniform)
+                                             repetition_penalty, uniform, min_p)
 
     def prefill_device(self, x: torch.Tensor, T: int) -> None:
         """All layers over a [batch*T, d] fp32 device tensor of prompt
@@ -393,8 +399,8 @@ class AceEngine:
 
     def generate_batch(self, prompts, max_new_tokens: int, stop_at_eos: bool = False, teacher=None,
                        return_logits: bool = False, use_graph: bool = False, timing: dict | None = None,
-                       temperature: float = 0.0, top_k: int = 40, top_p: float = 0.9,
-                       repetition_penalty: float = 1.0, uniforms=None, seed: int | None = None):
+                       temperature=0.0, top_k=40, top_p=0.9, repetition_penalty=1.0, uniforms=None,
+                       seed: int | None = None, min_p=0.0):
         """Generation for `batch` streams: prompts [batch, P] ids.  Returns
         tokens [batch, max_new_tokens] (-1 after a stream stopped at EOS id 2
         when stop_at_eos) and optionally the logits per step.  `teacher`
@@ -404,9 +410,13 @@ class AceEngine:
         (af_sample_rows) over the last 60 ids of prompt + output, as
         generate_stream_internal does (cpu/mod.rs:739-746), with draws from
         `uniforms` [batch, max_new_tokens] in [0, 1), else from a torch
-        generator seeded with `seed`."""
+        generator seeded with `seed`.  temperature, top_k, top_p, min_p and
+        repetition_penalty are one number for all streams or one per stream
+        [batch]; per-stream settings, a min_p (not in the reference) and
+        vocabularies beyond af_sample_rows' run af_sample_tokens."""
         self._check_generate()
-        sampling = temperature > 1e-4 or repetition_penalty != 1.0
+        sampling = bool(np.any(np.asarray(temperature) > 1e-4) or np.any(np.asarray(repetition_penalty) != 1.0))
+        filters = self._filters(temperature, top_k, top_p, min_p, repetition_penalty) if sampling else None
         pr = torch.as_tensor(np.asarray(prompts, np.int32)).to(self.device)
         B, P = pr.shape
         if B != self.batch:
@@ -454,6 +464,10 @@ class AceEngine:
                 w0 = max(0, n_seen - self.PENALTY_WINDOW)
                 win = seen[:, w0:n_seen]
                 ur = uni[:, s].contiguous()
+            if sampling and filters is not None:
+                toks = cuda_ops.sample_tokens(logits, ur, context=win if n_seen else None, **filters)
+                seen[:, n_seen] = toks
+            elif sampling:
                 _lib.call("af_sample_rows", self._ctx(), logits.data_ptr(), B, V, win.data_ptr() if n_seen else None,
                           seen.stride(0), n_seen - w0, float(temperature), int(top_k), float(top_p),
                           float(repetition_penalty), ur.data_ptr(), toks.data_ptr(), st)
@@ -474,6 +488,27 @@ class AceEngine:
         if return_logits:
             return res, torch.stack(all_logits, 1).cpu().numpy()
         return res
+
+    def _filters(self, temperature, top_k, top_p, min_p, repetition_penalty):
+        """sample_tokens' settings, those given per stream on the device; None
+        where af_sample_rows (one setting for all, no min_p) will do."""
+        given = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p,
+                     repetition_penalty=repetition_penalty)
+        out = {}
+        for name, v in given.items():
+            if np.ndim(v) == 0:
+                out[name] = int(v) if name == "top_k" else float(v)
+                continue
+            a = np.asarray(v, np.int32 if name == "top_k" else np.float32).reshape(-1)
+            if a.size != self.batch:
+                raise ValueError(f"{name}: expected one value or {self.batch}, got {a.size}")
+            if name == "repetition_penalty" and not np.all(a > 0):
+                raise ValueError("repetition_penalty must be positive")
+            out[name] = torch.from_numpy(np.ascontiguousarray(a)).to(self.device)
+        if (not any(isinstance(v, torch.Tensor) for v in out.values()) and not out["min_p"] > 0.0
+                and self.vocab_size <= _lib.AF_SAMPLE_MAX_VOCAB):
+            return None
+        return out
 
     def _generate_graph(self, cur, logits, toks, out, head, bf, n, timing):
         """Greedy decode with each step (embed, all layers, LM head, argmax)
@@ -517,7 +552,7 @@ class AceEngine:
 
     def generate_stream(self, prompt_tokens: Sequence[int], max_new_tokens: int, temperature: float = 0.7,
                         top_k: int = 40, top_p: float = 0.9, repetition_penalty: float = 1.2,
-                        seed: int | None = None) -> List[int]:
+                        seed: int | None = None, min_p: float = 0.0) -> List[int]:
         """AceEngine.generate_stream (cpu/mod.rs:454-484) for a one-stream
         engine: the reference's sampling (or greedy at temperature <= 1e-4
         without penalty); stops after EOS id 2 like the reference.  `seed`
@@ -526,7 +561,8 @@ class AceEngine:
         if self.batch != 1:
             raise ValueError("generate_stream drives one stream; use generate_batch")
         toks = self.generate_batch([list(prompt_tokens)], max_new_tokens, stop_at_eos=True, temperature=temperature,
-                                   top_k=top_k, top_p=top_p, repetition_penalty=repetition_penalty, seed=seed)[0]
+                                   top_k=top_k, top_p=top_p, repetition_penalty=repetition_penalty, seed=seed,
+                                   min_p=min_p)[0]
         res = []
         for t in toks:
             if t < 0:

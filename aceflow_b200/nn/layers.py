@@ -1,4 +1,5 @@
-"""Linear / RMSNorm / LayerNorm / SwiGLU (mirrors aceflow/nn/layers.py:11-88).
+"""Linear / RMSNorm / LayerNorm / SwiGLU (mirrors aceflow/nn/layers.py:11-88),
+and ResidualNorm and Rotary, which the reference lacks.
 
 Initialisation draws from ``np.random`` in the reference's order, so a
 seeded script builds identical weights with either package.  On a CUDA
@@ -8,7 +9,7 @@ numpy formulas apply unchanged.
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import Optional, Tuple
 
 import numpy as np
 
@@ -61,6 +62,104 @@ class RMSNorm(Module):
         arr = x.numpy()
         rms = np.sqrt(np.mean(np.square(arr), axis=-1, keepdims=True) + self.eps)
         return Tensor((arr / rms) * self.weight.numpy(), x.device)
+
+
+class ResidualNorm(Module):
+    """The seam between two blocks of a layer: the norm behind a block, its
+    gate and residual scale, the residual add and the norm in front of the next
+    block (an extension; the reference has the last two alone,
+    aceflow-core/src/cpu/mod.rs:672-700):
+
+        n = RMSNorm(h) * post_weight            (with post_norm, else h)
+        z = alpha * x + scale * swish(gate) * n  (scale with layer_scale; gate when given)
+        y = RMSNorm(z) * pre_weight
+
+    forward(x, h, gate=None) returns (z, y): the residual stream for the next
+    seam and the next block's input.  On CUDA it is one kernel
+    (af_residual_norm), x and h fp32 or bf16 each (y in h's dtype);
+    cuda_ops.residual_norm_autograd is its differentiable form."""
+
+    def __init__(self, d_model: int, eps: float = 1e-6, *, post_norm: bool = True,
+                 layer_scale: Optional[float] = None, alpha: float = 1.0):
+        super().__init__()
+        self.d_model = d_model
+        self.eps = eps
+        self.alpha = float(alpha)
+        self.pre_weight = Parameter(Tensor(np.ones(d_model, dtype=np.float32)))
+        self.post_weight = Parameter(Tensor(np.ones(d_model, dtype=np.float32))) if post_norm else None
+        self.scale = (None if layer_scale is None
+                      else Parameter(Tensor(np.full(d_model, layer_scale, dtype=np.float32))))
+
+    def forward(self, x: Tensor, h: Tensor, gate: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+        from ..ops.functional import residual_norm
+
+        return residual_norm(x, h, self.pre_weight, post_weight=self.post_weight, scale=self.scale, gate=gate,
+                             alpha=self.alpha, eps=self.eps)
+
+
+class Rotary(Module):
+    """Rotary positions for queries and keys (an extension; RetNet's rotation,
+    Sun et al. 2023, eq. 5): turns the first rotary_dim values (all of them by
+    default) of every head by position * inv_freq.  layout "interleaved" pairs
+    values (2i, 2i + 1), "half" (i, i + rotary_dim / 2); base, scaling, factor and
+    original_length as for cuda_ops.rotary_frequencies.
+
+    forward(x, positions=0): x [B, T, heads, head_dim] or [rows, heads, head_dim],
+    positions the first token's position or an integer array [T] or [B, T]
+    ([rows] for a 3-D x)."""
+
+    def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, base: float = 10000.0, *,
+                 layout: str = "interleaved", scaling: Optional[str] = None, factor: float = 1.0,
+                 original_length: Optional[int] = None):
+        super().__init__()
+        ops = _cuda_ops()
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        if layout not in ops.ROTARY_LAYOUTS:
+            raise ValueError(f"layout must be one of {ops.ROTARY_LAYOUTS}, got {layout!r}")
+        if rotary_dim > head_dim:
+            raise ValueError(f"rotary_dim ({rotary_dim}) exceeds head_dim ({head_dim})")
+        self.head_dim = head_dim
+        self.layout = layout
+        self.inv_freq, self.scale = ops.rotary_frequencies(rotary_dim, base, scaling=scaling, factor=factor,
+                                                           original_length=original_length)
+        self._on = {}  # inv_freq on each device it was used on
+
+    def turn(self, x, positions=0, inplace: bool = False):
+        """The CUDA form on torch tensors (af_rotary)."""
+        import torch
+
+        f = self._on.get(x.device)
+        if f is None:
+            f = self._on[x.device] = self.inv_freq.to(x.device)
+        if not isinstance(positions, (int, np.integer)):
+            if not isinstance(positions, torch.Tensor):
+                positions = torch.as_tensor(np.asarray(positions))
+            positions = positions.to(x.device)
+        return _cuda_ops().rotary(x, f, positions, layout=self.layout, scale=self.scale, inplace=inplace)
+
+    def turn_numpy(self, x: np.ndarray, positions=0) -> np.ndarray:
+        """The same formula on the host, angles in 64 bits."""
+        if isinstance(positions, (int, np.integer)):
+            positions = int(positions) + np.arange(x.shape[-3])
+        th = np.asarray(positions, np.float64)[..., None, None] * self.inv_freq.numpy().astype(np.float64)
+        cos, sin = (self.scale * f(th) for f in (np.cos, np.sin))
+        half = self.inv_freq.numel()
+        if self.layout == "interleaved":
+            first, second = slice(0, 2 * half, 2), slice(1, 2 * half, 2)
+        else:
+            first, second = slice(0, half), slice(half, 2 * half)
+        a, b = x[..., first], x[..., second]
+        out = x.copy()
+        out[..., first] = a * cos - b * sin
+        out[..., second] = a * sin + b * cos
+        return out
+
+    def forward(self, x: Tensor, positions=0) -> Tensor:
+        if x.shape[-1] != self.head_dim:
+            raise ValueError(f"heads of {x.shape[-1]} values, expected {self.head_dim}")
+        if x.device.is_cuda:
+            return Tensor._wrap(self.turn(x.torch, positions), x.device)
+        return Tensor(self.turn_numpy(x.numpy(), positions), x.device)
 
 
 class LayerNorm(Module):

@@ -36,6 +36,13 @@ W_o^T with O the reference's retention; the group norm (per head: mean 0,
 variance 1, eps of ret_norm, then group_norm_weight / group_norm_bias) takes
 the place of ret_norm.  w_g is drawn after the reference's four weights, so
 a seeded gated module has the same w_q, w_k, w_v, w_o as an ungated one.
+
+rotary=nn.Rotary(head_dim, ...) (an extension as well): RetNet turns queries
+and keys by their position before the retention (Sun et al. 2023, eq. 5).
+The prompt methods then take `position`, that of x's first token (a number, or
+an integer array [T] or [B, T]); forward_recurrent takes each stream's [B] (or
+one number for all), and needs it.  The state holds turned keys, so a prompt
+hands over to decode as before.
 """
 from __future__ import annotations
 
@@ -45,7 +52,7 @@ from typing import Optional, Tuple
 import numpy as np
 
 from ..core.tensor import Tensor
-from .layers import RMSNorm
+from .layers import RMSNorm, Rotary
 from .module import Module, Parameter
 
 TC_HEAD_DIM = 256   # head_dim of the tensor-core chunkwise kernel
@@ -55,12 +62,15 @@ DEFAULT_CHUNK = 64  # tokens per chunk of the chunkwise prefill
 class MultiScaleRetention(Module):
     """Multi-Scale Retention (MSR) layer."""
 
-    def __init__(self, d_model: int, num_heads: int, *, prefill_dtype: Optional[str] = None, gated: bool = False):
+    def __init__(self, d_model: int, num_heads: int, *, prefill_dtype: Optional[str] = None, gated: bool = False,
+                 rotary: Optional[Rotary] = None):
         super().__init__()
         if prefill_dtype not in (None, "float32", "bfloat16"):
             raise ValueError("prefill_dtype must be None, 'float32' or 'bfloat16'")
         if num_heads <= 0 or d_model % num_heads != 0:
             raise ValueError(f"d_model ({d_model}) must be divisible by num_heads ({num_heads})")
+        if rotary is not None and rotary.head_dim != d_model // num_heads:
+            raise ValueError(f"rotary turns heads of {rotary.head_dim} values, the layer's have {d_model // num_heads}")
         self.d_model = d_model
         self.num_heads = num_heads
         self.head_dim = d_model // num_heads
@@ -71,6 +81,7 @@ class MultiScaleRetention(Module):
         self.w_v = Parameter(Tensor(np.random.uniform(-k, k, (d_model, d_model)).astype(np.float32)))
         self.w_o = Parameter(Tensor(np.random.uniform(-k, k, (d_model, d_model)).astype(np.float32)))
         self.ret_norm = RMSNorm(d_model)
+        self.rotary = rotary
         self.gated = bool(gated)
         if self.gated:
             self.w_g = Parameter(Tensor(np.random.uniform(-k, k, (d_model, d_model)).astype(np.float32)))
@@ -148,12 +159,23 @@ class MultiScaleRetention(Module):
     def _use_tensor_cores(self, x: Tensor) -> bool:
         return x.dtype == "bfloat16" or (self.prefill_dtype == "bfloat16" and self.head_dim == TC_HEAD_DIM)
 
-    def forward_parallel(self, x: Tensor) -> Tensor:
+    def _check_position(self, position) -> None:
+        if self.rotary is None and not (isinstance(position, (int, np.integer)) and position == 0):
+            raise ValueError("a position without rotary=: this layer knows none")
+
+    def _turn(self, qkv, B: int, T: int, position) -> None:
+        """Turns q and k inside a packed device qkv [B*T, 3d], in place."""
+        if self.rotary is not None:
+            heads = qkv.view(B, T, 3 * self.num_heads, self.head_dim)
+            self.rotary.turn(heads[:, :, :2 * self.num_heads], position, inplace=True)
+
+    def forward_parallel(self, x: Tensor, position=0) -> Tensor:
+        self._check_position(position)
         if x.device.is_cuda:
             if self._use_tensor_cores(x):
-                out, _ = self._prefill_tensor_cores(x, self.prefill_chunk, None, want_state=False)
+                out, _ = self._prefill_tensor_cores(x, self.prefill_chunk, None, want_state=False, position=position)
             else:
-                out, _ = self._prefill_exact(x, None)
+                out, _ = self._prefill_exact(x, None, position)
             return out
         arr = x.numpy()
         b, n, d = arr.shape
@@ -161,6 +183,8 @@ class MultiScaleRetention(Module):
         q = np.matmul(arr, self.w_q.numpy().T).reshape(b, n, H, hd).transpose(0, 2, 1, 3)
         k = np.matmul(arr, self.w_k.numpy().T).reshape(b, n, H, hd).transpose(0, 2, 1, 3)
         v = np.matmul(arr, self.w_v.numpy().T).reshape(b, n, H, hd).transpose(0, 2, 1, 3)
+        if self.rotary is not None:
+            q, k = (self.rotary.turn_numpy(a.transpose(0, 2, 1, 3), position).transpose(0, 2, 1, 3) for a in (q, k))
         idx = np.arange(n)
         dist = idx[:, None] - idx[None, :]
         decay = np.zeros((H, n, n), dtype=np.float32)
@@ -173,28 +197,32 @@ class MultiScaleRetention(Module):
         normed = self.ret_norm(Tensor(out, x.device))
         return Tensor(np.matmul(normed.numpy(), self.w_o.numpy().T), x.device)
 
-    def forward(self, x: Tensor) -> Tensor:
-        return self.forward_parallel(x)
+    def forward(self, x: Tensor, position=0) -> Tensor:
+        return self.forward_parallel(x, position)
 
-    def forward_chunkwise(self, x: Tensor, chunk: int = DEFAULT_CHUNK,
-                          state: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    def forward_chunkwise(self, x: Tensor, chunk: int = DEFAULT_CHUNK, state: Optional[Tensor] = None,
+                          position=0) -> Tuple[Tensor, Tensor]:
         """Prefill x [B, T, d] from `state` (zeros if None) in chunks of
         `chunk` tokens; returns the layer output and the state after the last
         token.  On CUDA this is the tcgen05 chunkwise kernel (bf16 operands,
         fp32 accumulation and state; head_dim 256); on CPU the recurrence."""
         B, T, d = x.shape
+        self._check_position(position)
         if not x.device.is_cuda:
             if state is None:
                 state = self.init_state(B, x.device)
             outs = []
+            at = position + np.arange(T) if isinstance(position, (int, np.integer)) else np.asarray(position)
+            at = np.broadcast_to(at, (B, T))
             for t in range(T):
-                o, state = self.forward_recurrent(Tensor(x.numpy()[:, t]), state)
+                o, state = self.forward_recurrent(Tensor(x.numpy()[:, t]), state,
+                                                  at[:, t] if self.rotary is not None else None)
                 outs.append(o.numpy())
             return Tensor(np.stack(outs, 1), x.device), state
-        return self._prefill_tensor_cores(x, chunk, state, want_state=True)
+        return self._prefill_tensor_cores(x, chunk, state, want_state=True, position=position)
 
-    def _prefill_tensor_cores(self, x: Tensor, chunk: int, state: Optional[Tensor],
-                              want_state: bool) -> Tuple[Tensor, Optional[Tensor]]:
+    def _prefill_tensor_cores(self, x: Tensor, chunk: int, state: Optional[Tensor], want_state: bool,
+                              position=0) -> Tuple[Tensor, Optional[Tensor]]:
         """af_msr_prefill_bf16 on x [B, T, d] (bf16, or fp32 cast to bf16 on
         the device); output in x's dtype, final state fp32."""
         import torch
@@ -209,7 +237,9 @@ class MultiScaleRetention(Module):
             st_in = state.torch
             if st_in.dtype != torch.float32 or not st_in.is_contiguous() or st_in.device != xt.device:
                 raise ValueError("state must be a contiguous fp32 tensor on the input's device")
-        if self.gated:
+        if self.rotary is not None:
+            out, st = self._prefill_turned(xb, p, st_in, xt.dtype, want_state, chunk, position)
+        elif self.gated:
             gw, gb = self._gn_params()
             out, st = cuda_ops.msr_gated_prefill_bf16(xb, p["w_qkv_bf16"], p["w_g_bf16"], p["w_o_bf16"], gw, gb,
                                                       p["gamma"], self.ret_norm.eps, state_in=st_in,
@@ -220,7 +250,34 @@ class MultiScaleRetention(Module):
                                                 want_state=want_state, chunk=chunk)
         return Tensor._wrap(out, x.device), (Tensor._wrap(st, x.device) if st is not None else None)
 
-    def _prefill_exact(self, x: Tensor, state: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
+    def _prefill_turned(self, xb, p: dict, state, out_dtype, want_state: bool, chunk: int, position):
+        """The tensor-core prefill with the rotation between the QKV product
+        and the chunkwise kernel (which read and write the same packed bf16
+        qkv); bf16 q and k are rounded once more by it."""
+        import torch
+
+        from .. import cuda_ops
+
+        B, T, d = xb.shape
+        H, eps = self.num_heads, self.ret_norm.eps
+        rows = xb.view(B * T, d)
+        qkv = cuda_ops.linear_bf16(rows, p["w_qkv_bf16"], out_dtype=torch.bfloat16)
+        self._turn(qkv, B, T, position)
+        if self.gated:
+            o, _, st = cuda_ops.retention_chunkwise_bf16(qkv, B, T, H, p["gamma"], state, want_state=want_state,
+                                                         chunk=chunk)
+            g = cuda_ops.linear_bf16(rows, p["w_g_bf16"], out_dtype=torch.bfloat16)
+            gw, gb = self._gn_params()
+            out = cuda_ops.linear_bf16(cuda_ops.group_norm_gate(o, g, H, gw, gb, eps), p["w_o_bf16"],
+                                       out_dtype=out_dtype)
+        else:
+            o, sumsq, st = cuda_ops.retention_chunkwise_bf16(qkv, B, T, H, p["gamma"], state,
+                                                             self.ret_norm.weight.torch, want_state, chunk)
+            out = torch.empty(B * T, d, dtype=out_dtype, device=xb.device)
+            cuda_ops.gemm_bf16(o, p["w_o_bf16"], out, row_sumsq=sumsq, inv_d=1.0 / d, eps=eps)
+        return out.view(B, T, d), st
+
+    def _prefill_exact(self, x: Tensor, state: Optional[Tensor], position=0) -> Tuple[Tensor, Tensor]:
         """The fp32 path: QKV GEMM (3xTF32), the recurrence token by token
         (af_retention_scan, as AceEngine.prefill_recurrent), RMSNorm, W_o GEMM."""
         from .. import cuda_ops
@@ -233,6 +290,7 @@ class MultiScaleRetention(Module):
         p = self._packed(x)
         st = state.torch
         qkv = cuda_ops.linear(x.torch.reshape(B * T, d), p["w_qkv"]).reshape(B, T, 3 * d)
+        self._turn(qkv, B, T, position)
         o = cuda_ops.retention_scan(st, p["gamma"], qkv[:, :, :d], qkv[:, :, d:2 * d], qkv[:, :, 2 * d:])
         if self.gated:
             g = cuda_ops.linear(x.torch.reshape(B * T, d), p["w_g"]).reshape(B, T, d)
@@ -243,16 +301,23 @@ class MultiScaleRetention(Module):
         out = cuda_ops.linear(normed, p["w_o"])
         return Tensor._wrap(out, x.device), state
 
-    def forward_recurrent(self, x_t: Tensor, state: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    def forward_recurrent(self, x_t: Tensor, state: Optional[Tensor] = None,
+                          position=None) -> Tuple[Tensor, Tensor]:
         """One decode step for B streams: x_t [B, d] -> ([B, d], state)."""
         B, d = x_t.shape
+        if (position is None) != (self.rotary is None):
+            raise ValueError("a layer with rotary= needs the streams' position, one without takes none")
+        if position is not None and isinstance(position, (int, np.integer)):
+            position = np.full(B, position, np.int64)
         if state is None:
             state = self.init_state(B, x_t.device)
         if x_t.device.is_cuda:
             from .. import cuda_ops
 
             p = self._packed(x_t)
-            if self.gated:
+            if self.rotary is not None:
+                out = self._decode_turned(x_t.torch.contiguous(), state.torch, p, position)
+            elif self.gated:
                 gw, gb = self._gn_params()
                 out = cuda_ops.msr_gated_decode_step(x_t.torch.contiguous(), state.torch, p["gamma"], p["w_qkv"],
                                                      p["w_g"], p["w_o"], gw, gb, self.ret_norm.eps)
@@ -265,8 +330,9 @@ class MultiScaleRetention(Module):
             return Tensor._wrap(out, x_t.device), state
         H, hd = self.num_heads, self.head_dim
         arr = x_t.numpy()
-        q = (arr @ self.w_q.numpy().T).reshape(B, H, hd)
-        k = (arr @ self.w_k.numpy().T).reshape(B, H, hd)
+        turned = (lambda a: a) if self.rotary is None else (lambda a: self.rotary.turn_numpy(a, position))
+        q = turned((arr @ self.w_q.numpy().T).reshape(B, H, hd))
+        k = turned((arr @ self.w_k.numpy().T).reshape(B, H, hd))
         v = (arr @ self.w_v.numpy().T).reshape(B, H, hd)
         S = state.numpy()
         S = self.gamma[None, :, None, None] * S + k[:, :, :, None] * v[:, :, None, :]
@@ -276,3 +342,21 @@ class MultiScaleRetention(Module):
                     Tensor(S.astype(np.float32), x_t.device))
         normed = self.ret_norm(Tensor(o, x_t.device))
         return Tensor(normed.numpy() @ self.w_o.numpy().T, x_t.device), Tensor(S.astype(np.float32), x_t.device)
+
+    def _decode_turned(self, x, state, p: dict, position):
+        """One decode step with the rotation between the projection and the
+        state's update (positions may be a device tensor, so that a captured
+        step moves on by itself)."""
+        from .. import cuda_ops
+
+        B, d = x.shape
+        H, eps = self.num_heads, self.ret_norm.eps
+        qkv = cuda_ops.linear(x, p["w_qkv"])
+        self.rotary.turn(qkv.view(B, 3 * H, self.head_dim)[:, :2 * H], position, inplace=True)
+        o = cuda_ops.retention_step(state, p["gamma"], qkv[:, :d], qkv[:, d:2 * d], qkv[:, 2 * d:])
+        if self.gated:
+            gw, gb = self._gn_params()
+            normed = cuda_ops.group_norm_gate(o, cuda_ops.linear(x, p["w_g"]), H, gw, gb, eps)
+        else:
+            normed = cuda_ops.rms_norm(o, self.ret_norm.weight.torch, eps)
+        return cuda_ops.linear(normed, p["w_o"])

@@ -1,3 +1,3 @@
-from .functional import gelu, matmul, rms_norm, silu, softmax, swiglu
+from .functional import gelu, matmul, residual_norm, rms_norm, rotary, silu, softmax, swiglu
 
-__all__ = ["matmul", "rms_norm", "swiglu", "gelu", "silu", "softmax"]
+__all__ = ["matmul", "rms_norm", "residual_norm", "rotary", "swiglu", "gelu", "silu", "softmax"]

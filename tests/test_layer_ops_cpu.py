@@ -111,3 +111,53 @@ def test_oracle_rotary_turns_back():
         y = L.rotary64(x, f, 7 + np.arange(5), layout, 2.0)
         assert np.allclose(L.rotary64(y, f, 7 + np.arange(5), layout, 0.5, True), x)
         assert np.array_equal(y[..., 6:], x[..., 6:])
+
+
+def test_modules_on_the_cpu():
+    """nn.Rotary, nn.ResidualNorm and a rotated MultiScaleRetention: the parallel
+    form, the recurrence and the prompt in two parts agree."""
+    import aceflow_b200 as af
+
+    rng = np.random.default_rng(6)
+    rot = af.nn.Rotary(16, 8, layout="half", scaling="linear", factor=2.0)
+    x = rng.standard_normal((2, 5, 3, 16)).astype(np.float32)
+    ref = L.rotary64(x, rot.inv_freq.numpy(), 3 + np.arange(5), "half")
+    assert np.max(np.abs(rot(af.Tensor(x), 3).numpy() - ref)) < 1e-6
+    assert list(rot.parameters()) == []
+    np.random.seed(9)
+    m = af.nn.MultiScaleRetention(64, 4, rotary=af.nn.Rotary(16))
+    np.random.seed(9)
+    assert np.array_equal(m.w_q.numpy(), af.nn.MultiScaleRetention(64, 4).w_q.numpy())
+    t = rng.standard_normal((2, 9, 64)).astype(np.float32)
+    full = m(af.Tensor(t), 40).numpy()
+    a, st = m.forward_chunkwise(af.Tensor(t[:, :4]), position=40)
+    b, st = m.forward_chunkwise(af.Tensor(t[:, 4:]), state=st, position=44)
+    assert np.max(np.abs(np.concatenate([a.numpy(), b.numpy()], 1) - full)) < 1e-5
+    assert np.max(np.abs(m(af.Tensor(t), 900).numpy() - full)) < 1e-4  # relative positions alone matter
+    assert np.max(np.abs(m(af.Tensor(t), np.arange(9) * 3).numpy() - full)) > 1e-3
+    s = af.nn.ResidualNorm(64, layer_scale=0.1)
+    z, y = s(af.Tensor(t), af.Tensor(full))
+    want, _ = L.seam64(t, full, None, np.ones(64), np.full(64, 0.1), np.ones(64))
+    assert np.max(np.abs(z.numpy() - want["z"])) < 1e-5 and np.max(np.abs(y.numpy() - want["y"])) < 1e-5
+    assert [n for n, _ in s.named_parameters()] == ["pre_weight", "post_weight", "scale"]
+
+
+def test_module_refusals():
+    import aceflow_b200 as af
+
+    with pytest.raises(ValueError, match="rotary"):
+        af.nn.MultiScaleRetention(64, 4, rotary=af.nn.Rotary(32))
+    with pytest.raises(ValueError, match="exceeds"):
+        af.nn.Rotary(16, 18)
+    with pytest.raises(ValueError, match="layout"):
+        af.nn.Rotary(16, layout="both")
+    plain, turned = af.nn.MultiScaleRetention(64, 4), af.nn.MultiScaleRetention(64, 4, rotary=af.nn.Rotary(16))
+    x = af.Tensor(np.zeros((2, 3, 64)))
+    with pytest.raises(ValueError, match="position"):
+        plain(x, 5)
+    with pytest.raises(ValueError, match="position"):
+        plain.forward_recurrent(af.Tensor(np.zeros((2, 64))), None, 5)
+    with pytest.raises(ValueError, match="position"):
+        turned.forward_recurrent(af.Tensor(np.zeros((2, 64))))
+    with pytest.raises(ValueError, match="CUDA"):
+        af.ops.rotary(x, af.Tensor(np.ones(4)))
