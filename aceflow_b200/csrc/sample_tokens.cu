@@ -13,16 +13,16 @@
 // first place where F >= u M.  The row is never sorted.  A cluster of CTAs
 // holds it in shared memory, one slice each (one read of the logits), and
 //   1. finds the maximum;
-//   2. with top-k: counts the tokens in bins of 1/16 octave of w and takes the
-//      bins through the one that holds the k-th; else: sums w, which bounds
-//      from below the w of any token that can still matter (a token below
-//      (1 - top_p) Z / V lies behind the crossing: all such tokens together
-//      weigh less than (1 - top_p) Z);
-//   3. if at most kList tokens are left, the first CTA reads the places off
+//   2. with top-k: counts the tokens in bins of 1/16 octave of w and takes
+//      those through the bin that holds the k-th; with min-p alone: takes what
+//      it may keep;
+//   3. if at most kList tokens were taken, the first CTA reads the places off
 //      them: it sums their masses by bins, finds a place's bin from the running
-//      sum and sorts that bin's few tokens; this is the usual case;
-//   4. else (a broad nucleus) the row's masses go into the bins, and the first
-//      CTA gets a place's bin alone and does the same in finer ones;
+//      sum and orders that bin's few tokens;
+//   4. without top-k: the row's masses go into the bins.  Their running sums
+//      give Z and the bin where top-p is crossed, and that bin's two ends the
+//      few bins where the draw can end; the first CTA gets the tokens of all
+//      these at once and finds both places, each by finer bins of one bin;
 //   5. else (a bin of more than kList tokens: great numbers of equal or nearly
 //      equal logits, or a top_k above kList) every place is found by
 //      descending the digits of its key over histograms.
@@ -31,11 +31,17 @@
 // than 2^-29 of itself off), in 64 bits: their sums do not depend on any
 // order, so a row's token is the same in every run and in every launch shape.
 //
-// Bound: a long row by instructions (about 35 per token for the mass; two
-// histogram additions where step 4 runs), a short one by the chain of cluster
-// barriers and the latency of 64-bit arithmetic.
+// Bound: one read of the logits would take 20.5 us for 256 rows of 131072 in
+// fp32; with top-p 0.95 over a broad row the call takes 183 us: in 7 waves of
+// clusters, each a chain of about 48000 cycles (8300 to load, 9300 for the
+// masses, the rest barriers, scans and the first CTA's search).  Summing Z in
+// a pass of its own, with a second one for the bins and a collection for each
+// place, took 365 us.  Few rows are bound by the chain alone: 12.4 us for one
+// row of 32000 with top-k 40, 23 us for 64 such rows with mixed settings.
 #include "common.cuh"
 #include "sm100.cuh"
+
+#include <algorithm>
 
 namespace {
 
@@ -46,9 +52,11 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCtas = 8;       // CTAs of a row's cluster
 constexpr int kList = 2048;       // tokens the first CTA takes over at once
 constexpr int kSome = 512;        // of them, those of one bin that are sorted at once
-constexpr int kAlone = 64;        // tokens that one warp sorts alone
+constexpr int kPairs = 128;       // tokens that are compared each with each
 constexpr int kBins = 46 * 16;    // w down to 2^-46 in sixteenths of an octave; the rest behind them
 constexpr int kBinRoom = 2 * kThreads;
+constexpr int kWords = 3;         // words that hold a bit for each of a thread's tokens
+static_assert(kWords * 32 * kThreads * kMaxCtas >= AF_SAMPLE_TOKENS_MAX_VOCAB + 8 * kMaxCtas, "every token has a bit");
 constexpr u64 kOne = 1ull << 44;  // the mass of the largest logit
 constexpr float kLowest = -3.4028235e38f;
 
@@ -97,9 +105,10 @@ struct Layout {
   static constexpr uint32_t slot = power + 8 * 16;           // u64 [2][kMaxCtas]
   static constexpr uint32_t warp = slot + 8 * 2 * kMaxCtas;  // u64 [kWarps]
   static constexpr uint32_t before = warp + 8 * kWarps;      // u64 [2]
-  static constexpr uint32_t listed = before + 16;            // u32, then found
-  static constexpr uint32_t found = listed + 4;
-  static constexpr uint32_t logits = found + 12;  // float [slice]
+  static constexpr uint32_t listed = before + 16;            // u32
+  static constexpr uint32_t found = listed + 4;              // u32
+  static constexpr uint32_t settings = found + 4;             // u32 [5]
+  static constexpr uint32_t logits = settings + 24;           // float [slice]
 };
 static_assert(Layout::logits % 16 == 0, "logits are read sixteen bytes at a time");
 static_assert(16 * kBinRoom <= 8 * kList && 16 * kSome <= 8 * kBinRoom, "what shares the running masses' place fits");
@@ -193,7 +202,7 @@ struct Weigher {
   __device__ __forceinline__ static bool some(float t) { return t < 46.0f; }
   // floor(16 t): behind 1.5 * 2^23 a sum holds no fraction.
   __device__ __forceinline__ static int sixteenths(float t) {
-    return __float_as_int(__fadd_rd(t * 16.0f, 12582912.0f)) - 0x4b400000;
+    return __float_as_int(__fmaf_rd(t, 16.0f, 12582912.0f)) - 0x4b400000;
   }
   __device__ __forceinline__ int bin(float x) const {
     const float t = lead(x);
@@ -310,46 +319,60 @@ struct Row {
       f(__uint_as_float(v.z), 4 * i + 2), f(__uint_as_float(v.w), 4 * i + 3);
     }
   }
-  // Brings the tokens of the row whose logits lie in [lo, hi] and that `take`
-  // accepts onto the first CTA's list; returns their number, with nothing
-  // brought if it is above kList.  Threads count theirs first: the places follow
-  // from the counts, without atomics.  Ends with a cluster barrier.
+  // Brings the tokens of the row that `take` accepts to the first CTA's memory
+  // at `to`, in no order; returns their number, with nothing brought if it is
+  // above kList.  Ends with a cluster barrier.
   template <typename F>
-  __device__ unsigned collect(float lo, float hi, F &&take) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    unsigned mine = 0;
-    each([&](float x, int) { mine += x >= lo && x <= hi && take(x); });
-    unsigned through = mine;
+  __device__ unsigned bring(uint32_t to, F &&take) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n4 = (n + 3) / 4;
+    const uint32_t mine = sm + Layout::run;  // this CTA's, before their place is known
+    unsigned hits[kWords], through = 0;
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      hits[w] = 0;
+      const int i0 = threadIdx.x + 8 * w * kThreads;
+#pragma unroll 4
+      for (int j = 0; j < 8; ++j)
+        if (i0 + j * kThreads < n4) {
+          const uint4 v = lds128(sm + Layout::logits + 16 * (i0 + j * kThreads));
+          hits[w] |= ((unsigned)take(__uint_as_float(v.x)) | (unsigned)take(__uint_as_float(v.y)) << 1 |
+                      (unsigned)take(__uint_as_float(v.z)) << 2 | (unsigned)take(__uint_as_float(v.w)) << 3)
+                     << 4 * j;
+        }
+      through += __popc(hits[w]);
+    }
+    unsigned to_at = through;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned v = __shfl_up_sync(0xffffffffu, through, o);
       if (lane >= o) through += v;
     }
+    to_at = through - to_at;
     __syncthreads();
     if (lane == 31) sts32(sm + Layout::warp + 8 * warp, through);
     __syncthreads();
-    unsigned warps = lds32(sm + Layout::warp + 8 * (lane & (kWarps - 1)));
+    const unsigned of = lds32(sm + Layout::warp + 8 * (lane & (kWarps - 1)));
+    to_at += __reduce_add_sync(0xffffffffu, lane < warp ? of : 0);
+    const unsigned have = __reduce_add_sync(0xffffffffu, lane < kWarps ? of : 0);
 #pragma unroll
-    for (int o = 1; o < kWarps; o <<= 1) {
-      const unsigned v = __shfl_up_sync(0xffffffffu, warps, o, kWarps);
-      if ((lane & (kWarps - 1)) >= o) warps += v;
-    }
-    unsigned at = through - mine;
-    const unsigned prior = __shfl_sync(0xffffffffu, warps, warp ? warp - 1 : 0);
-    if (warp) at += prior;
-    const uint32_t slot = exchange(__shfl_sync(0xffffffffu, warps, kWarps - 1));
-    unsigned all = 0;
+    for (int w = 0; w < kWords; ++w)
+      for (; hits[w]; hits[w] &= hits[w] - 1) {
+        const int k = __ffs(hits[w]) - 1, i = 4 * (threadIdx.x + (8 * w + (k >> 2)) * kThreads) + (k & 3);
+        const float x = __uint_as_float(lds32(sm + Layout::logits + 4 * i));
+        if (to_at < kList) sts64(mine + 8 * to_at, (u64)~key_of(x) << 32 | (unsigned)(base + i));
+        ++to_at;
+      }
+    const uint32_t slot = exchange(have);
+    unsigned at = 0, all = 0;
 #pragma unroll
     for (int c = 0; c < kMaxCtas; ++c) {
-      const unsigned have = c < ctas ? (unsigned)lds64(slot + 8 * c) : 0;
-      all += have;
-      at += c < rank ? have : 0;
+      const unsigned v = c < ctas ? (unsigned)lds64(slot + 8 * c) : 0;
+      all += v;
+      at += c < rank ? v : 0;
     }
-    if (all <= kList && mine) {
-      const uint32_t list = in_cta(sm + Layout::list, 0);
-      each([&](float x, int i) {
-        if (x >= lo && x <= hi && take(x)) put_far64(list + 8 * at++, (u64)~key_of(x) << 32 | (unsigned)(base + i));
-      });
+    if (all <= kList) {
+      const uint32_t there = in_cta(to, 0) + 8 * at;
+      for (unsigned i = threadIdx.x; i < have; i += kThreads) put_far64(there + 8 * i, lds64(mine + 8 * i));
     }
     cluster_barrier();
     return all;
@@ -364,32 +387,55 @@ struct Row {
     red32(sm + Layout::lo + 4 * b, q & 0xffffu);
     red32(sm + Layout::hi + 4 * b, q >> 16);
   }
-  // Running sums over the bins: of this CTA, or (far) of the whole row, which
-  // the first CTA alone forms (all of them reading all others' bins took five
-  // times as long) and passes the answers on.  shift(b) < 0: counts.
-  template <bool far, typename S>
-  __device__ void run_bins(S &&shift) {
-    const uint32_t to = sm + (far ? Layout::bins : Layout::own_bins);
-    u64 before = 0;
-#pragma unroll
-    for (int i = 0; i < kBinRoom; i += kThreads) {
-      const int b = i + (int)threadIdx.x, s = shift(b);
-      u64 lo = 0, hi = 0;
-      if (far) {
-        uint32_t l[kMaxCtas], h[kMaxCtas];  // all loads under way before the first is used
-#pragma unroll
-        for (int c = 0; c < kMaxCtas; ++c) {
-          l[c] = c < ctas ? far32(in_cta(sm + Layout::lo + 4 * b, c)) : 0;
-          h[c] = c < ctas && s >= 0 ? far32(in_cta(sm + Layout::hi + 4 * b, c)) : 0;
-        }
-#pragma unroll
-        for (int c = 0; c < kMaxCtas; ++c) lo += l[c], hi += h[c];
-      } else {
-        lo = lds32(sm + Layout::lo + 4 * b), hi = lds32(sm + Layout::hi + 4 * b);
-      }
-      before = scan(s < 0 ? lo : ((hi << 16) + lo) << s, before, to + 8 * b);
-    }
+  __device__ __forceinline__ static u64 in_bin(u64 lo, u64 hi, int s) { return s < 0 ? lo : ((hi << 16) + lo) << s; }
+  // Running sums over kBinRoom bins, two neighbours a thread.
+  __device__ void run_sums(u64 a, u64 b, uint32_t to) {
+    to += 16 * threadIdx.x;
+    scan(a + b, 0, to + 8);
+    sts64(to, lds64(to + 8) - b);
     __syncthreads();
+  }
+  // Of this CTA's bins.
+  template <typename S>
+  __device__ void run_own_bins(S &&shift) {
+    const int b = 2 * threadIdx.x;
+    const uint32_t lo = sm + Layout::lo + 4 * b, hi = sm + Layout::hi + 4 * b;
+    run_sums(in_bin(lds32(lo), lds32(hi), shift(b)), in_bin(lds32(lo + 4), lds32(hi + 4), shift(b + 1)),
+             sm + Layout::own_bins);
+  }
+  // Of the whole row's, on every CTA: each CTA adds up its share of the bins
+  // over all CTAs and gives the sums to all.  shift(b) < 0: counts.  Returns the
+  // sum of `also` over the CTAs.
+  template <typename S>
+  __device__ u64 run_bins(u64 also, S &&shift) {
+    const uint32_t slot = exchange(also), to = sm + Layout::bins;
+    const int share = (kBins + ctas - 1) / ctas;
+    for (int i = threadIdx.x; i < share; i += kThreads) {
+      const int b = rank * share + i, s = shift(b);
+      if (b >= kBins) break;
+      uint32_t l[kMaxCtas], h[kMaxCtas];  // all loads under way before the first is used
+#pragma unroll
+      for (int c = 0; c < kMaxCtas; ++c) {
+        l[c] = c < ctas ? far32(in_cta(sm + Layout::lo + 4 * b, c)) : 0;
+        h[c] = c < ctas && s >= 0 ? far32(in_cta(sm + Layout::hi + 4 * b, c)) : 0;
+      }
+      u64 lo = 0, hi = 0;
+#pragma unroll
+      for (int c = 0; c < kMaxCtas; ++c) lo += l[c], hi += h[c];
+      const u64 v = in_bin(lo, hi, s);
+#pragma unroll
+      for (int c = 0; c < kMaxCtas; ++c)
+        if (c < ctas) put_far64(in_cta(to + 8 * b, c), v);
+    }
+    cluster_barrier();
+    const int b = 2 * threadIdx.x;
+    static_assert(kBins % 2 == 0, "a thread's two bins are both used or neither");
+    const u64 v = b < kBins ? lds64(to + 8 * b) : 0, w = b < kBins ? lds64(to + 8 * b + 8) : 0;
+    run_sums(v, w, to);
+    u64 sum = 0;
+#pragma unroll
+    for (int c = 0; c < kMaxCtas; ++c) sum += c < ctas ? lds64(slot + 8 * c) : 0;
+    return sum;
   }
   __device__ __forceinline__ u64 through_bin(int b, uint32_t of = Layout::bins) const {
     return b < 0 ? 0 : lds64(sm + of + 8 * b);
@@ -403,6 +449,19 @@ struct Row {
   }
 
   // ---- in one CTA
+  // Of m entries, those that `take` accepts onto this CTA's list; their number.
+  template <typename F>
+  __device__ int select(uint32_t from, int m, F &&take) {
+    __syncthreads();  // what was on the list has been read
+    if (threadIdx.x == 0) sts32(sm + Layout::listed, 0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < m; i += kThreads) {
+      const u64 e = lds64(from + 8 * i);
+      if (take(logit_of(e))) sts64(sm + Layout::list + 8 * add32(sm + Layout::listed, 1), e);
+    }
+    __syncthreads();
+    return (int)lds32(sm + Layout::listed);
+  }
   // Running sum over the CTA's threads behind `before`, into `to`; returns the total.
   __device__ u64 scan(u64 v, u64 before, uint32_t to) {
     const int lane = threadIdx.x & 31;
@@ -483,66 +542,30 @@ struct Row {
     __syncthreads();
   }
   __device__ __forceinline__ static float logit_of(u64 entry) { return value_of((uint32_t)~(entry >> 32)); }
-  // The same for up to 32 E places in one warp, and the running mass.
-  template <int E, typename W>
-  __device__ __forceinline__ void order_alone(uint32_t list, uint32_t run, int m, const W &weigh) {
-    const int lane = threadIdx.x, first = E * lane;
-    u64 v[E], w[E];
-#pragma unroll
-    for (int r = 0; r < E; ++r) v[r] = first + r < m ? lds64(list + 8 * (first + r)) : ~0ull;
-#pragma unroll
-    for (int k = 2; k <= 32 * E; k <<= 1) {
-#pragma unroll
-      for (int j = k >> 1; j; j >>= 1) {
-        if (j >= E) {
-          const bool small = ((first & j) == 0) == ((first & k) == 0);
-#pragma unroll
-          for (int r = 0; r < E; ++r) {
-            const u64 o = __shfl_xor_sync(0xffffffffu, v[r], j / E);
-            v[r] = (o < v[r]) == small ? o : v[r];
-          }
-        } else {  // E is 2
-          const bool up = (first & k) == 0;
-          const u64 x = v[0], y = v[E - 1];
-          v[0] = (x < y) == up ? x : y;
-          v[E - 1] = (x < y) == up ? y : x;
-        }
-      }
-    }
-    u64 t = 0;
-#pragma unroll
-    for (int r = 0; r < E; ++r) {
-      t += first + r < m ? weigh(logit_of(v[r])) : 0;
-      w[r] = t;
-    }
-    u64 s = t;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 u = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += u;
-    }
-#pragma unroll
-    for (int r = 0; r < E; ++r)
-      if (first + r < m) {
-        sts64(list + 8 * (first + r), v[r]);
-        sts64(run + 8 * (first + r), s - t + w[r]);
-      }
-  }
   // Sorts a list's m tokens and sums their masses along it.  All threads have
   // seen the list's entries; they see the results.
   template <typename W>
   __device__ void order(uint32_t list, uint32_t run, int m, const W &weigh) {
-    if (m <= kAlone) {  // one warp does it alone
-      if (threadIdx.x < 32) {
-        if (m <= 32)
-          order_alone<1>(list, run, m, weigh);
-        else
-          order_alone<2>(list, run, m, weigh);
+    const int tid = threadIdx.x;
+    if (m <= kPairs) {  // few: every token against every other
+      u64 e = 0, through = 0;
+      int place = -1;
+      if (tid < m) {
+        e = lds64(list + 8 * tid);
+        sts64(run + 8 * tid, weigh(logit_of(e)));
       }
+      __syncthreads();
+      if (tid < m) {
+#pragma unroll 4
+        for (int i = 0; i < m; ++i)
+          if (lds64(list + 8 * i) <= e) through += lds64(run + 8 * i), ++place;
+      }
+      __syncthreads();
+      if (tid < m) sts64(list + 8 * place, e), sts64(run + 8 * place, through);
       __syncthreads();
       return;
     }
-    int size = 2 * kAlone;
+    int size = 2 * kPairs;
     while (size < m) size <<= 1;
     if (size <= kThreads)
       sort_list<1>(list, m, size);
@@ -557,39 +580,47 @@ struct Row {
   }
 };
 
-// The first CTA's list of m tokens, all tokens of the order between two places;
-// `base` is the mass in front of it.  Finds places by mass: bin(logit) puts the
-// tokens into at most kBinRoom bins in their order, a bin's masses have `shift`.
-template <typename W, typename B, typename S>
+// Finds places by mass among those of the m tokens at `from` that `take`
+// accepts (the first CTA's list, or a part of what lies elsewhere): all tokens of
+// the order between two places, `base` the mass in front of them.  bin(logit)
+// puts them into at most kBinRoom bins in their order, a bin's masses have
+// `shift`.
+template <typename W, typename T, typename B, typename S>
 struct Head {
   Row &row;
   const W &weigh;
+  T take;
   B bin;
   S shift;
+  uint32_t from;
   int m;
   u64 base;
-  uint32_t list = 0, run = 0;  // what is sorted now: the whole list, or the tokens of bin `at`
+  bool part;
+  uint32_t list = 0, run = 0;  // what is sorted now: all of them, or the tokens of bin `at`
   int n = 0, at = -1;
   u64 before = 0;  // the mass in front of what is sorted
 
-  __device__ __forceinline__ u64 entry(int i) const { return lds64(row.sm + Layout::list + 8 * i); }
+  __device__ __forceinline__ u64 entry(int i) const { return lds64(from + 8 * i); }
   __device__ void sort_all() {
     list = row.sm + Layout::list, run = row.sm + Layout::run;
-    n = m, at = kBinRoom, before = base;
-    row.order(list, run, m, weigh);
+    n = part ? row.select(from, m, take) : m;
+    at = kBinRoom, before = base;
+    row.order(list, run, n, weigh);
   }
   __device__ void begin() {
-    if (m <= kAlone) return sort_all();
+    if (!part && m <= kPairs) return sort_all();
     row.clear_bins();
     for (int i = threadIdx.x; i < m; i += kThreads) {
       const float x = Row::logit_of(entry(i));
-      const int b = bin(x);
-      row.add_to_bin(b, (uint32_t)(weigh(x) >> shift(b)));
+      if (take(x)) {
+        const int b = bin(x);
+        row.add_to_bin(b, (uint32_t)(weigh(x) >> shift(b)));
+      }
     }
     __syncthreads();
-    row.template run_bins<false>(shift);
+    row.run_own_bins(shift);
   }
-  __device__ u64 mass() const { return at == kBinRoom ? lds64(run + 8 * (m - 1)) : row.through_bin(kBinRoom - 1, Layout::own_bins); }
+  __device__ u64 mass() const { return at == kBinRoom ? lds64(run + 8 * (n - 1)) : row.through_bin(kBinRoom - 1, Layout::own_bins); }
   __device__ void focus(int b) {
     if (at == kBinRoom || at == b) return;
     if (threadIdx.x == 0) sts32(row.sm + Layout::listed, 0);
@@ -597,7 +628,8 @@ struct Head {
     list = row.sm + Layout::some, run = row.sm + Layout::some_run;
     for (int i = threadIdx.x; i < m; i += kThreads) {
       const u64 e = entry(i);
-      if (bin(Row::logit_of(e)) == b) {
+      const float x = Row::logit_of(e);
+      if (take(x) && bin(x) == b) {
         const uint32_t p = add32(row.sm + Layout::listed, 1);
         if (p < kSome) sts64(list + 8 * p, e);
       }
@@ -626,9 +658,10 @@ struct Head {
     return pick((at == kBinRoom ? rank : rank - in_front) - 1);
   }
 };
-template <typename W, typename B, typename S>
-__device__ __forceinline__ Head<W, B, S> head_of(Row &row, const W &weigh, B bin, S shift, int m, u64 base) {
-  return Head<W, B, S>{row, weigh, bin, shift, m, base};
+template <typename W, typename T, typename B, typename S>
+__device__ __forceinline__ Head<W, T, B, S> head_of(Row &row, const W &weigh, T take, B bin, S shift, uint32_t from,
+                                                    int m, u64 base, bool part) {
+  return Head<W, T, B, S>{row, weigh, take, bin, shift, from, m, base, part};
 }
 
 __device__ __forceinline__ u64 draw_target(float u, u64 mass) {
@@ -765,7 +798,7 @@ __device__ __noinline__ void descend(Row row, Weigher weigh, Filters f, int32_t 
   }
 }
 
-__global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p) {
+__global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   const uint32_t sm = sm100::smem_u32(smem), logits = sm + Layout::logits;
   const uint32_t seen = logits + 4 * p.slice;  // a bit for each token of the context in this slice
@@ -774,12 +807,14 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
   const int base = rank * p.slice, n = max(0, min(p.slice, p.V - base));
   Row row{sm, n, base, ctas, rank};
 
-  const float temp = p.temperature ? p.temperature[r] : p.temperature_all;
-  const float top_p = p.top_p ? p.top_p[r] : p.top_p_all;
-  const float min_p = p.min_p ? p.min_p[r] : p.min_p_all;
   const float pen = p.penalty ? p.penalty[r] : p.penalty_all;
-  const int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
-  const float u = fminf(fmaxf(p.uniforms[r], 0.0f), 0.99999994f);
+  if (tid == 0) {  // the row's settings, until the slice is there
+    sts32(sm + Layout::settings, __float_as_uint(p.temperature ? p.temperature[r] : p.temperature_all));
+    sts32(sm + Layout::settings + 4, __float_as_uint(p.top_p ? p.top_p[r] : p.top_p_all));
+    sts32(sm + Layout::settings + 8, __float_as_uint(p.min_p ? p.min_p[r] : p.min_p_all));
+    sts32(sm + Layout::settings + 12, p.top_k ? p.top_k[r] : p.top_k_all);
+    sts32(sm + Layout::settings + 16, __float_as_uint(p.uniforms[r]));
+  }
   if (tid < 16) sts64(sm + Layout::power + 8 * tid, (u64)__double_as_longlong(kPower[tid]));
 
   // the slice
@@ -802,7 +837,7 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
     return __float_as_uint(x);
   };
   const int64_t at0 = (int64_t)r * p.ld + base;
-  constexpr int kBatch = 8;  // loads a thread has in flight
+  constexpr int kBatch = 4;  // loads a thread has in flight
   auto scalar = [&](int from, auto &&load) {
     for (int i0 = from + tid; i0 < n; i0 += kBatch * kThreads) {
       float v[kBatch];
@@ -872,6 +907,8 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
     if (rank == 0 && tid == 0) write(-1, -INFINITY);
     return;
   }
+  auto setting = [&](int i) { return lds32(sm + Layout::settings + 4 * i); };
+  const float temp = __uint_as_float(setting(0));
   if (!(temp > 1e-4f)) {
     const int t = token_at(row, top, 1);
     if (t >= 0 && tid == 0) write(t, 0.f);
@@ -879,16 +916,17 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
   }
   const double c = 1.4426950408889634 / (double)fminf(temp, 1e36f);  // octaves of w per unit of a logit
   const Weigher weigh{top, (float)c, (double)top, c, sm + Layout::power};
+  const float top_p = __uint_as_float(setting(1)), min_p = __uint_as_float(setting(2));
+  const int top_k = (int)setting(3);
+  const float u = fminf(fmaxf(__uint_as_float(setting(4)), 0.0f), 0.99999994f);
   Filters f;
   f.cut_p = !(top_p >= 1.0f), f.cut_k = top_k > 0 && top_k < p.V, f.cut_m = min_p > 0.0f;
   f.top_k = top_k, f.u = u;
   f.share = f.cut_p ? (top_p > 0.f ? (double)top_p : 0.0) : 1.0;
   f.floor_m = f.cut_m ? (u64)ceil(fmin((double)min_p, 1.0) * (double)kOne) : 1;
 
-  u64 z = 0;
   unsigned m = kList + 1;
   int last = 0, in_front = 0;
-  float lowest = kLowest;
   if (top == INFINITY) {
     // step 5 alone knows what to do
   } else if (f.cut_k) {
@@ -898,41 +936,27 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
       const float t = weigh.lead(x);
       if (weigh.some(t)) red32(sm + Layout::lo + 4 * weigh.sixteenths(t), 1u);
     });
-    cluster_barrier();
-    u64 said = 0;  // the bin, and how many tokens lie through it
-    if (rank == 0) {
-      row.run_bins<true>([](int) { return -1; });
-      last = row.bin_of(min((u64)top_k, row.through_bin(kBinRoom - 1)));
-      in_front = (int)row.through_bin(last - 1);
-      said = (u64)last << 32 | row.through_bin(last);
-    }
-    said = row.from_first(said);
-    last = (int)(said >> 32);
-    if ((uint32_t)said <= kList)
-      m = row.collect(weigh.logit_below((last + 1) / 16.0), INFINITY, [&](float x) { return weigh.bin(x) <= last; });
-  } else {
-    // 2. the sum of all masses, then the tokens that can still matter
-    u64 least = f.floor_m;
-    if (f.cut_p || !f.cut_m) {
-      row.each([&](float x, int) { z += weigh(x); });
-      z = row.total(z);
-      const double behind = (f.cut_p ? 1.0 - f.share : 1.0 - (double)u) * (double)z / (double)p.V;
-      const u64 t = behind > 2.0 ? (u64)behind - 1 : 1;
-      least = t > least ? t : least;
-    }
-    lowest = weigh.logit_below(44.0 - (double)log2f((float)least));
-    m = row.collect(lowest, INFINITY, [](float) { return true; });
+    row.run_bins(0, [](int) { return -1; });
+    last = row.bin_of(min((u64)top_k, row.through_bin(kBinRoom - 1)));
+    in_front = (int)row.through_bin(last - 1);
+    const float end = (last + 1) / 16.0f;
+    if (row.through_bin(last) <= kList)
+      m = row.bring(sm + Layout::list, [&](float x) { return weigh.lead(x) < end; });
+  } else if (!f.cut_p && f.cut_m) {
+    // 2. the tokens that min-p may keep
+    const float lowest = weigh.logit_below(44.0 - (double)log2f((float)f.floor_m));
+    m = row.bring(sm + Layout::list, [&](float x) { return x >= lowest; });
   }
 
   if (m <= kList) {
     // 3. every place is on the first CTA's list
     if (rank) return;
-    auto head = head_of(row, weigh, [&](float x) { return weigh.bin(x); }, [](int b) { return Weigher::shift(b); },
-                        (int)m, 0);
+    auto head = head_of(row, weigh, [](float) { return true; }, [&](float x) { return weigh.bin(x); },
+                        [](int b) { return Weigher::shift(b); }, sm + Layout::list, (int)m, 0, false);
     head.begin();
     const u64 held = head.mass();
-    if (f.cut_k) z = (int)m > top_k ? head.by_rank(top_k, last, in_front).through : held;
-    u64 mass = f.cut_k || f.cut_p || !f.cut_m ? z : held;
+    const u64 z = f.cut_k && (int)m > top_k ? head.by_rank(top_k, last, in_front).through : held;
+    u64 mass = z;
     if (f.cut_m) {
       u64 v = 0;
       for (int i = tid; i < (int)m; i += kThreads) {
@@ -948,60 +972,71 @@ __global__ void __launch_bounds__(kThreads) sample_tokens_kernel(SampleParams p)
   }
 
   if (!f.cut_k && top < INFINITY) {
-    // 4. masses by bins; the crossing of top_p and the draw each in one bin
+    // 4. masses by bins, and in which of them the places lie
     row.clear_bins();
     u64 kept_m = 0;
-    row.each([&](float x, int) {
-      if (x >= lowest) {
-        const float t = weigh.lead(x);
-        if (weigh.some(t)) {
-          const int b = weigh.sixteenths(t);
-          const uint32_t q = weigh.bits(x, b);
-          const u64 w = (u64)q << weigh.shift(b);
-          row.add_to_bin(b, q);
-          kept_m += w >= f.floor_m ? w : 0;
-        }
+    for (int i = tid; i < (n + 3) / 4; i += kThreads) {
+      const uint4 v = lds128(logits + 16 * i);
+      const float x[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
+      float t[4];
+      int b[4];
+      uint32_t q[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        t[j] = weigh.lead(x[j]);
+        b[j] = weigh.sixteenths(fminf(t[j], 46.0f));
+        q[j] = weigh.bits(x[j], b[j]);
       }
-    });
-    u64 mass = f.cut_p || !f.cut_m ? z : ~0ull;
-    if (f.cut_m)
-      mass = min(mass, row.total(kept_m));
-    else
-      cluster_barrier();
-    // the first CTA decides and says in which bin the next place lies
-    u64 held = 0, target = 0;
-    bool crossing = false;  // the place is where top_p is crossed, else the draw's
-    int b = 0;
-    if (rank == 0) {
-      row.run_bins<true>([](int i) { return Weigher::shift(i); });
-      held = row.through_bin(kBinRoom - 1);
-      crossing = f.cut_p && f.over(z) <= held;
-      target = crossing ? f.over(z) : min(draw_target(u, mass), held);
-      b = row.bin_of(target);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (weigh.some(t[j])) {
+          row.add_to_bin(b[j], q[j]);
+          const u64 w = (u64)q[j] << weigh.shift(b[j]);
+          if (f.cut_m) kept_m += w >= f.floor_m ? w : 0;
+        }
     }
-    for (;;) {
-      const u64 said = row.from_first((u64)b << 1 | crossing);
-      b = (int)(said >> 1), crossing = said & 1;
-      const float lo = weigh.logit_below((b + 1) / 16.0), hi = weigh.logit_above(b / 16.0);
-      const unsigned in_bin = row.collect(lo, hi, [&](float x) { return x >= lowest && weigh.bin(x) == b; });
-      if (in_bin > kList) break;
-      if (!crossing && rank) return;
+    if (f.cut_m) kept_m = row.block_sum(kept_m);
+    kept_m = row.run_bins(kept_m, [](int b) { return Weigher::shift(b); });
+    const u64 z = row.through_bin(kBinRoom - 1);
+    u64 mass = f.cut_m ? min(z, kept_m) : z;
+    // the crossing of top_p, unless it lies behind the mass that min-p keeps; the mass through it lies between
+    // its bin's ends, and the draw in few bins
+    const u64 over = f.cut_p ? f.over(z) : mass;
+    const bool crossing = over < mass;
+    const int b1 = crossing ? row.bin_of(over) : -1;
+    const int b2 = row.bin_of(draw_target(u, min(mass, over)));
+    const int b3 = crossing ? row.bin_of(draw_target(u, min(mass, row.through_bin(b1)))) : b2;
+    const uint32_t stash = logits;  // nobody needs the first CTA's logits once its tokens are counted
+    // t >= 0, so its bits have its order
+    auto bits_at = [](int b) { return __float_as_uint(b / 16.0f); };
+    auto in = [](float t, uint32_t from, uint32_t span) { return __float_as_uint(t) - from < span; };
+    const uint32_t from1 = bits_at(b1), span1 = crossing ? bits_at(b1 + 1) - from1 : 0;
+    const uint32_t from2 = bits_at(b2), span2 = bits_at(b3 + 1) - from2;
+    m = row.bring(stash, [&](float x) {
+      const float t = weigh.lead(x);
+      return in(t, from1, span1) | in(t, from2, span2);
+    });
+    const bool all_there = m <= kList;  // else one bin after the other
+    if (all_there && rank) return;
+    for (bool draw = !crossing;; draw = true) {
+      const u64 target = draw ? draw_target(u, mass) : over;
+      const int b = row.bin_of(target);
+      const uint32_t from = bits_at(b), span = bits_at(b + 1) - from;
+      auto here = [&](float x) { return in(weigh.lead(x), from, span); };
+      if (!all_there && (m = row.bring(sm + Layout::list, here)) > kList) break;
       if (rank == 0) {
-        const uint32_t first = key_of(hi), span = first - key_of(lo);
+        const uint32_t first = key_of(weigh.logit_above(b / 16.0)), span = first - key_of(weigh.logit_below((b + 1) / 16.0));
         const int s = max(0, 32 - __clz(span) - 10);  // span >> s < kBinRoom
-        auto head = head_of(row, weigh, [&](float x) { return (int)((first - key_of(x)) >> s); },
-                            [&](int) { return Weigher::shift(b); }, (int)in_bin, row.through_bin(b - 1));
+        auto fine = [&](float x) { return (int)min((first - key_of(x)) >> s, kBinRoom - 1u); };
+        auto head = head_of(row, weigh, here, fine, [&](int) { return Weigher::shift(b); },
+                            all_there ? stash : sm + Layout::list, (int)m, row.through_bin(b - 1), all_there);
         head.begin();
         const Pick t = head.by_mass(target);
-        if (!crossing) {
-          if (tid == 0) write((int)t.token, weigh.log_share(t.logit, mass));
-          return;
-        }
+        if (draw && tid == 0) write((int)t.token, weigh.log_share(t.logit, mass));
         mass = min(mass, t.through);
-        target = min(draw_target(u, mass), held);
-        b = row.bin_of(target);
-        crossing = false;
       }
+      if (draw) return;
+      if (!all_there) mass = row.from_first(mass);
     }
   }
   descend(row, weigh, f, p.token + r, p.logprob ? p.logprob + r : nullptr);
@@ -1036,7 +1071,9 @@ extern "C" int af_sample_tokens(af_ctx *ctx, const void *logits, int logits_bf16
   SampleParams p{logits, logits_bf16 != 0, row_stride, vocab, slice, vec, context_tokens, context_stride, context_len,
                  temperature, top_p, min_p, penalty, top_k, temperature_all, top_p_all, min_p_all, penalty_all,
                  top_k_all, uniforms, token, logprob};
-  auto bytes = [](int s) { return (size_t)Layout::logits + (size_t)s * 4 + (size_t)((s + 31) / 32) * 4; };
+  auto bytes = [](int s) {  // the slice with its context's bits; later the first CTA's tokens of a few bins
+    return (size_t)Layout::logits + std::max((size_t)s * 4 + (size_t)((s + 31) / 32) * 4, (size_t)8 * kList);
+  };
   static std::atomic<unsigned long long> attr_devices{0};
   if (int rc = af::smem_attr(ctx, reinterpret_cast<const void *>(sample_tokens_kernel),
                              bytes((AF_SAMPLE_TOKENS_MAX_VOCAB / kMaxCtas + 7) & ~7), attr_devices, fn))

@@ -182,3 +182,36 @@ def test_agrees_with_the_one_setting_sampler(dev):
     for r in torch.nonzero(a != b).flatten().tolist():
         _, _, margin = L.sample64(lg[r].cpu().numpy(), float(u[r]), 0.8, 60, 0.95)
         assert margin < 1e-4
+
+
+def test_places_in_crowded_bins(dev):
+    """Bins of a sixteenth of an octave (0.043 of a logit at temperature 1) with
+    more tokens than one CTA takes over at once (2048): two bins that are too
+    many together, a crossing of top-p in a small bin before a draw in an
+    overfull one, and the other way round."""
+    rng = np.random.default_rng(77)
+    wide = 2.5 * rng.standard_normal((4, 327680))
+    # where top-p 0.95 is crossed a token weighs exp(2.1) / (327680 exp(3.1)) = 1.1e-6 of the row: 1e-7 on either
+    # side leave 0.82 of the crossings and of the draws next to them, 0.67 of the rows
+    _check(dev, wide, [0.97, 0.99, 0.9995, 0.5], need=0.5, top_p=[0.95, 0.97, 0.95, 1.0], min_p=[0.0, 0.0, 1e-6, 1e-5])
+    head = 0.03 * rng.random((6, 3000))
+    tail = -3.0 + rng.standard_normal((6, 20000))
+    crowd = rng.permuted(np.concatenate([head, tail], 1), axis=1)
+    _check(dev, crowd, [0.3, 0.6, 0.9, 0.97, 0.999, 0.2], need=0.6, top_p=[0.95, 0.9, 0.5, 0.97, 1.0, 0.3])
+    _check(dev, crowd, [0.3, 0.6, 0.9, 0.97, 0.999, 0.2], need=0.6, min_p=[0.0, 0.97, 0.99, 0.02, 0.01, 0.5], top_p=0.99)
+
+
+@pytest.mark.parametrize("rows,V", [(200, 5000), (160, 20001), (160, 50000)])
+def test_many_rows_take_fewer_blocks_each(dev, rows, V):
+    """The number of CTAs that share a row depends on both sizes (here one, two
+    and four); the token does not."""
+    rng = np.random.default_rng(V)
+    pick = lambda v: np.asarray(v)[rng.integers(0, len(v), rows)]  # noqa: E731
+    logits, u = 3.0 * rng.standard_normal((rows, V)), rng.random(rows)
+    kw = dict(temperature=pick([0.0, 0.7, 1.2]), top_k=pick([0, 0, 30]), top_p=pick([1.0, 0.95, 0.6]),
+              min_p=pick([0.0, 0.0, 0.02]))
+    _check(dev, logits[:48], u[:48], **{k: v[:48] for k, v in kw.items()})
+    many, few = _draw(dev, logits, u, **dict(kw)), _draw(dev, logits[:2], u[:2], **{k: v[:2] for k, v in kw.items()})
+    assert (many[0][:2] == few[0]).all() and (many[1][:2] == few[1]).all()
+    part = _draw(dev, logits[:48], u[:48], **{k: v[:48] for k, v in kw.items()})
+    assert (many[0][:48] == part[0]).all() and (many[1][:48] == part[1]).all()
