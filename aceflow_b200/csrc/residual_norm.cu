@@ -235,23 +235,26 @@ __device__ __forceinline__ float sigmoid(float g) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
   return r;
 }
-// swish(g) = g sigmoid(g) and its derivative; at -inf (where sg is 0) their limit 0.
-__device__ __forceinline__ float swish(float g, float sg) { return fmaxf(g, -3.0e38f) * sg; }
-__device__ __forceinline__ float swish_slope(float g, float sg) {
-  return fmaf(swish(g, sg), 1.f - sg, sg);
-}
-
-// sg = sigmoid(g), o = o swish(g)
+// sw = swish(g), sg = sigmoid(g), o = o sw
 template <int VEC>
-__device__ __forceinline__ void gate_by(float (&o)[VEC], const float (&g)[VEC], float (&sg)[VEC]) {
-  float w[VEC];
+__device__ __forceinline__ void gate_by(float (&o)[VEC], const float (&g)[VEC], float (&sw)[VEC], float (&sg)[VEC]) {
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
     sg[i] = sigmoid(g[i]);
-    w[i] = fmaxf(g[i], -3.0e38f);
+    sw[i] = fmaxf(g[i], -3.0e38f);  // at -inf (where sg is 0) swish has the limit 0
   }
-  mul(w, w, sg);
-  mul(o, o, w);
+  mul(sw, sw, sg);
+  mul(o, o, sw);
+}
+// o = o swish'(g) = o (sg + sw - sw sg)
+template <int VEC>
+__device__ __forceinline__ void slope_by(float (&o)[VEC], const float (&sw)[VEC], const float (&sg)[VEC]) {
+  float v[VEC];
+  const float one = 1.f;
+  mul(v, sw, -one);
+  fma(v, v, sg, sg);
+  fma(v, sw, one, v);
+  mul(o, o, v);
 }
 
 constexpr int kRed = 2 * 3 * 32;
@@ -261,10 +264,30 @@ constexpr int kRed = 2 * 3 * 32;
 template <int NV>
 __device__ __forceinline__ void row_sum(float (&v)[NV], bool one_warp, float *red, int &flip) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) v[i] = warp_sum(v[i]);
+  for (int i = 0; i < NV; ++i)
+    if (one_warp || NV != 3) v[i] = warp_sum(v[i]);
   if (one_warp) return;
   float *r = red + flip * 96;
   flip ^= 1;
+  if constexpr (NV == 3) {  // the lanes share the three sums: half the shuffles, an eighth of the reads
+    const int lane = threadIdx.x & 31;
+    float a = __shfl_xor_sync(0xffffffffu, lane & 16 ? v[0] : v[1], 16) + (lane & 16 ? v[1] : v[0]);
+    const float b = v[2] + __shfl_xor_sync(0xffffffffu, v[2], 16);
+    a = __shfl_xor_sync(0xffffffffu, lane & 8 ? a : b, 8) + (lane & 8 ? b : a);
+#pragma unroll
+    for (int o = 4; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    // lanes 0 .. 7 have the first sum, 16 .. 23 the second, the rest the third
+    const int which = lane & 8 ? 2 : lane >> 4;
+    if ((lane & 7) == 0 && lane < 24) r[which * 32 + (threadIdx.x >> 5)] = a;
+    __syncthreads();
+    const float *q = r + which * 32 + (lane & 7);
+    a = q[0];
+    if ((int)blockDim.x > 256) a += q[8];  // 16 warps at most
+#pragma unroll
+    for (int o = 4; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    v[0] = __shfl_sync(0xffffffffu, a, 0), v[1] = __shfl_sync(0xffffffffu, a, 16), v[2] = __shfl_sync(0xffffffffu, a, 8);
+    return;
+  }
   if ((threadIdx.x & 31) == 0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) r[i * 32 + (threadIdx.x >> 5)] = v[i];
@@ -358,9 +381,9 @@ __global__ void __launch_bounds__(VEC == 8 && K == 1 ? 1024 : 512, VEC == 8 ? 1 
         dot.add(z[c], z[c]);
         // all of n but r1
         if (p.g) {
-          float v[VEC], sg[VEC];
+          float v[VEC], sw[VEC], sg[VEC];
           gr[c].get(v, h16);
-          gate_by(z[c], v, sg);
+          gate_by(z[c], v, sw, sg);
         }
         if (kAhead) {
           mul(z[c], z[c], kept1[c]);
@@ -418,14 +441,14 @@ __global__ void __launch_bounds__(VEC == 8 && K == 1 ? 1024 : 512, VEC == 8 ? 1 
   }
 }
 
-template <int VEC, int K, int TX, int TH>
+template <int VEC, int K, int TX, int TH, bool one_warp>
 __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
   constexpr bool kAhead = VEC * K <= 8 && K <= 4;
   __shared__ __align__(16) float red[kRed];
   int flip = 0;
   clear_red(red);
   const int n = blockDim.x;
-  const bool one_warp = n == 32, x16 = TX == 1, h16 = TH == 1;
+  const bool x16 = TX == 1, h16 = TH == 1;
   float a1[K][VEC], a2[K][VEC];  // this thread's columns of sum Z swish hh and of dw2
 #pragma unroll
   for (int c = 0; c < K; ++c) fill(a1[c], 0.f), fill(a2[c], 0.f);
@@ -447,14 +470,15 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
       }
     }
   };
-  const int part = blockIdx.x * blockDim.y + threadIdx.y;  // also this row group's place among all
+  // also this row group's place among all; one for the whole block keeps a row's address in uniform registers
+  const int part = one_warp ? blockIdx.x * blockDim.y + threadIdx.y : blockIdx.x;
   if (kAhead && part < p.rows) fetch(part);
   for (int row = part; row < p.rows; row += p.parts) {
     if (!kAhead) fetch(row);
     const float r1 = p.w1 ? p.stats[row] : 1.f, r2 = p.w2 ? p.stats[p.rows + row] : 1.f;
     Dot tz, eq, zq;  // t zh, e q, zh q
     // hh (h without post_w), the gate and its sigmoid, zh, e = dz + r2 t; q is what z has of n
-    float hh[K][VEC], g[K][VEC], sg[K][VEC], zh[K][VEC], e[K][VEC];
+    float hh[K][VEC], sw[K][VEC], sg[K][VEC], zh[K][VEC], e[K][VEC];
 #pragma unroll
     for (int c = 0; c < K; ++c) {
       const int col = (c * n + (int)threadIdx.x) * VEC;
@@ -469,8 +493,8 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
           mul(q, hh[c], w);
         }
         if (p.g) {
-          gr[c].get(g[c], h16);
-          gate_by(q, g[c], sg[c]);
+          gr[c].get(v, h16);
+          gate_by(q, v, sw[c], sg[c]);
         }
         if (p.dz)
           dzr[c].get(e[c], x16);
@@ -517,19 +541,11 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
         else
           mul(v, e[c], w);
         if (p.g) {
-          float sw[VEC], sl[VEC];
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            sw[i] = fmaxf(g[c][i], -3.0e38f);
-            sl[i] = 1.f - sg[c][i];
-          }
-          mul(sw, sw, sg[c]);
-          fma(a1[c], o, sw, a1[c]);
-          fma(sl, sw, sl, sg[c]);  // swish'
+          fma(a1[c], o, sw[c], a1[c]);
           mul(o, v, hh[c]);
-          mul(o, o, sl);
+          slope_by(o, sw[c], sg[c]);
           put<VEC>(p.dg, at, o, h16);
-          mul(v, v, sw);
+          mul(v, v, sw[c]);
         } else {
 #pragma unroll
           for (int i = 0; i < VEC; ++i) a1[c][i] += o[i];
@@ -554,9 +570,154 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
   }
 }
 
-// Rows too wide for a thread's registers: the same in two passes over the row,
-// the second from the caches, with the column sums in shared memory, [2][d],
-// where every thread alone touches its columns.
+// The same for wide rows, in two passes that each form a row's values anew: what
+// a thread has of a row as it lies in memory,
+template <int VEC>
+struct RawRow {
+  Raw<VEC> h, g, x, dz, dy;
+  __device__ __forceinline__ void load(const SeamParams &p, int row, int col, bool x16, bool h16) {
+    h.load(p.h, row * p.ldh + col, h16);
+    if (p.g) g.load(p.g, row * p.ldg + col, h16);
+    if (p.dz) dz.load(p.dz, row * p.lddz + col, x16);
+    if (p.dy) {
+      dy.load(p.dy, row * p.lddy + col, p.y16);
+      x.load(p.x, row * p.ldx + col, x16);
+    }
+  }
+};
+// and the values that follow from it (w: post_w scale; t = dy pre_w; e = dz + r2 t).
+template <int VEC>
+struct SeamValues {
+  float hh[VEC], sw[VEC], sg[VEC], w[VEC], q[VEC], zh[VEC], e[VEC], dy[VEC], t[VEC];
+  __device__ __forceinline__ void form(const SeamParams &p, const RawRow<VEC> &r, int col, float r1, float r2, bool x16,
+                                       bool h16) {
+    both_weights<VEC>(p, col, w);
+    r.h.get(hh, h16);
+    mul(hh, hh, r1);
+    mul(q, hh, w);
+    if (p.g) {
+      float g[VEC];
+      r.g.get(g, h16);
+      gate_by(q, g, sw, sg);
+    }
+    fill(e, 0.f), fill(zh, 0.f), fill(t, 0.f), fill(dy, 0.f);
+    if (p.dz) r.dz.get(e, x16);
+    if (p.dy) {
+      float v[VEC];
+      r.x.get(v, x16);
+      r.dy.get(dy, p.y16);
+      fma(zh, v, p.alpha, q);
+      mul(zh, zh, r2);
+      weights<VEC>(p.w2, col, v);
+      mul(t, dy, v);
+      fma(e, t, r2, e);
+    }
+  }
+  // The gradients; o1 and o2: what they add to the columns' sums.
+  __device__ __forceinline__ void write(const SeamParams &p, int64_t at, float r1, float m1, float m2, bool x16, bool h16,
+                                        float (&o1)[VEC], float (&o2)[VEC]) {
+    float v[VEC];
+    fma(e, zh, -m2, e);  // Z
+    mul(v, e, p.alpha);
+    put<VEC>(p.dx, at, v, x16);
+    mul(o1, e, hh);
+    mul(o2, dy, zh);
+    mul(v, e, w);
+    if (p.g) {
+      float o[VEC];
+      mul(o1, o1, sw);
+      mul(o, v, hh);
+      slope_by(o, sw, sg);
+      put<VEC>(p.dg, at, o, h16);
+      mul(v, v, sw);
+    }
+    if (p.w1) {
+      fma(v, hh, -m1, v);
+      mul(v, v, r1);
+    }
+    put<VEC>(p.dh, at, v, h16);
+  }
+};
+
+__device__ __forceinline__ void ahead(const void *p, int64_t i, bool b16) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char *>(p) + i * (b16 ? 2 : 4)));
+}
+
+// Rows of up to K 512 VEC values: the row as it lies in memory and the columns'
+// sums stay in registers, the block's next row is on its way into L2.
+template <int VEC, int K, int TX, int TH>
+__global__ void __launch_bounds__(512, 1) seam_backward_held_kernel(SeamParams p) {
+  __shared__ __align__(16) float red[kRed];
+  int flip = 0;
+  clear_red(red);
+  const int n = blockDim.x;
+  const bool x16 = TX == 1, h16 = TH == 1;
+  float a1[K][VEC], a2[K][VEC];
+#pragma unroll
+  for (int c = 0; c < K; ++c) fill(a1[c], 0.f), fill(a2[c], 0.f);
+  for (int row = blockIdx.x; row < p.rows; row += p.parts) {
+    RawRow<VEC> raw[K];
+#pragma unroll
+    for (int c = 0; c < K; ++c) {
+      const int col = (c * n + (int)threadIdx.x) * VEC;
+      if (col < p.d) raw[c].load(p, row, col, x16, h16);
+    }
+    const int next = row + p.parts;
+    if (next < p.rows && threadIdx.x % 4 == 0) {
+#pragma unroll
+      for (int c = 0; c < K; ++c) {
+        const int col = (c * n + (int)threadIdx.x) * VEC;
+        if (col < p.d) {
+          ahead(p.h, next * p.ldh + col, h16);
+          if (p.g) ahead(p.g, next * p.ldg + col, h16);
+          if (p.dz) ahead(p.dz, next * p.lddz + col, x16);
+          if (p.dy) ahead(p.dy, next * p.lddy + col, p.y16), ahead(p.x, next * p.ldx + col, x16);
+        }
+      }
+    }
+    const float r1 = p.w1 ? p.stats[row] : 1.f, r2 = p.w2 ? p.stats[p.rows + row] : 1.f;
+    Dot tz, eq, zq;
+#pragma unroll
+    for (int c = 0; c < K; ++c) {
+      const int col = (c * n + (int)threadIdx.x) * VEC;
+      if (col < p.d) {
+        SeamValues<VEC> s;
+        s.form(p, raw[c], col, r1, r2, x16, h16);
+        tz.add(s.t, s.zh);
+        eq.add(s.e, s.q);
+        zq.add(s.zh, s.q);
+      }
+    }
+    float sum[3] = {tz.sum(), eq.sum(), zq.sum()};
+    row_sum(sum, false, red, flip);
+    const float m2 = r2 * (sum[0] * p.inv_d), m1 = (sum[1] - m2 * sum[2]) * p.inv_d;
+#pragma unroll
+    for (int c = 0; c < K; ++c) {
+      const int col = (c * n + (int)threadIdx.x) * VEC;
+      if (col < p.d) {
+        SeamValues<VEC> s;
+        float o1[VEC], o2[VEC];
+        s.form(p, raw[c], col, r1, r2, x16, h16);
+        s.write(p, (int64_t)row * p.d + col, r1, m1, m2, x16, h16, o1, o2);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) a1[c][i] += o1[i], a2[c][i] += o2[i];
+      }
+    }
+  }
+  const int64_t plane = (int64_t)p.parts * p.d;
+#pragma unroll
+  for (int c = 0; c < K; ++c) {
+    const int col = (c * n + (int)threadIdx.x) * VEC;
+    if (col < p.d) {
+      const int64_t at = (int64_t)blockIdx.x * p.d + col;
+      if (p.w1 || p.s) put<VEC>(p.part, at, a1[c], false);
+      if (p.w2) put<VEC>(p.part, plane + at, a2[c], false);
+    }
+  }
+}
+
+// Wider ones: the second pass reads the row from the caches, the column sums
+// lie in shared memory, [2][d], where every thread alone touches its columns.
 template <int VEC, int TX, int TH>
 __global__ void __launch_bounds__(512, 1) seam_backward_wide_kernel(SeamParams p) {
   extern __shared__ __align__(16) float acc[];
@@ -569,45 +730,14 @@ __global__ void __launch_bounds__(512, 1) seam_backward_wide_kernel(SeamParams p
   for (int col = threadIdx.x * VEC; col < p.d; col += n * VEC)
 #pragma unroll
     for (int i = 0; i < VEC; ++i) a1[col + i] = a2[col + i] = 0.f;
-  struct Values {
-    float hh[VEC], g[VEC], sg[VEC], w[VEC], q[VEC], zh[VEC], e[VEC], dy[VEC], t[VEC];
-  };
-  auto values = [&](int row, int col, float r1, float r2, Values &s) {
-    Raw<VEC> hr, gr, xr, dzr, dyr;
-    hr.load(p.h, row * p.ldh + col, h16);
-    if (p.g) gr.load(p.g, row * p.ldg + col, h16);
-    if (p.dz) dzr.load(p.dz, row * p.lddz + col, x16);
-    if (p.dy) {
-      dyr.load(p.dy, row * p.lddy + col, p.y16);
-      xr.load(p.x, row * p.ldx + col, x16);
-    }
-    both_weights<VEC>(p, col, s.w);
-    hr.get(s.hh, h16);
-    mul(s.hh, s.hh, r1);
-    mul(s.q, s.hh, s.w);
-    if (p.g) {
-      gr.get(s.g, h16);
-      gate_by(s.q, s.g, s.sg);
-    }
-    fill(s.e, 0.f), fill(s.zh, 0.f), fill(s.t, 0.f), fill(s.dy, 0.f);
-    if (p.dz) dzr.get(s.e, x16);
-    if (p.dy) {
-      float v[VEC];
-      xr.get(v, x16);
-      dyr.get(s.dy, p.y16);
-      fma(s.zh, v, p.alpha, s.q);
-      mul(s.zh, s.zh, r2);
-      weights<VEC>(p.w2, col, v);
-      mul(s.t, s.dy, v);
-      fma(s.e, s.t, r2, s.e);
-    }
-  };
   for (int row = blockIdx.x; row < p.rows; row += p.parts) {
     const float r1 = p.w1 ? p.stats[row] : 1.f, r2 = p.w2 ? p.stats[p.rows + row] : 1.f;
     Dot tz, eq, zq;
     for (int col = threadIdx.x * VEC; col < p.d; col += n * VEC) {
-      Values s;
-      values(row, col, r1, r2, s);
+      RawRow<VEC> raw;
+      SeamValues<VEC> s;
+      raw.load(p, row, col, x16, h16);
+      s.form(p, raw, col, r1, r2, x16, h16);
       tz.add(s.t, s.zh);
       eq.add(s.e, s.q);
       zq.add(s.zh, s.q);
@@ -616,40 +746,14 @@ __global__ void __launch_bounds__(512, 1) seam_backward_wide_kernel(SeamParams p
     row_sum(sum, false, red, flip);
     const float m2 = r2 * (sum[0] * p.inv_d), m1 = (sum[1] - m2 * sum[2]) * p.inv_d;
     for (int col = threadIdx.x * VEC; col < p.d; col += n * VEC) {
-      const int64_t at = (int64_t)row * p.d + col;
-      Values s;
-      values(row, col, r1, r2, s);
-      float o[VEC], v[VEC];
-      fma(s.e, s.zh, -m2, s.e);  // Z
-      mul(o, s.e, p.alpha);
-      put<VEC>(p.dx, at, o, x16);
-      mul(o, s.e, s.hh);
-      mul(v, s.e, s.w);
-      if (p.g) {
-        float sw[VEC], sl[VEC];
+      RawRow<VEC> raw;
+      SeamValues<VEC> s;
+      float o1[VEC], o2[VEC];
+      raw.load(p, row, col, x16, h16);
+      s.form(p, raw, col, r1, r2, x16, h16);
+      s.write(p, (int64_t)row * p.d + col, r1, m1, m2, x16, h16, o1, o2);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          sw[i] = fmaxf(s.g[i], -3.0e38f);
-          sl[i] = 1.f - s.sg[i];
-        }
-        mul(sw, sw, s.sg);
-        fma(sl, sw, sl, s.sg);  // swish'
-        mul(o, o, sw);
-        mul(sl, sl, s.hh);
-        mul(sl, sl, v);
-        put<VEC>(p.dg, at, sl, h16);
-        mul(v, v, sw);
-      }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        a1[col + i] += o[i];
-        a2[col + i] = fmaf(s.dy[i], s.zh[i], a2[col + i]);
-      }
-      if (p.w1) {
-        fma(v, s.hh, -m1, v);
-        mul(v, v, r1);
-      }
-      put<VEC>(p.dh, at, v, h16);
+      for (int i = 0; i < VEC; ++i) a1[col + i] += o1[i], a2[col + i] += o2[i];
     }
   }
   const int64_t plane = (int64_t)p.parts * p.d;
@@ -703,6 +807,7 @@ Shape shape_of(int d, int vec, bool backward) {
   if (vec == 8) {
     if (d <= 256) return {8, 1, 32, 4};
     if (d <= (backward ? 4096 : 8192)) return {8, 1, threads(8), 1};
+    if (backward && d <= 8192) return {8, 2, threads(16), 1};
     return {8, backward ? 0 : 4, 512, 1};
   }
   if (d <= 128) return {1, 4, 32, 4};
@@ -723,13 +828,17 @@ using SeamKernel = void (*)(SeamParams);
 template <int TX, int TH>
 SeamKernel typed_kernel(const Shape &s, bool backward) {
   if (backward) {
-    if (s.vec == 8) return s.k == 1 ? seam_backward_kernel<8, 1, TX, TH> : seam_backward_wide_kernel<8, TX, TH>;
+    const bool warp = s.rows_per_block > 1;
+    if (s.vec == 8)
+      return s.k == 1   ? (warp ? seam_backward_kernel<8, 1, TX, TH, true> : seam_backward_kernel<8, 1, TX, TH, false>)
+             : s.k == 2 ? seam_backward_held_kernel<8, 2, TX, TH>
+                        : seam_backward_wide_kernel<8, TX, TH>;
     if (s.vec == 2)
-      return s.k == 2   ? seam_backward_kernel<2, 2, TX, TH>
-             : s.k == 4 ? seam_backward_kernel<2, 4, TX, TH>
+      return s.k == 2   ? seam_backward_kernel<2, 2, TX, TH, false>
+             : s.k == 4 ? seam_backward_kernel<2, 4, TX, TH, false>
                         : seam_backward_wide_kernel<2, TX, TH>;
-    return s.k == 4   ? seam_backward_kernel<1, 4, TX, TH>
-           : s.k == 8 ? seam_backward_kernel<1, 8, TX, TH>
+    return s.k == 4   ? (warp ? seam_backward_kernel<1, 4, TX, TH, true> : seam_backward_kernel<1, 4, TX, TH, false>)
+           : s.k == 8 ? seam_backward_kernel<1, 8, TX, TH, false>
                       : seam_backward_wide_kernel<1, TX, TH>;
   }
   if (s.vec == 8) return s.k == 1 ? seam_forward_kernel<8, 1, TX, TH> : seam_forward_kernel<8, 4, TX, TH>;
