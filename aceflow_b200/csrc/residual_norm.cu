@@ -30,7 +30,6 @@
 #include "common.cuh"
 
 #include <algorithm>
-#include <initializer_list>
 
 namespace {
 
@@ -46,8 +45,9 @@ struct SeamParams {
   const void *dz, *dy;  // either may be NULL (zero)
   int64_t lddz, lddy;
   void *dx, *dh, *dg;
-  float *part;  // [2][parts][d]: sum Z swish(g) hh, sum dy zh
-  int parts;
+  float *part;    // planes of [parts][d], `plane` apart: sum Z swish(g) hh, sum dy zh
+  int64_t plane;
+  int parts;      // row groups: group i has the rows i, i + parts, ..
 };
 
 // VEC consecutive values of a row as they lie in memory: loads are issued
@@ -75,22 +75,6 @@ struct Raw<8> {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
     }
-  }
-};
-template <>
-struct Raw<2> {
-  uint32_t a, b;
-  __device__ __forceinline__ void load(const void *p, int64_t i, bool b16) {
-    if (b16) {
-      a = __ldcs(reinterpret_cast<const unsigned int *>(static_cast<const char *>(p) + 2 * i));
-    } else {
-      const uint2 q = __ldcs(reinterpret_cast<const uint2 *>(static_cast<const char *>(p) + 4 * i));
-      a = q.x, b = q.y;
-    }
-  }
-  __device__ __forceinline__ void get(float (&v)[2], bool b16) const {
-    v[0] = __uint_as_float(b16 ? a << 16 : a);
-    v[1] = __uint_as_float(b16 ? a & 0xffff0000u : b);
   }
 };
 template <>
@@ -122,13 +106,6 @@ __device__ __forceinline__ void put<8>(void *p, int64_t i, const float (&v)[8], 
   }
 }
 template <>
-__device__ __forceinline__ void put<2>(void *p, int64_t i, const float (&v)[2], bool b16) {
-  if (b16)
-    *reinterpret_cast<__nv_bfloat162 *>(static_cast<__nv_bfloat16 *>(p) + i) = __floats2bfloat162_rn(v[0], v[1]);
-  else
-    *reinterpret_cast<float2 *>(static_cast<float *>(p) + i) = make_float2(v[0], v[1]);
-}
-template <>
 __device__ __forceinline__ void put<1>(void *p, int64_t i, const float (&v)[1], bool b16) {
   if (b16)
     static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16(v[0]);
@@ -142,9 +119,6 @@ __device__ __forceinline__ void weights(const float *w, int col, float (&v)[VEC]
     const float4 a = __ldg(reinterpret_cast<const float4 *>(w + col)),
                  b = __ldg(reinterpret_cast<const float4 *>(w + col) + 1);
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else if constexpr (VEC == 2) {
-    const float2 a = __ldg(reinterpret_cast<const float2 *>(w + col));
-    v[0] = a.x, v[1] = a.y;
   } else {
     v[0] = __ldg(w + col);
   }
@@ -313,86 +287,154 @@ __device__ __forceinline__ void clear_red(float *red) {
   __syncthreads();
 }
 
-// post_w scale (what is not given counts as 1) of VEC columns.
-template <int VEC>
-__device__ __forceinline__ void both_weights(const SeamParams &p, int col, float (&v)[VEC]) {
-  fill(v, 1.f);
-  if (p.w1) weights<VEC>(p.w1, col, v);
-  if (p.s) {
-    float s[VEC];
-    weights<VEC>(p.s, col, s);
-    mul(v, v, s);
-  }
-}
-
-// Those and pre_w of all of a thread's columns.
-template <int VEC, int K>
-__device__ __forceinline__ void keep_weights(const SeamParams &p, int n, float (&w1)[K][VEC], float (&w2)[K][VEC]) {
-#pragma unroll
-  for (int c = 0; c < K; ++c) {
-    const int col = (c * n + (int)threadIdx.x) * VEC;
-    fill(w1[c], 0.f), fill(w2[c], 0.f);
-    if (col < p.d) {
-      both_weights<VEC>(p, col, w1[c]);
-      if (p.w2) weights<VEC>(p.w2, col, w2[c]);
+// The VEC columns of a thread's chunk c.  Rows whose width is no multiple of 8
+// start anywhere in 16 bytes (SHIFT); a group's rows, 8 or a multiple of it
+// apart, all at the same place, so its threads' chunks start `phase` values in
+// front of the row, where every access is aligned.  The chunks at a row's ends
+// are cut: their values outside [lo, hi) count as 0 and are not written.
+template <int VEC, bool SHIFT>
+struct Chunk {
+  int col, lo, hi;
+  bool in, cut;
+  __device__ __forceinline__ Chunk(const SeamParams &p, int c, int phase) {
+    col = (c * (int)blockDim.x + (int)threadIdx.x) * VEC - (SHIFT ? phase : 0);
+    in = col < p.d, cut = false, lo = 0, hi = VEC;
+    if (SHIFT) {
+      lo = max(0, -col), hi = min(VEC, p.d - col);
+      cut = in && hi - lo < VEC;
     }
   }
-}
+  // Loads of a row.  A cut chunk's values outside belong to the rows next to it,
+  // or lie behind the tensor's last value: there, single loads.
+  __device__ __forceinline__ void load(Raw<VEC> &r, const SeamParams &p, const void *from, int row, int64_t ld,
+                                       bool b16) const {
+    const int64_t at = row * ld + col;
+    if constexpr (SHIFT) {
+      if (hi < VEC && at + VEC > (p.rows - 1) * ld + p.d) {
+        uint32_t w[8] = {};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i >= lo && i < hi) {
+            if (b16)
+              w[i / 2] |= (uint32_t) static_cast<const unsigned short *>(from)[at + i] << (16 * (i & 1));
+            else
+              w[i] = static_cast<const uint32_t *>(from)[at + i];
+          }
+        r.a = make_uint4(w[0], w[1], w[2], w[3]), r.b = make_uint4(w[4], w[5], w[6], w[7]);
+        return;
+      }
+    }
+    r.load(from, at, b16);
+  }
+  __device__ __forceinline__ void get(const Raw<VEC> &r, float (&v)[VEC], bool b16) const {
+    r.get(v, b16);
+    if (SHIFT && cut) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = i >= lo && i < hi ? v[i] : 0.f;
+    }
+  }
+  __device__ __forceinline__ void store(void *to, int64_t row_at, const float (&v)[VEC], bool b16) const {
+    if (SHIFT && cut) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (i >= lo && i < hi) {
+          const float one[1] = {v[i]};
+          put<1>(to, row_at + col + i, one, b16);
+        }
+    } else {
+      put<VEC>(to, row_at + col, v, b16);
+    }
+  }
+  __device__ __forceinline__ void weight(const float *w, float (&v)[VEC]) const {
+    if constexpr (SHIFT) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = i >= lo && i < hi ? __ldg(w + col + i) : 0.f;
+    } else {
+      weights<VEC>(w, col, v);
+    }
+  }
+  // post_w scale (what is not given counts as 1).
+  __device__ __forceinline__ void both_weights(const SeamParams &p, float (&v)[VEC]) const {
+    fill(v, 1.f);
+    if (p.w1) weight(p.w1, v);
+    if (p.s) {
+      float s[VEC];
+      weight(p.s, s);
+      mul(v, v, s);
+    }
+  }
+  // Those and pre_w.
+  __device__ __forceinline__ void all_weights(const SeamParams &p, float (&v)[VEC], float (&w2)[VEC]) const {
+    fill(v, 0.f), fill(w2, 0.f);
+    if (in) {
+      both_weights(p, v);
+      if (p.w2) weight(p.w2, w2);
+    }
+  }
+};
+// Where the rows of a group start in 16 bytes, its first one given.
+__device__ __forceinline__ int phase_of(int row, int d) { return (int)((int64_t)row * d & 7); }
 
 // Threads of a row: a warp (blockDim.y rows per block) or the whole block
-// (blockDim.y == 1).  Thread k of a row holds values (c * n + k) * VEC ..,
+// (blockDim.y == 1).  Thread k of a row holds chunks c * n + k of VEC values,
 // c < K, n the row's threads.  Where those are few, the weights stay in
 // registers while a block walks over rows, and a row's loads are under way
 // while the row before it is summed.
-template <int VEC, int K, int TX, int TH>
+template <int VEC, int K, int TX, int TH, bool SHIFT>
 __global__ void __launch_bounds__(VEC == 8 && K == 1 ? 1024 : 512, VEC == 8 ? 1 : 2) seam_forward_kernel(SeamParams p) {
   constexpr bool kAhead = VEC * K <= 8 && K <= 4;
+  static_assert(kAhead || !SHIFT, "a group's rows share their phase");
   __shared__ __align__(16) float red[kRed];
   int flip = 0;
   clear_red(red);
   const int n = blockDim.x;
   const bool one_warp = n == 32, x16 = TX == 1, h16 = TH == 1;
-  const int step = gridDim.x * blockDim.y;
+  const int step = p.parts;  // row groups
+  int row = blockIdx.x * blockDim.y + threadIdx.y;
+  const int phase = SHIFT ? phase_of(row, p.d) : 0;
   Raw<VEC> hr[K], gr[K], xr[K];
   auto fetch = [&](int row) {
 #pragma unroll
     for (int c = 0; c < K; ++c) {
-      const int col = (c * n + (int)threadIdx.x) * VEC;
-      if (col < p.d) {
-        hr[c].load(p.h, row * p.ldh + col, h16);
-        if (p.g) gr[c].load(p.g, row * p.ldg + col, h16);
-        xr[c].load(p.x, row * p.ldx + col, x16);
+      const Chunk<VEC, SHIFT> k(p, c, phase);
+      if (k.in) {
+        k.load(hr[c], p, p.h, row, p.ldh, h16);
+        if (p.g) k.load(gr[c], p, p.g, row, p.ldg, h16);
+        k.load(xr[c], p, p.x, row, p.ldx, x16);
       }
     }
   };
   float kept1[K][VEC], kept2[K][VEC];  // with kAhead: post_w scale, pre_w
-  if (kAhead) keep_weights<VEC, K>(p, n, kept1, kept2);
-  int row = blockIdx.x * blockDim.y + threadIdx.y;
+  if (kAhead) {
+#pragma unroll
+    for (int c = 0; c < K; ++c) Chunk<VEC, SHIFT>(p, c, phase).all_weights(p, kept1[c], kept2[c]);
+  }
   if (kAhead && row < p.rows) fetch(row);
   for (; row < p.rows; row += step) {  // a block's threads leave together where they share a row
     if (!kAhead) fetch(row);
+    const int64_t at = (int64_t)row * p.d;
     float z[K][VEC], x[K][VEC];
     Dot dot;
 #pragma unroll
     for (int c = 0; c < K; ++c) {
-      const int col = (c * n + (int)threadIdx.x) * VEC;
-      if (col < p.d) {
-        hr[c].get(z[c], h16);
+      const Chunk<VEC, SHIFT> k(p, c, phase);
+      if (k.in) {
+        k.get(hr[c], z[c], h16);
         dot.add(z[c], z[c]);
         // all of n but r1
         if (p.g) {
           float v[VEC], sw[VEC], sg[VEC];
-          gr[c].get(v, h16);
+          k.get(gr[c], v, h16);
           gate_by(z[c], v, sw, sg);
         }
         if (kAhead) {
           mul(z[c], z[c], kept1[c]);
         } else {
           float v[VEC];
-          both_weights<VEC>(p, col, v);
+          k.both_weights(p, v);
           mul(z[c], z[c], v);
         }
-        xr[c].get(x[c], x16);
+        k.get(xr[c], x[c], x16);
         mul(x[c], x[c], p.alpha);
       }
     }
@@ -406,11 +448,11 @@ __global__ void __launch_bounds__(VEC == 8 && K == 1 ? 1024 : 512, VEC == 8 ? 1 
     Dot dz;
 #pragma unroll
     for (int c = 0; c < K; ++c) {
-      const int col = (c * n + (int)threadIdx.x) * VEC;
-      if (col < p.d) {
+      const Chunk<VEC, SHIFT> k(p, c, phase);
+      if (k.in) {
         fma(z[c], z[c], r1, x[c]);
         dz.add(z[c], z[c]);
-        put<VEC>(p.z, (int64_t)row * p.d + col, z[c], x16);
+        k.store(p.z, at, z[c], x16);
       }
     }
     float r2 = 1.f;
@@ -420,17 +462,17 @@ __global__ void __launch_bounds__(VEC == 8 && K == 1 ? 1024 : 512, VEC == 8 ? 1 
       r2 = rsqrtf(fmaf(sz[0], p.inv_d, p.eps));
 #pragma unroll
       for (int c = 0; c < K; ++c) {
-        const int col = (c * n + (int)threadIdx.x) * VEC;
-        if (col < p.d) {
+        const Chunk<VEC, SHIFT> k(p, c, phase);
+        if (k.in) {
           mul(z[c], z[c], r2);
           if (kAhead) {
             mul(z[c], z[c], kept2[c]);
           } else {
             float v[VEC];
-            weights<VEC>(p.w2, col, v);
+            k.weight(p.w2, v);
             mul(z[c], z[c], v);
           }
-          put<VEC>(p.y, (int64_t)row * p.d + col, z[c], p.y16);
+          k.store(p.y, at, z[c], p.y16);
         }
       }
     }
@@ -441,76 +483,102 @@ __global__ void __launch_bounds__(VEC == 8 && K == 1 ? 1024 : 512, VEC == 8 ? 1 
   }
 }
 
-template <int VEC, int K, int TX, int TH, bool one_warp>
+// What a thread has of a row in the backward, as it lies in memory.
+template <int VEC>
+struct RawRow {
+  Raw<VEC> h, g, x, dz, dy;
+  template <bool SHIFT>
+  __device__ __forceinline__ void load(const SeamParams &p, const Chunk<VEC, SHIFT> &k, int row, bool x16, bool h16) {
+    k.load(h, p, p.h, row, p.ldh, h16);
+    if (p.g) k.load(g, p, p.g, row, p.ldg, h16);
+    if (p.dz) k.load(dz, p, p.dz, row, p.lddz, x16);
+    if (p.dy) {
+      k.load(dy, p, p.dy, row, p.lddy, p.y16);
+      k.load(x, p, p.x, row, p.ldx, x16);
+    }
+  }
+};
+
+// A row group's column sums, each its part of the planes.
+template <int VEC, int K, bool SHIFT>
+__device__ __forceinline__ void write_part(const SeamParams &p, int part, int phase, const float (&a1)[K][VEC],
+                                           const float (&a2)[K][VEC]) {
+#pragma unroll
+  for (int c = 0; c < K; ++c) {
+    const Chunk<VEC, SHIFT> k(p, c, phase);
+    if (k.in) {
+      if (p.w1 || p.s) k.store(p.part, (int64_t)part * p.d, a1[c], false);
+      if (p.w2) k.store(p.part + p.plane, (int64_t)part * p.d, a2[c], false);
+    }
+  }
+}
+
+template <int VEC, int K, int TX, int TH, bool one_warp, bool SHIFT>
 __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
   constexpr bool kAhead = VEC * K <= 8 && K <= 4;
+  static_assert(kAhead || !SHIFT, "a group's rows share their phase");
   __shared__ __align__(16) float red[kRed];
   int flip = 0;
   clear_red(red);
-  const int n = blockDim.x;
   const bool x16 = TX == 1, h16 = TH == 1;
+  // the row group's place among all; one for the whole block keeps a row's address in uniform registers
+  const int part = one_warp ? blockIdx.x * blockDim.y + threadIdx.y : blockIdx.x;
+  const int phase = SHIFT ? phase_of(part, p.d) : 0;
   float a1[K][VEC], a2[K][VEC];  // this thread's columns of sum Z swish hh and of dw2
 #pragma unroll
   for (int c = 0; c < K; ++c) fill(a1[c], 0.f), fill(a2[c], 0.f);
   float kept1[K][VEC], kept2[K][VEC];  // with kAhead: post_w scale, pre_w
-  if (kAhead) keep_weights<VEC, K>(p, n, kept1, kept2);
-  Raw<VEC> hr[K], gr[K], xr[K], dzr[K], dyr[K];
+  if (kAhead) {
+#pragma unroll
+    for (int c = 0; c < K; ++c) Chunk<VEC, SHIFT>(p, c, phase).all_weights(p, kept1[c], kept2[c]);
+  }
+  RawRow<VEC> raw[K];
   auto fetch = [&](int row) {
 #pragma unroll
     for (int c = 0; c < K; ++c) {
-      const int col = (c * n + (int)threadIdx.x) * VEC;
-      if (col < p.d) {
-        hr[c].load(p.h, row * p.ldh + col, h16);
-        if (p.g) gr[c].load(p.g, row * p.ldg + col, h16);
-        if (p.dz) dzr[c].load(p.dz, row * p.lddz + col, x16);
-        if (p.dy) {
-          dyr[c].load(p.dy, row * p.lddy + col, p.y16);
-          xr[c].load(p.x, row * p.ldx + col, x16);
-        }
-      }
+      const Chunk<VEC, SHIFT> k(p, c, phase);
+      if (k.in) raw[c].load(p, k, row, x16, h16);
     }
   };
-  // also this row group's place among all; one for the whole block keeps a row's address in uniform registers
-  const int part = one_warp ? blockIdx.x * blockDim.y + threadIdx.y : blockIdx.x;
   if (kAhead && part < p.rows) fetch(part);
   for (int row = part; row < p.rows; row += p.parts) {
     if (!kAhead) fetch(row);
     const float r1 = p.w1 ? p.stats[row] : 1.f, r2 = p.w2 ? p.stats[p.rows + row] : 1.f;
     Dot tz, eq, zq;  // t zh, e q, zh q
-    // hh (h without post_w), the gate and its sigmoid, zh, e = dz + r2 t; q is what z has of n
+    // hh (h without post_w), swish and sigmoid of the gate, zh, e = dz + r2 t; q is what z has of n
     float hh[K][VEC], sw[K][VEC], sg[K][VEC], zh[K][VEC], e[K][VEC];
 #pragma unroll
     for (int c = 0; c < K; ++c) {
-      const int col = (c * n + (int)threadIdx.x) * VEC;
-      if (col < p.d) {
+      const Chunk<VEC, SHIFT> k(p, c, phase);
+      if (k.in) {
         float q[VEC], v[VEC], w[VEC];
-        hr[c].get(hh[c], h16);
+        k.get(raw[c].h, hh[c], h16);
         mul(hh[c], hh[c], r1);
         if (kAhead) {
           mul(q, hh[c], kept1[c]);
         } else {
-          both_weights<VEC>(p, col, w);
+          k.both_weights(p, w);
           mul(q, hh[c], w);
         }
         if (p.g) {
-          gr[c].get(v, h16);
+          k.get(raw[c].g, v, h16);
           gate_by(q, v, sw[c], sg[c]);
         }
         if (p.dz)
-          dzr[c].get(e[c], x16);
+          k.get(raw[c].dz, e[c], x16);
         else
           fill(e[c], 0.f);
         if (p.dy) {
           float dy[VEC];
-          xr[c].get(v, x16);
-          dyr[c].get(dy, p.y16);
+          k.get(raw[c].x, v, x16);
+          k.get(raw[c].dy, dy, p.y16);
           fma(zh[c], v, p.alpha, q);
           mul(zh[c], zh[c], r2);
           fma(a2[c], dy, zh[c], a2[c]);
           if (kAhead) {
             mul(dy, dy, kept2[c]);  // t
           } else {
-            weights<VEC>(p.w2, col, w);
+            k.weight(p.w2, w);
             mul(dy, dy, w);
           }
           tz.add(dy, zh[c]);
@@ -525,16 +593,16 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
     if (p.w1 || p.dy) row_sum(sum, one_warp, red, flip);
     const float m2 = p.dy ? r2 * (sum[0] * p.inv_d) : 0.f;  // r2 mean(t zh)
     const float m1 = (sum[1] - m2 * sum[2]) * p.inv_d;       // mean(N w1 hh)
+    const int64_t at = (int64_t)row * p.d;
 #pragma unroll
     for (int c = 0; c < K; ++c) {
-      const int col = (c * n + (int)threadIdx.x) * VEC;
-      if (col < p.d) {
-        const int64_t at = (int64_t)row * p.d + col;
+      const Chunk<VEC, SHIFT> k(p, c, phase);
+      if (k.in) {
         float o[VEC], v[VEC], w[VEC];
         if (p.dy) fma(e[c], zh[c], -m2, e[c]);  // Z
         mul(o, e[c], p.alpha);
-        put<VEC>(p.dx, at, o, x16);
-        if (!kAhead) both_weights<VEC>(p, col, w);
+        k.store(p.dx, at, o, x16);
+        if (!kAhead) k.both_weights(p, w);
         mul(o, e[c], hh[c]);
         if (kAhead)
           mul(v, e[c], kept1[c]);
@@ -544,7 +612,7 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
           fma(a1[c], o, sw[c], a1[c]);
           mul(o, v, hh[c]);
           slope_by(o, sw[c], sg[c]);
-          put<VEC>(p.dg, at, o, h16);
+          k.store(p.dg, at, o, h16);
           mul(v, v, sw[c]);
         } else {
 #pragma unroll
@@ -554,124 +622,149 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
           fma(v, hh[c], -m1, v);
           mul(v, v, r1);
         }
-        put<VEC>(p.dh, at, v, h16);
+        k.store(p.dh, at, v, h16);
       }
     }
   }
-  const int64_t plane = (int64_t)p.parts * p.d;
-#pragma unroll
-  for (int c = 0; c < K; ++c) {
-    const int col = (c * n + (int)threadIdx.x) * VEC;
-    if (col < p.d) {
-      const int64_t at = (int64_t)part * p.d + col;
-      if (p.w1 || p.s) put<VEC>(p.part, at, a1[c], false);
-      if (p.w2) put<VEC>(p.part, plane + at, a2[c], false);
-    }
-  }
+  write_part<VEC, K, SHIFT>(p, part, phase, a1, a2);
 }
 
-// The same for wide rows, in two passes that each form a row's values anew: what
-// a thread has of a row as it lies in memory,
-template <int VEC>
-struct RawRow {
-  Raw<VEC> h, g, x, dz, dy;
-  __device__ __forceinline__ void load(const SeamParams &p, int row, int col, bool x16, bool h16) {
-    h.load(p.h, row * p.ldh + col, h16);
-    if (p.g) g.load(p.g, row * p.ldg + col, h16);
-    if (p.dz) dz.load(p.dz, row * p.lddz + col, x16);
-    if (p.dy) {
-      dy.load(p.dy, row * p.lddy + col, p.y16);
-      x.load(p.x, row * p.ldx + col, x16);
-    }
-  }
-};
-// and the values that follow from it (w: post_w scale; t = dy pre_w; e = dz + r2 t).
+// For wide rows, in two passes that each form a row's values anew from those in
+// memory (w: post_w scale; t = dy pre_w; e = dz + r2 t).
+// `of` gives the weights where they are needed.
 template <int VEC>
 struct SeamValues {
   float hh[VEC], sw[VEC], sg[VEC], w[VEC], q[VEC], zh[VEC], e[VEC], dy[VEC], t[VEC];
-  __device__ __forceinline__ void form(const SeamParams &p, const RawRow<VEC> &r, int col, float r1, float r2, bool x16,
-                                       bool h16) {
-    both_weights<VEC>(p, col, w);
-    r.h.get(hh, h16);
+  template <bool SHIFT, typename W>
+  __device__ __forceinline__ void form(const SeamParams &p, const Chunk<VEC, SHIFT> &k, const RawRow<VEC> &r,
+                                       const W &of, float r1, float r2, bool x16, bool h16) {
+    of.both(w);
+    k.get(r.h, hh, h16);
     mul(hh, hh, r1);
     mul(q, hh, w);
     if (p.g) {
       float g[VEC];
-      r.g.get(g, h16);
+      k.get(r.g, g, h16);
       gate_by(q, g, sw, sg);
     }
     fill(e, 0.f), fill(zh, 0.f), fill(t, 0.f), fill(dy, 0.f);
-    if (p.dz) r.dz.get(e, x16);
+    if (p.dz) k.get(r.dz, e, x16);
     if (p.dy) {
       float v[VEC];
-      r.x.get(v, x16);
-      r.dy.get(dy, p.y16);
+      k.get(r.x, v, x16);
+      k.get(r.dy, dy, p.y16);
       fma(zh, v, p.alpha, q);
       mul(zh, zh, r2);
-      weights<VEC>(p.w2, col, v);
+      of.pre(v);
       mul(t, dy, v);
       fma(e, t, r2, e);
     }
   }
-  // The gradients; o1 and o2: what they add to the columns' sums.
-  __device__ __forceinline__ void write(const SeamParams &p, int64_t at, float r1, float m1, float m2, bool x16, bool h16,
-                                        float (&o1)[VEC], float (&o2)[VEC]) {
-    float v[VEC];
+  // The gradients; what they add to the columns' sums goes to a1 and a2.
+  template <bool SHIFT>
+  __device__ __forceinline__ void write(const SeamParams &p, const Chunk<VEC, SHIFT> &k, int64_t at, float r1, float m1, float m2, bool x16, bool h16,
+                                        float (&a1)[VEC], float (&a2)[VEC]) {
+    float v[VEC], o[VEC];
+    fma(a2, dy, zh, a2);
     fma(e, zh, -m2, e);  // Z
     mul(v, e, p.alpha);
-    put<VEC>(p.dx, at, v, x16);
-    mul(o1, e, hh);
-    mul(o2, dy, zh);
+    k.store(p.dx, at, v, x16);
+    mul(o, e, hh);
     mul(v, e, w);
     if (p.g) {
-      float o[VEC];
-      mul(o1, o1, sw);
+      fma(a1, o, sw, a1);
       mul(o, v, hh);
       slope_by(o, sw, sg);
-      put<VEC>(p.dg, at, o, h16);
+      k.store(p.dg, at, o, h16);
       mul(v, v, sw);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) a1[i] += o[i];
     }
     if (p.w1) {
       fma(v, hh, -m1, v);
       mul(v, v, r1);
     }
-    put<VEC>(p.dh, at, v, h16);
+    k.store(p.dh, at, v, h16);
   }
+};
+
+template <int VEC, bool SHIFT>
+struct GivenWeights {
+  const SeamParams &p;
+  const Chunk<VEC, SHIFT> &k;
+  __device__ __forceinline__ void both(float (&v)[VEC]) const { k.both_weights(p, v); }
+  __device__ __forceinline__ void pre(float (&v)[VEC]) const { k.weight(p.w2, v); }
+};
+// A thread's own vectors in shared memory, each as two halves that lie `half`
+// apart: those of its chunks, then as many of another kind.
+struct Own {
+  float4 *at;
+  int half, kind;
+  __device__ __forceinline__ void read(int i, float (&v)[8]) const {
+    const float4 a = at[i], b = at[i + half];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  }
+  __device__ __forceinline__ void write(int i, const float (&v)[8]) const {
+    at[i] = make_float4(v[0], v[1], v[2], v[3]), at[i + half] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+  __device__ __forceinline__ void both(float (&v)[8]) const { read(0, v); }
+  __device__ __forceinline__ void pre(float (&v)[8]) const { read(kind, v); }
 };
 
 __device__ __forceinline__ void ahead(const void *p, int64_t i, bool b16) {
   asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char *>(p) + i * (b16 ? 2 : 4)));
 }
 
-// Rows of up to K 512 VEC values: the row as it lies in memory and the columns'
-// sums stay in registers, the block's next row is on its way into L2.
-template <int VEC, int K, int TX, int TH>
+// Rows of up to K 512 chunks: the row as it lies in memory stays in registers,
+// the columns' sums in shared memory where each thread alone touches its own, the
+// block's next row is on its way into L2.  So do weights of rows that start
+// anywhere: no vector holds them elsewhere.
+template <int K, int TX, int TH, bool SHIFT>
 __global__ void __launch_bounds__(512, 1) seam_backward_held_kernel(SeamParams p) {
+  constexpr int VEC = 8;
+  extern __shared__ __align__(16) float4 own[];  // [sums, weights][2][K][2][threads]
   __shared__ __align__(16) float red[kRed];
   int flip = 0;
   clear_red(red);
   const int n = blockDim.x;
   const bool x16 = TX == 1, h16 = TH == 1;
-  float a1[K][VEC], a2[K][VEC];
+  const int phase = SHIFT ? phase_of(blockIdx.x, p.d) : 0;
+  auto sums = [&](int c) { return Own{own + c * 2 * n + threadIdx.x, n, 2 * K * n}; };
+  auto own_weights = [&](int c) { return Own{own + (2 * K + c) * 2 * n + threadIdx.x, n, 2 * K * n}; };
 #pragma unroll
-  for (int c = 0; c < K; ++c) fill(a1[c], 0.f), fill(a2[c], 0.f);
+  for (int c = 0; c < K; ++c) {
+    float w[VEC], w2[VEC];
+    fill(w, 0.f);
+    sums(c).write(0, w), sums(c).write(sums(c).kind, w);
+    if (SHIFT) {
+      Chunk<VEC, SHIFT>(p, c, phase).all_weights(p, w, w2);
+      own_weights(c).write(0, w), own_weights(c).write(own_weights(c).kind, w2);
+    }
+  }
+  auto form = [&](SeamValues<VEC> &s, const Chunk<VEC, SHIFT> &k, int c, const RawRow<VEC> &r, float r1, float r2) {
+    if constexpr (SHIFT)
+      s.form(p, k, r, own_weights(c), r1, r2, x16, h16);
+    else
+      s.form(p, k, r, GivenWeights<VEC, SHIFT>{p, k}, r1, r2, x16, h16);
+  };
   for (int row = blockIdx.x; row < p.rows; row += p.parts) {
     RawRow<VEC> raw[K];
 #pragma unroll
     for (int c = 0; c < K; ++c) {
-      const int col = (c * n + (int)threadIdx.x) * VEC;
-      if (col < p.d) raw[c].load(p, row, col, x16, h16);
+      const Chunk<VEC, SHIFT> k(p, c, phase);
+      if (k.in) raw[c].load(p, k, row, x16, h16);
     }
     const int next = row + p.parts;
     if (next < p.rows && threadIdx.x % 4 == 0) {
 #pragma unroll
       for (int c = 0; c < K; ++c) {
-        const int col = (c * n + (int)threadIdx.x) * VEC;
-        if (col < p.d) {
-          ahead(p.h, next * p.ldh + col, h16);
-          if (p.g) ahead(p.g, next * p.ldg + col, h16);
-          if (p.dz) ahead(p.dz, next * p.lddz + col, x16);
-          if (p.dy) ahead(p.dy, next * p.lddy + col, p.y16), ahead(p.x, next * p.ldx + col, x16);
+        const Chunk<VEC, SHIFT> k(p, c, phase);
+        if (k.in) {  // next is not the first row: what is in front of it is there
+          ahead(p.h, next * p.ldh + k.col, h16);
+          if (p.g) ahead(p.g, next * p.ldg + k.col, h16);
+          if (p.dz) ahead(p.dz, next * p.lddz + k.col, x16);
+          if (p.dy) ahead(p.dy, next * p.lddy + k.col, p.y16), ahead(p.x, next * p.ldx + k.col, x16);
         }
       }
     }
@@ -679,10 +772,10 @@ __global__ void __launch_bounds__(512, 1) seam_backward_held_kernel(SeamParams p
     Dot tz, eq, zq;
 #pragma unroll
     for (int c = 0; c < K; ++c) {
-      const int col = (c * n + (int)threadIdx.x) * VEC;
-      if (col < p.d) {
+      const Chunk<VEC, SHIFT> k(p, c, phase);
+      if (k.in) {
         SeamValues<VEC> s;
-        s.form(p, raw[c], col, r1, r2, x16, h16);
+        form(s, k, c, raw[c], r1, r2);
         tz.add(s.t, s.zh);
         eq.add(s.e, s.q);
         zq.add(s.zh, s.q);
@@ -693,27 +786,21 @@ __global__ void __launch_bounds__(512, 1) seam_backward_held_kernel(SeamParams p
     const float m2 = r2 * (sum[0] * p.inv_d), m1 = (sum[1] - m2 * sum[2]) * p.inv_d;
 #pragma unroll
     for (int c = 0; c < K; ++c) {
-      const int col = (c * n + (int)threadIdx.x) * VEC;
-      if (col < p.d) {
+      const Chunk<VEC, SHIFT> k(p, c, phase);
+      if (k.in) {
         SeamValues<VEC> s;
-        float o1[VEC], o2[VEC];
-        s.form(p, raw[c], col, r1, r2, x16, h16);
-        s.write(p, (int64_t)row * p.d + col, r1, m1, m2, x16, h16, o1, o2);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) a1[c][i] += o1[i], a2[c][i] += o2[i];
+        form(s, k, c, raw[c], r1, r2);
+        float a1[VEC], a2[VEC];
+        sums(c).read(0, a1), sums(c).read(sums(c).kind, a2);
+        s.write(p, k, (int64_t)row * p.d, r1, m1, m2, x16, h16, a1, a2);
+        sums(c).write(0, a1), sums(c).write(sums(c).kind, a2);
       }
     }
   }
-  const int64_t plane = (int64_t)p.parts * p.d;
+  float a1[K][VEC], a2[K][VEC];
 #pragma unroll
-  for (int c = 0; c < K; ++c) {
-    const int col = (c * n + (int)threadIdx.x) * VEC;
-    if (col < p.d) {
-      const int64_t at = (int64_t)blockIdx.x * p.d + col;
-      if (p.w1 || p.s) put<VEC>(p.part, at, a1[c], false);
-      if (p.w2) put<VEC>(p.part, plane + at, a2[c], false);
-    }
-  }
+  for (int c = 0; c < K; ++c) sums(c).read(0, a1[c]), sums(c).read(sums(c).kind, a2[c]);
+  write_part<VEC, K, SHIFT>(p, blockIdx.x, phase, a1, a2);
 }
 
 // Wider ones: the second pass reads the row from the caches, the column sums
@@ -724,20 +811,29 @@ __global__ void __launch_bounds__(512, 1) seam_backward_wide_kernel(SeamParams p
   __shared__ __align__(16) float red[kRed];
   int flip = 0;
   clear_red(red);
-  const int n = blockDim.x;
   const bool x16 = TX == 1, h16 = TH == 1;
+  const int chunks = (p.d + VEC * (int)blockDim.x - 1) / (VEC * (int)blockDim.x);
   float *a1 = acc, *a2 = acc + p.d;
-  for (int col = threadIdx.x * VEC; col < p.d; col += n * VEC)
+  for (int c = 0; c < chunks; ++c) {
+    const Chunk<VEC, false> k(p, c, 0);
+    if (k.in) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) a1[col + i] = a2[col + i] = 0.f;
+      for (int i = 0; i < VEC; ++i) a1[k.col + i] = a2[k.col + i] = 0.f;
+    }
+  }
+  auto values = [&](const Chunk<VEC, false> &k, int row, float r1, float r2, SeamValues<VEC> &s) {
+    RawRow<VEC> raw;
+    raw.load(p, k, row, x16, h16);
+    s.form(p, k, raw, GivenWeights<VEC, false>{p, k}, r1, r2, x16, h16);
+  };
   for (int row = blockIdx.x; row < p.rows; row += p.parts) {
     const float r1 = p.w1 ? p.stats[row] : 1.f, r2 = p.w2 ? p.stats[p.rows + row] : 1.f;
     Dot tz, eq, zq;
-    for (int col = threadIdx.x * VEC; col < p.d; col += n * VEC) {
-      RawRow<VEC> raw;
+    for (int c = 0; c < chunks; ++c) {
+      const Chunk<VEC, false> k(p, c, 0);
+      if (!k.in) continue;
       SeamValues<VEC> s;
-      raw.load(p, row, col, x16, h16);
-      s.form(p, raw, col, r1, r2, x16, h16);
+      values(k, row, r1, r2, s);
       tz.add(s.t, s.zh);
       eq.add(s.e, s.q);
       zq.add(s.zh, s.q);
@@ -745,24 +841,27 @@ __global__ void __launch_bounds__(512, 1) seam_backward_wide_kernel(SeamParams p
     float sum[3] = {tz.sum(), eq.sum(), zq.sum()};
     row_sum(sum, false, red, flip);
     const float m2 = r2 * (sum[0] * p.inv_d), m1 = (sum[1] - m2 * sum[2]) * p.inv_d;
-    for (int col = threadIdx.x * VEC; col < p.d; col += n * VEC) {
-      RawRow<VEC> raw;
+    for (int c = 0; c < chunks; ++c) {
+      const Chunk<VEC, false> k(p, c, 0);
+      if (!k.in) continue;
       SeamValues<VEC> s;
-      float o1[VEC], o2[VEC];
-      raw.load(p, row, col, x16, h16);
-      s.form(p, raw, col, r1, r2, x16, h16);
-      s.write(p, (int64_t)row * p.d + col, r1, m1, m2, x16, h16, o1, o2);
+      float b1[VEC], b2[VEC];
+      values(k, row, r1, r2, s);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) a1[col + i] += o1[i], a2[col + i] += o2[i];
+      for (int i = 0; i < VEC; ++i) b1[i] = a1[k.col + i], b2[i] = a2[k.col + i];
+      s.write(p, k, (int64_t)row * p.d, r1, m1, m2, x16, h16, b1, b2);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) a1[k.col + i] = b1[i], a2[k.col + i] = b2[i];
     }
   }
-  const int64_t plane = (int64_t)p.parts * p.d;
-  for (int col = threadIdx.x * VEC; col < p.d; col += n * VEC) {
-    const int64_t at = (int64_t)blockIdx.x * p.d + col;
+  for (int c = 0; c < chunks; ++c) {
+    const Chunk<VEC, false> k(p, c, 0);
+    if (!k.in) continue;
+    const int64_t at = (int64_t)blockIdx.x * p.d + k.col;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      if (p.w1 || p.s) p.part[at + i] = a1[col + i];
-      if (p.w2) p.part[plane + at + i] = a2[col + i];
+      if (p.w1 || p.s) p.part[at + i] = a1[k.col + i];
+      if (p.w2) p.part[p.plane + at + i] = a2[k.col + i];
     }
   }
 }
@@ -770,12 +869,13 @@ __global__ void __launch_bounds__(512, 1) seam_backward_wide_kernel(SeamParams p
 // Column sums of the [parts][d] planes (blockIdx.y: which): 16 warps share a
 // block of 32 columns, each adds every sixteenth part in order.  The first
 // plane's sum times scale is dw1, times post_w it is ds.
-__global__ void __launch_bounds__(512) seam_columns_kernel(const float *part, int parts, int d, const float *w1,
-                                                           const float *s, float *dw1, float *ds, float *dw2) {
+__global__ void __launch_bounds__(512) seam_columns_kernel(const float *part, int64_t plane, int parts, int d,
+                                                           const float *w1, const float *s, float *dw1, float *ds,
+                                                           float *dw2) {
   __shared__ float red[16][32];
   if (blockIdx.y ? !dw2 : !(dw1 || ds)) return;
   const int col = blockIdx.x * 32 + threadIdx.x;
-  const float *src = part + (int64_t)blockIdx.y * parts * d + col;
+  const float *src = part + blockIdx.y * plane + col;
   float t = 0.f;
   if (col < d) {
 #pragma unroll 4
@@ -798,28 +898,30 @@ constexpr int kMaxWidth = 16384;
 
 // Threads of a row and values per thread for rows of d values.  A block's
 // registers allow 512 threads (1024 in the vectorised forward); while they
-// suffice, few values a thread, so that much is under way.
+// suffice, few values a thread, so that much is under way.  Vectors where the
+// rows' addresses allow them (vec 8): in rows of any width, `shift` then says
+// that they start anywhere in 16 bytes and a thread's vectors may start 7 values
+// in front of the row.  16384 x 1531 bf16: forward 181 -> ..., backward 241 ->
+// ... us against single values.
 struct Shape {
   int vec, k, threads, rows_per_block;
+  bool shift;
 };
 Shape shape_of(int d, int vec, bool backward) {
-  auto threads = [&](int per) { return (d + per * 32 - 1) / (per * 32) * 32; };  // whole warps that hold d values
+  const bool shift = vec == 8 && d % 8 != 0;
+  const int span = shift ? d + 7 : d;
+  auto threads = [&](int per) { return (span + per * 32 - 1) / (per * 32) * 32; };  // whole warps that hold a row
   if (vec == 8) {
-    if (d <= 256) return {8, 1, 32, 4};
-    if (d <= (backward ? 4096 : 8192)) return {8, 1, threads(8), 1};
-    if (backward && d <= 8192) return {8, 2, threads(16), 1};
-    return {8, backward ? 0 : 4, 512, 1};
+    if (span <= 256) return {8, 1, 32, 4, shift};
+    if (span <= (backward ? 4096 : 8192)) return {8, 1, threads(8), 1, shift};
+    if (backward && span <= 8192) return {8, 2, threads(16), 1, shift};
+    if (!shift) return {8, backward ? 0 : 4, 512, 1, false};
   }
-  if (d <= 128) return {1, 4, 32, 4};
-  if (vec == 2) {
-    if (d <= 2048) return {2, 2, threads(4), 1};
-    if (d <= 4096) return {2, 4, threads(8), 1};
-    return backward ? Shape{2, 0, 512, 1} : Shape{2, 16, 512, 1};
-  }
-  if (d <= 2048) return {1, 4, threads(4), 1};
-  if (d <= 4096) return {1, 8, threads(8), 1};
-  if (backward) return {1, 0, 512, 1};
-  return d <= 8192 ? Shape{1, 16, 512, 1} : Shape{1, 32, 512, 1};
+  if (d <= 128) return {1, 4, 32, 4, false};
+  if (d <= 2048) return {1, 4, threads(4), 1, false};
+  if (d <= 4096) return {1, 8, threads(8), 1, false};
+  if (backward) return {1, 0, 512, 1, false};
+  return d <= 8192 ? Shape{1, 16, 512, 1, false} : Shape{1, 32, 512, 1, false};
 }
 bool walks(const Shape &s) { return s.vec * s.k <= 8 && s.k > 0 && s.k <= 4; }  // the kernels' kAhead
 
@@ -827,56 +929,58 @@ bool walks(const Shape &s) { return s.vec * s.k <= 8 && s.k > 0 && s.k <= 4; }  
 using SeamKernel = void (*)(SeamParams);
 template <int TX, int TH>
 SeamKernel typed_kernel(const Shape &s, bool backward) {
+  const bool warp = s.rows_per_block > 1;
   if (backward) {
-    const bool warp = s.rows_per_block > 1;
-    if (s.vec == 8)
-      return s.k == 1   ? (warp ? seam_backward_kernel<8, 1, TX, TH, true> : seam_backward_kernel<8, 1, TX, TH, false>)
-             : s.k == 2 ? seam_backward_held_kernel<8, 2, TX, TH>
-                        : seam_backward_wide_kernel<8, TX, TH>;
-    if (s.vec == 2)
-      return s.k == 2   ? seam_backward_kernel<2, 2, TX, TH, false>
-             : s.k == 4 ? seam_backward_kernel<2, 4, TX, TH, false>
-                        : seam_backward_wide_kernel<2, TX, TH>;
-    return s.k == 4   ? (warp ? seam_backward_kernel<1, 4, TX, TH, true> : seam_backward_kernel<1, 4, TX, TH, false>)
-           : s.k == 8 ? seam_backward_kernel<1, 8, TX, TH, false>
+    if (s.vec == 8) {
+      if (s.k == 1 && s.shift)
+        return warp ? seam_backward_kernel<8, 1, TX, TH, true, true> : seam_backward_kernel<8, 1, TX, TH, false, true>;
+      if (s.k == 1)
+        return warp ? seam_backward_kernel<8, 1, TX, TH, true, false> : seam_backward_kernel<8, 1, TX, TH, false, false>;
+      if (s.k == 2) return s.shift ? seam_backward_held_kernel<2, TX, TH, true> : seam_backward_held_kernel<2, TX, TH, false>;
+      return seam_backward_wide_kernel<8, TX, TH>;
+    }
+    return s.k == 4   ? (warp ? seam_backward_kernel<1, 4, TX, TH, true, false>
+                              : seam_backward_kernel<1, 4, TX, TH, false, false>)
+           : s.k == 8 ? seam_backward_kernel<1, 8, TX, TH, false, false>
                       : seam_backward_wide_kernel<1, TX, TH>;
   }
-  if (s.vec == 8) return s.k == 1 ? seam_forward_kernel<8, 1, TX, TH> : seam_forward_kernel<8, 4, TX, TH>;
-  if (s.vec == 2)
-    return s.k == 2   ? seam_forward_kernel<2, 2, TX, TH>
-           : s.k == 4 ? seam_forward_kernel<2, 4, TX, TH>
-                      : seam_forward_kernel<2, 16, TX, TH>;
-  return s.k == 4    ? seam_forward_kernel<1, 4, TX, TH>
-         : s.k == 8  ? seam_forward_kernel<1, 8, TX, TH>
-         : s.k == 16 ? seam_forward_kernel<1, 16, TX, TH>
-                     : seam_forward_kernel<1, 32, TX, TH>;
+  if (s.vec == 8)
+    return s.k == 1 ? (s.shift ? seam_forward_kernel<8, 1, TX, TH, true> : seam_forward_kernel<8, 1, TX, TH, false>)
+                    : seam_forward_kernel<8, 4, TX, TH, false>;
+  return s.k == 4    ? seam_forward_kernel<1, 4, TX, TH, false>
+         : s.k == 8  ? seam_forward_kernel<1, 8, TX, TH, false>
+         : s.k == 16 ? seam_forward_kernel<1, 16, TX, TH, false>
+                     : seam_forward_kernel<1, 32, TX, TH, false>;
 }
 SeamKernel kernel_of(const Shape &s, bool x16, bool h16, bool backward) {
   if (x16) return h16 ? typed_kernel<1, 1>(s, backward) : typed_kernel<1, 0>(s, backward);
   return h16 ? typed_kernel<0, 1>(s, backward) : typed_kernel<0, 0>(s, backward);
 }
 
-// Values an access may take where rows lie at p, ld elements apart: 8 need 16
-// bytes (of fp32 rows, which are then aligned too, every half), 2 the pair's size.
-int access_of(const void *p, int64_t ld, int is16) {
+// Values an access may take where rows of d values lie at p, ld elements apart:
+// 8 if the first row starts on 16 bytes and every row does (fp32 rows: half of
+// the accesses then start between), or all rows start where contiguous ones
+// would.
+int access_of(const void *p, int64_t ld, int d, int is16) {
   if (!p) return 8;
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
-  if (a % 16 == 0 && ld % (is16 ? 8 : 4) == 0) return 8;
-  return a % (is16 ? 4 : 8) == 0 && ld % 2 == 0 ? 2 : 1;
+  if (reinterpret_cast<uintptr_t>(p) % 16) return 1;
+  return d % 8 == 0 ? (ld % (is16 ? 8 : 4) == 0 ? 8 : 1) : (ld >= d && (ld - d) % 8 == 0 ? 8 : 1);
 }
-int least_access(int d, std::initializer_list<int> all) {
-  const int v = std::min(all);
-  return d % v == 0 ? v : d % 2 == 0 && v >= 2 ? 2 : 1;
-}
+// Weights: the shifted kernels read them one by one.
+int access_of(const float *w, int d) { return d % 8 ? 8 : access_of(w, 8, 8, 0); }
 
-// Row groups that share the rows of a backward: about 512 threads an SM, as
-// many as its registers hold; few enough that their partial rows stay small
-// beside the data.
-int parts_of(int num_sms, int rows, const Shape &s) {
-  const int per_sm = 512 / (s.threads * s.rows_per_block), blocks = num_sms * (per_sm < 1 ? 1 : per_sm);
-  const int need = (rows + s.rows_per_block - 1) / s.rows_per_block;
-  return (need < blocks ? need : blocks) * s.rows_per_block;
+// Row groups that share the rows: `threads` an SM, as many as its registers
+// hold; few enough that the backward's partial rows stay small beside the data.
+// Where a group has several rows they start alike: the groups are a multiple of 8.
+int parts_of(int num_sms, int64_t rows, const Shape &s, int threads) {
+  const int per_sm = threads / (s.threads * s.rows_per_block);
+  const int64_t blocks = (int64_t)num_sms * (per_sm < 1 ? 1 : per_sm), need = (rows + s.rows_per_block - 1) / s.rows_per_block;
+  if (need <= blocks) return (int)need * s.rows_per_block;
+  return (int)(s.shift ? blocks / 8 * 8 : blocks) * s.rows_per_block;
 }
+// Of a plane of partial rows, so that the second starts on 16 bytes too.
+int64_t plane_of(int parts, int d) { return ((int64_t)parts * d + 7) / 8 * 8; }
+constexpr int64_t kMaxRows = 1 << 30;  // rows and row groups are counted in 31 bits
 
 }  // namespace
 
@@ -889,7 +993,7 @@ int af_residual_norm(af_ctx *ctx, const void *x, int64_t ldx, int x_bf16, const 
   const char *fn = "af_residual_norm";
   af::DeviceScope scope;
   AF_ENTER(ctx, fn);
-  AF_REQUIRE(rows >= 0 && rows < (1ll << 31) && d > 0, "af_residual_norm", "bad sizes");
+  AF_REQUIRE(rows >= 0 && rows <= kMaxRows && d > 0, "af_residual_norm", "bad sizes");
   AF_REQUIRE(d <= kMaxWidth, "af_residual_norm", "rows of %d values: at most %d are supported", d, kMaxWidth);
   if (rows == 0) return AF_OK;
   AF_REQUIRE(x && h && z && (!pre_w || y), "af_residual_norm", "null argument");
@@ -898,15 +1002,13 @@ int af_residual_norm(af_ctx *ctx, const void *x, int64_t ldx, int x_bf16, const 
   p.x16 = x_bf16 != 0, p.h16 = h_bf16 != 0, p.y16 = y_bf16 != 0;
   p.w1 = post_w, p.s = scale, p.w2 = pre_w, p.alpha = alpha, p.eps = eps, p.inv_d = 1.0f / (float)d;
   p.rows = (int)rows, p.d = d, p.z = z, p.y = y, p.stats = stats;
-  const int vec = least_access(
-      d, {access_of(x, ldx, x_bf16), access_of(h, ldh, h_bf16), access_of(gate, ldg, h_bf16), access_of(post_w, 8, 0),
-          access_of(scale, 8, 0), access_of(pre_w, 8, 0), access_of(z, d, x_bf16), access_of(y, d, y_bf16)});
+  const int vec = std::min({access_of(x, ldx, d, x_bf16), access_of(h, ldh, d, h_bf16), access_of(gate, ldg, d, h_bf16),
+                            access_of(post_w, d), access_of(scale, d), access_of(pre_w, d), access_of(z, d, d, x_bf16),
+                            access_of(y, d, d, y_bf16)});
   const Shape s = shape_of(d, vec, false);
   int64_t blocks = (rows + s.rows_per_block - 1) / s.rows_per_block;
-  if (walks(s)) {  // blocks that walk: 1024 threads an SM, what its registers hold
-    const int per_sm = 1024 / (s.threads * s.rows_per_block);
-    blocks = std::min<int64_t>(blocks, (int64_t)ctx->num_sms * (per_sm < 1 ? 1 : per_sm));
-  }
+  if (walks(s)) blocks = parts_of(ctx->num_sms, rows, s, 1024) / s.rows_per_block;
+  p.parts = (int)blocks * s.rows_per_block;
   kernel_of(s, p.x16, p.h16, false)<<<(unsigned)blocks, dim3(s.threads, s.rows_per_block), 0,
                                       af::stream_of(stream)>>>(p);
   return af::launched(ctx, fn);
@@ -916,12 +1018,11 @@ int af_residual_norm_scratch(af_ctx *ctx, int64_t rows, int d, int64_t *floats) 
   const char *fn = "af_residual_norm_scratch";
   af::DeviceScope scope;
   AF_ENTER(ctx, fn);
-  AF_REQUIRE(floats && rows >= 0 && rows < (1ll << 31) && d > 0 && d <= kMaxWidth, "af_residual_norm_scratch",
+  AF_REQUIRE(floats && rows >= 0 && rows <= kMaxRows && d > 0 && d <= kMaxWidth, "af_residual_norm_scratch",
              "bad sizes");
   int most = 0;  // whatever accesses the call's tensors will allow
-  for (int vec : {1, 2, 8})
-    if (d % vec == 0) most = std::max(most, parts_of(ctx->num_sms, (int)rows, shape_of(d, vec, true)));
-  *floats = 2ll * most * d;
+  for (int vec : {1, 8}) most = std::max(most, parts_of(ctx->num_sms, rows, shape_of(d, vec, true), 512));
+  *floats = 2 * plane_of(most, d);
   return AF_OK;
 }
 
@@ -934,7 +1035,7 @@ int af_residual_norm_backward(af_ctx *ctx, const void *dz, int64_t lddz, const v
   const char *fn = "af_residual_norm_backward";
   af::DeviceScope scope;
   AF_ENTER(ctx, fn);
-  AF_REQUIRE(rows >= 0 && rows < (1ll << 31) && d > 0, "af_residual_norm_backward", "bad sizes");
+  AF_REQUIRE(rows >= 0 && rows <= kMaxRows && d > 0, "af_residual_norm_backward", "bad sizes");
   AF_REQUIRE(d <= kMaxWidth, "af_residual_norm_backward", "rows of %d values: at most %d are supported", d, kMaxWidth);
   AF_REQUIRE(!dy || pre_w, "af_residual_norm_backward", "dy without the norm that made y");
   AF_REQUIRE((!post_w || dpost_w) && (!scale || dscale) && (!pre_w || dpre_w), "af_residual_norm_backward",
@@ -954,29 +1055,30 @@ int af_residual_norm_backward(af_ctx *ctx, const void *dz, int64_t lddz, const v
   p.w1 = post_w, p.s = scale, p.w2 = pre_w, p.alpha = alpha, p.inv_d = 1.0f / (float)d;
   p.rows = (int)rows, p.d = d, p.stats = const_cast<float *>(stats);
   p.dz = dz, p.dy = dy, p.lddz = lddz, p.lddy = lddy, p.dx = dx, p.dh = dh, p.dg = dgate, p.part = scratch;
-  const int vec = least_access(
-      d, {access_of(x, ldx, x_bf16), access_of(h, ldh, h_bf16), access_of(gate, ldg, h_bf16), access_of(post_w, 8, 0),
-          access_of(scale, 8, 0), access_of(pre_w, 8, 0), access_of(dz, lddz, x_bf16), access_of(dy, lddy, y_bf16),
-          access_of(dx, d, x_bf16), access_of(dh, d, h_bf16), access_of(dgate, d, h_bf16), access_of(scratch, 8, 0)});
+  const int vec = std::min({access_of(x, ldx, d, x_bf16), access_of(h, ldh, d, h_bf16), access_of(gate, ldg, d, h_bf16),
+                            access_of(post_w, d), access_of(scale, d), access_of(pre_w, d), access_of(dz, lddz, d, x_bf16),
+                            access_of(dy, lddy, d, y_bf16), access_of(dx, d, d, x_bf16), access_of(dh, d, d, h_bf16),
+                            access_of(dgate, d, d, h_bf16), access_of(scratch, d, d, 0)});
   const Shape s = shape_of(d, vec, true);
-  p.parts = parts_of(ctx->num_sms, (int)rows, s);
+  p.parts = parts_of(ctx->num_sms, rows, s, 512), p.plane = plane_of(p.parts, d);
   const bool sums = post_w || scale || pre_w;
-  AF_REQUIRE(!sums || (scratch && scratch_floats >= 2ll * p.parts * d), "af_residual_norm_backward",
-             "scratch of %lld floats, %lld are needed", (long long)scratch_floats, 2ll * p.parts * d);
+  AF_REQUIRE(!sums || (scratch && scratch_floats >= 2 * p.plane), "af_residual_norm_backward",
+             "scratch of %lld floats, %lld are needed", (long long)scratch_floats, 2ll * p.plane);
   const SeamKernel kernel = kernel_of(s, p.x16, p.h16, true);
   size_t smem = 0;
-  if (s.k == 0) {
-    smem = (size_t)2 * d * sizeof(float);
-    static std::atomic<unsigned long long> attr_devices[3][4];
+  if (s.k == 0 || (s.vec == 8 && s.k == 2)) {  // column sums, with weights
+    smem = s.k == 0 ? (size_t)2 * d * sizeof(float) : (size_t)(s.shift ? 4 : 2) * 16 * s.threads * sizeof(float);
+    static std::atomic<unsigned long long> attr_devices[4][4];
+    const int which = s.k == 0 ? s.vec == 8 : 2 + s.shift;
     if (int rc = af::smem_attr(ctx, reinterpret_cast<const void *>(kernel), (size_t)2 * kMaxWidth * sizeof(float),
-                               attr_devices[s.vec == 8 ? 2 : s.vec - 1][p.x16 * 2 + p.h16], fn))
+                               attr_devices[which][p.x16 * 2 + p.h16], fn))
       return rc;
   }
   kernel<<<(unsigned)(p.parts / s.rows_per_block), dim3(s.threads, s.rows_per_block), smem, st>>>(p);
   if (int rc = af::launched(ctx, fn)) return rc;
   if (!sums) return AF_OK;
   seam_columns_kernel<<<dim3((unsigned)((d + 31) / 32), 2), dim3(32, 16), 0, st>>>(
-      scratch, p.parts, d, post_w, scale, post_w ? dpost_w : nullptr, scale ? dscale : nullptr,
+      scratch, p.plane, p.parts, d, post_w, scale, post_w ? dpost_w : nullptr, scale ? dscale : nullptr,
       pre_w ? dpre_w : nullptr);
   return af::launched(ctx, fn);
 }

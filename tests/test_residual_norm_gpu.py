@@ -220,3 +220,32 @@ def test_two_graphs_and_another_stream(dev):
     for w, o in zip(want, outs):
         for a, b in zip(w, o):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows,d", [(9, 1), (40, 3), (33, 7), (2500, 9), (17, 130), (2400, 241), (1300, 249), (11, 250),
+                                    (1021, 1531), (700, 2030), (310, 4089), (5, 4090), (160, 5003), (3, 8185), (3, 8186)])
+@pytest.mark.parametrize("xt,ht", [(F32, F32), (BF16, BF16), (F32, BF16)])
+def test_rows_that_start_anywhere(dev, rows, d, xt, ht):
+    """Widths that are no multiple of 8: rows start anywhere in 16 bytes, a
+    thread's vectors reach into the rows next to its own, groups of rows walk."""
+    t, dz, dy = _case(dev, rows, d, xt, ht, ht, True, True, True, True)
+    _check(t, dz, dy, ht, 1.2)
+
+
+@pytest.mark.parametrize("d,gap", [(1531, 8), (1531, 3), (75, 16), (5003, 8), (512, 8), (512, 3)])
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_what_lies_between_rows_does_not_matter(dev, d, gap, dt):
+    """NaN between the rows of every input, and rows before and behind."""
+    rows = 400
+    t, dz, dy = _case(dev, rows, d, dt, dt, dt, True, True, True, True)
+
+    def inside(v):
+        big = torch.full((rows + 2, d + gap), float("nan"), device=dev, dtype=dt)
+        skip = 8 * ((d + gap) // 8 + 1) if (d + gap) % 8 else d + gap  # the first row starts on 16 bytes
+        view = big.view(-1)[skip:].as_strided((rows, d), (d + gap, 1))
+        view.copy_(v)
+        return view
+
+    for k in ("x", "h", "gate"):
+        t[k] = inside(t[k])
+    _check(t, inside(dz), inside(dy), dt, 0.9)
