@@ -21,12 +21,18 @@
 // z is formed again in fp32 from x, h and g (reading x costs what reading z
 // would), so the rounding of the stored z does not enter the gradients.
 //
-// Bound: HBM, every row of every tensor moved once.  A row is held in
-// registers by one group of threads; sums, statistics and the row itself are
-// fp32, and each output is rounded once.  The column sums of the weights'
-// gradients stay in registers while a block walks its rows, go out as one
-// partial row per block and are added in a fixed order by a second kernel: no
+// Bound: HBM, every row of every tensor moved once; the backward and odd rows
+// by the issue of instructions and their latency, at 16 warps an SM.  A row is
+// held in registers by one group of threads; sums, statistics and the row itself
+// are fp32, and each output is rounded once.  The column sums of the weights'
+// gradients stay with the threads while a block walks its rows, go out as one
+// partial row per group and are added in a fixed order by a second kernel: no
 // atomics, the same bits every run.
+// Measured with gate and all weights (floor: the tensors' bytes at 6547 GB/s):
+//   32768 x 2048 bf16   forward 111 us (0.93 of it), backward 228 (0.72)
+//   16384 x 2048 fp32            123 (0.83),                  188 (0.87)
+//    4096 x 8192 bf16             65 (0.79),                  139 (0.59)
+//   16384 x 1531 bf16             72 (0.53),                  133 (0.46)
 #include "common.cuh"
 
 #include <algorithm>
@@ -269,16 +275,13 @@ __device__ __forceinline__ void row_sum(float (&v)[NV], bool one_warp, float *re
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const float4 *q = reinterpret_cast<const float4 *>(r + i * 32);
-    float4 a = q[0], b = q[1];
-#pragma unroll
-    for (int k = 2; k < 8; k += 2)
-      if ((int)blockDim.x > 128 * k) {  // more than 4 k warps
-        const float4 c = q[k], d = q[k + 1];
-        a.x += c.x, a.y += c.y, a.z += c.z, a.w += c.w;
-        b.x += d.x, b.y += d.y, b.z += d.z, b.w += d.w;
-      }
-    v[i] = ((a.x + b.x) + (a.y + b.y)) + ((a.z + b.z) + (a.w + b.w));
+    if (blockDim.x > 256) {
+      v[i] = warp_sum(r[i * 32 + (threadIdx.x & 31)]);
+    } else {  // 8 warps at most
+      const float4 *q = reinterpret_cast<const float4 *>(r + i * 32);
+      const float4 a = q[0], b = q[1];
+      v[i] = ((a.x + b.x) + (a.y + b.y)) + ((a.z + b.z) + (a.w + b.w));
+    }
   }
 }
 __device__ __forceinline__ void clear_red(float *red) {
@@ -901,13 +904,16 @@ constexpr int kMaxWidth = 16384;
 // suffice, few values a thread, so that much is under way.  Vectors where the
 // rows' addresses allow them (vec 8): in rows of any width, `shift` then says
 // that they start anywhere in 16 bytes and a thread's vectors may start 7 values
-// in front of the row.  16384 x 1531 bf16: forward 181 -> ..., backward 241 ->
-// ... us against single values.
+// in front of the row.  16384 x 1531 bf16: forward 72 us, backward 133, against
+// 181 and 241 with single values.  Backward rows wider than 4096 (k 2; 4, where x
+// and h are bf16, `narrow`) keep their raw values: 4096 x 8192 bf16 139 us,
+// against 323 with a second reading of the row (k 0), which remains for what no
+// thread can hold.
 struct Shape {
   int vec, k, threads, rows_per_block;
   bool shift;
 };
-Shape shape_of(int d, int vec, bool backward) {
+Shape shape_of(int d, int vec, bool backward, bool narrow) {
   const bool shift = vec == 8 && d % 8 != 0;
   const int span = shift ? d + 7 : d;
   auto threads = [&](int per) { return (span + per * 32 - 1) / (per * 32) * 32; };  // whole warps that hold a row
@@ -915,6 +921,7 @@ Shape shape_of(int d, int vec, bool backward) {
     if (span <= 256) return {8, 1, 32, 4, shift};
     if (span <= (backward ? 4096 : 8192)) return {8, 1, threads(8), 1, shift};
     if (backward && span <= 8192) return {8, 2, threads(16), 1, shift};
+    if (backward && narrow && !shift) return {8, 4, 512, 1, false};
     if (!shift) return {8, backward ? 0 : 4, 512, 1, false};
   }
   if (d <= 128) return {1, 4, 32, 4, false};
@@ -937,7 +944,10 @@ SeamKernel typed_kernel(const Shape &s, bool backward) {
       if (s.k == 1)
         return warp ? seam_backward_kernel<8, 1, TX, TH, true, false> : seam_backward_kernel<8, 1, TX, TH, false, false>;
       if (s.k == 2) return s.shift ? seam_backward_held_kernel<2, TX, TH, true> : seam_backward_held_kernel<2, TX, TH, false>;
-      return seam_backward_wide_kernel<8, TX, TH>;
+      if constexpr (TX && TH)
+        return seam_backward_held_kernel<4, TX, TH, false>;
+      else
+        return seam_backward_wide_kernel<8, TX, TH>;
     }
     return s.k == 4   ? (warp ? seam_backward_kernel<1, 4, TX, TH, true, false>
                               : seam_backward_kernel<1, 4, TX, TH, false, false>)
@@ -1005,7 +1015,7 @@ int af_residual_norm(af_ctx *ctx, const void *x, int64_t ldx, int x_bf16, const 
   const int vec = std::min({access_of(x, ldx, d, x_bf16), access_of(h, ldh, d, h_bf16), access_of(gate, ldg, d, h_bf16),
                             access_of(post_w, d), access_of(scale, d), access_of(pre_w, d), access_of(z, d, d, x_bf16),
                             access_of(y, d, d, y_bf16)});
-  const Shape s = shape_of(d, vec, false);
+  const Shape s = shape_of(d, vec, false, p.x16 && p.h16);
   int64_t blocks = (rows + s.rows_per_block - 1) / s.rows_per_block;
   if (walks(s)) blocks = parts_of(ctx->num_sms, rows, s, 1024) / s.rows_per_block;
   p.parts = (int)blocks * s.rows_per_block;
@@ -1021,7 +1031,7 @@ int af_residual_norm_scratch(af_ctx *ctx, int64_t rows, int d, int64_t *floats) 
   AF_REQUIRE(floats && rows >= 0 && rows <= kMaxRows && d > 0 && d <= kMaxWidth, "af_residual_norm_scratch",
              "bad sizes");
   int most = 0;  // whatever accesses the call's tensors will allow
-  for (int vec : {1, 8}) most = std::max(most, parts_of(ctx->num_sms, rows, shape_of(d, vec, true), 512));
+  for (int vec : {1, 8}) most = std::max(most, parts_of(ctx->num_sms, rows, shape_of(d, vec, true, false), 512));
   *floats = 2 * plane_of(most, d);
   return AF_OK;
 }
@@ -1059,17 +1069,17 @@ int af_residual_norm_backward(af_ctx *ctx, const void *dz, int64_t lddz, const v
                             access_of(post_w, d), access_of(scale, d), access_of(pre_w, d), access_of(dz, lddz, d, x_bf16),
                             access_of(dy, lddy, d, y_bf16), access_of(dx, d, d, x_bf16), access_of(dh, d, d, h_bf16),
                             access_of(dgate, d, d, h_bf16), access_of(scratch, d, d, 0)});
-  const Shape s = shape_of(d, vec, true);
+  const Shape s = shape_of(d, vec, true, p.x16 && p.h16);
   p.parts = parts_of(ctx->num_sms, rows, s, 512), p.plane = plane_of(p.parts, d);
   const bool sums = post_w || scale || pre_w;
   AF_REQUIRE(!sums || (scratch && scratch_floats >= 2 * p.plane), "af_residual_norm_backward",
              "scratch of %lld floats, %lld are needed", (long long)scratch_floats, 2ll * p.plane);
   const SeamKernel kernel = kernel_of(s, p.x16, p.h16, true);
   size_t smem = 0;
-  if (s.k == 0 || (s.vec == 8 && s.k == 2)) {  // column sums, with weights
-    smem = s.k == 0 ? (size_t)2 * d * sizeof(float) : (size_t)(s.shift ? 4 : 2) * 16 * s.threads * sizeof(float);
-    static std::atomic<unsigned long long> attr_devices[4][4];
-    const int which = s.k == 0 ? s.vec == 8 : 2 + s.shift;
+  if (s.k == 0 || (s.vec == 8 && s.k > 1)) {  // column sums, with weights
+    smem = s.k == 0 ? (size_t)2 * d * sizeof(float) : (size_t)(s.shift ? 4 : 2) * 8 * s.k * s.threads * sizeof(float);
+    static std::atomic<unsigned long long> attr_devices[5][4];
+    const int which = s.k == 0 ? s.vec == 8 : s.k + s.shift;
     if (int rc = af::smem_attr(ctx, reinterpret_cast<const void *>(kernel), (size_t)2 * kMaxWidth * sizeof(float),
                                attr_devices[which][p.x16 * 2 + p.h16], fn))
       return rc;
