@@ -168,7 +168,8 @@ int af_add_f32(af_ctx *ctx, const float *a, const float *b, float *out, int64_t 
  *   z [rows][d] in x's type; y [rows][d] fp32 or bf16 (y_bf16).  fp32 inside;
  *               y comes from z before z is rounded.  z and y overlap nothing.
  *   stats [2][rows] fp32 or NULL: 1/rms of h and of z, for the backward.
- * d <= 16384. */
+ * d <= 16384, rows <= 2^30.  Rows that start on 16 bytes, or where contiguous
+ * ones behind such a first row would, are moved 16 bytes at a time. */
 int af_residual_norm(af_ctx *ctx, const void *x, int64_t ldx, int x_bf16, const void *h, int64_t ldh, int h_bf16,
                      const void *gate, int64_t ldg, const float *post_w, const float *scale, const float *pre_w,
                      float alpha, float eps, int64_t rows, int d, void *z, void *y, int y_bf16, float *stats,
@@ -490,9 +491,9 @@ int af_sample_rows(af_ctx *ctx, const float *logits, int rows, int vocab, const 
  *           -inf; among +inf only these are drawn.  Not modified.
  *   temperature, top_k, top_p, min_p, penalty: [rows] each, or NULL, and then
  *           *_all stands for every row.  temperature <= 1e-4 (or NaN): the
- *           first maximum.  top_k <= 0 and top_p >= 1: no cut; top_p <= 0 or
+ *           first maximum; above 1e36: as 1e36.  top_k <= 0 and top_p >= 1: no cut; top_p <= 0 or
  *           NaN: the likeliest token alone; min_p <= 0 or NaN: no cut; min_p >= 1: only
- *           the maximum and its equals.  penalty 1: none.
+ *           the maximum and its equals.  penalty > 0; 1: none.
  *   context_tokens, context_stride, context_len: as for af_sample_rows.
  *   uniforms [rows] in [0, 1).
  *   token   [rows]: the drawn id, -1 where every logit is -inf or NaN.
