@@ -750,7 +750,10 @@ class _Rotary(torch.autograd.Function):
 def rotary_autograd(x: torch.Tensor, inv_freq: torch.Tensor, positions=0, *, layout: str = "interleaved",
                     scale: float = 1.0, inverse: bool = False) -> torch.Tensor:
     """`rotary` as a differentiable torch op (gradients flow to x; inv_freq
-    and positions are constants)."""
+    and positions are constants).  Forward and backward can be captured into a
+    CUDA graph; as for every torch op, not while an eager graph of the same
+    leaves is alive (torch then accumulates on the eager stream and the capture
+    raises)."""
     return _Rotary.apply(x, inv_freq, positions, layout, float(scale), bool(inverse))
 
 
@@ -904,7 +907,7 @@ def residual_norm_autograd(x: torch.Tensor, h: torch.Tensor, *, gate: torch.Tens
                            post_w: torch.Tensor | None = None, scale: torch.Tensor | None = None,
                            pre_w: torch.Tensor | None = None, alpha: float = 1.0, eps: float = 1e-6, out_dtype=None):
     """residual_norm as a differentiable torch op: (z, y), gradients to x, h,
-    gate and the weights."""
+    gate and the weights.  Captured as rotary_autograd is."""
     return _ResidualNorm.apply(x, h, gate, post_w, scale, pre_w, float(alpha), float(eps), out_dtype)
 
 

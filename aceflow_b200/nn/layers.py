@@ -122,20 +122,21 @@ class Rotary(Module):
         self.layout = layout
         self.inv_freq, self.scale = ops.rotary_frequencies(rotary_dim, base, scaling=scaling, factor=factor,
                                                            original_length=original_length)
-        self._on = {}  # inv_freq on each device it was used on
+        self._on = {}  # (inv_freq, its version, its copy) for each device it was used on
 
     def turn(self, x, positions=0, inplace: bool = False):
         """The CUDA form on torch tensors (af_rotary)."""
         import torch
 
-        f = self._on.get(x.device)
-        if f is None:
-            f = self._on[x.device] = self.inv_freq.to(x.device)
+        src = self.inv_freq
+        kept = self._on.get(x.device)
+        if kept is None or kept[0] is not src or kept[1] != src._version:
+            kept = self._on[x.device] = (src, src._version, src.to(x.device))
         if not isinstance(positions, (int, np.integer)):
             if not isinstance(positions, torch.Tensor):
                 positions = torch.as_tensor(np.asarray(positions))
             positions = positions.to(x.device)
-        return _cuda_ops().rotary(x, f, positions, layout=self.layout, scale=self.scale, inplace=inplace)
+        return _cuda_ops().rotary(x, kept[2], positions, layout=self.layout, scale=self.scale, inplace=inplace)
 
     def turn_numpy(self, x: np.ndarray, positions=0) -> np.ndarray:
         """The same formula on the host, angles in 64 bits."""

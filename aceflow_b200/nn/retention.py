@@ -201,12 +201,17 @@ class MultiScaleRetention(Module):
         return self.forward_parallel(x, position)
 
     def forward_chunkwise(self, x: Tensor, chunk: int = DEFAULT_CHUNK, state: Optional[Tensor] = None,
-                          position=0) -> Tuple[Tensor, Tensor]:
+                          position=None) -> Tuple[Tensor, Tensor]:
         """Prefill x [B, T, d] from `state` (zeros if None) in chunks of
         `chunk` tokens; returns the layer output and the state after the last
-        token.  On CUDA this is the tcgen05 chunkwise kernel (bf16 operands,
+        token.  A layer with rotary= starts at position 0 unless told; with a
+        state it has to be told.  On CUDA this is the tcgen05 chunkwise kernel (bf16 operands,
         fp32 accumulation and state; head_dim 256); on CPU the recurrence."""
         B, T, d = x.shape
+        if position is None:
+            if self.rotary is not None and state is not None:
+                raise ValueError("a layer with rotary= needs the position at which x continues the state")
+            position = 0
         self._check_position(position)
         if not x.device.is_cuda:
             if state is None:
@@ -307,8 +312,6 @@ class MultiScaleRetention(Module):
         B, d = x_t.shape
         if (position is None) != (self.rotary is None):
             raise ValueError("a layer with rotary= needs the streams' position, one without takes none")
-        if position is not None and isinstance(position, (int, np.integer)):
-            position = np.full(B, position, np.int64)
         if state is None:
             state = self.init_state(B, x_t.device)
         if x_t.device.is_cuda:
@@ -330,7 +333,8 @@ class MultiScaleRetention(Module):
             return Tensor._wrap(out, x_t.device), state
         H, hd = self.num_heads, self.head_dim
         arr = x_t.numpy()
-        turned = (lambda a: a) if self.rotary is None else (lambda a: self.rotary.turn_numpy(a, position))
+        at = np.broadcast_to(position, (B,)) if self.rotary is not None else None
+        turned = (lambda a: a) if self.rotary is None else (lambda a: self.rotary.turn_numpy(a, at))
         q = turned((arr @ self.w_q.numpy().T).reshape(B, H, hd))
         k = turned((arr @ self.w_k.numpy().T).reshape(B, H, hd))
         v = (arr @ self.w_v.numpy().T).reshape(B, H, hd)
@@ -352,7 +356,10 @@ class MultiScaleRetention(Module):
         B, d = x.shape
         H, eps = self.num_heads, self.ret_norm.eps
         qkv = cuda_ops.linear(x, p["w_qkv"])
-        self.rotary.turn(qkv.view(B, 3 * H, self.head_dim)[:, :2 * H], position, inplace=True)
+        if isinstance(position, (int, np.integer)):
+            self._turn(qkv, B, 1, position)  # one position for all streams
+        else:
+            self.rotary.turn(qkv.view(B, 3 * H, self.head_dim)[:, :2 * H], position, inplace=True)
         o = cuda_ops.retention_step(state, p["gamma"], qkv[:, :d], qkv[:, d:2 * d], qkv[:, 2 * d:])
         if self.gated:
             gw, gb = self._gn_params()

@@ -159,5 +159,8 @@ def test_module_refusals():
         plain.forward_recurrent(af.Tensor(np.zeros((2, 64))), None, 5)
     with pytest.raises(ValueError, match="position"):
         turned.forward_recurrent(af.Tensor(np.zeros((2, 64))))
+    with pytest.raises(ValueError, match="position"):
+        turned.forward_chunkwise(x, state=turned.init_state(2))
+    turned.forward_chunkwise(x, state=turned.init_state(2), position=7)
     with pytest.raises(ValueError, match="CUDA"):
         af.ops.rotary(x, af.Tensor(np.ones(4)))

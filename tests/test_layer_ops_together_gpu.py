@@ -237,3 +237,48 @@ def test_a_training_step_of_a_layer(dev):
     ((zr * cz.double()).sum() + (norm(zr, ref["pre"]) * cy.double()).sum()).backward()
     for name in p:
         assert rel_err(leaf[name].grad.double().cpu().numpy(), ref[name].grad.cpu().numpy()) < 2e-2, name
+
+
+def test_a_captured_training_step(dev):
+    """Forward and backward of rotation and seam captured into two graphs of
+    different leaves and replayed in turn give the eager gradients."""
+    from aceflow_b200 import cuda_ops
+
+    freq, _ = cuda_ops.rotary_frequencies(64, device=dev)
+
+    def leaves(rows, seed):
+        g = torch.Generator(device=dev).manual_seed(seed)
+        return [torch.randn(*s, generator=g, device=dev).requires_grad_()
+                for s in ((rows, 320), (rows, 320), (rows, 320), (320,), (320,), (320,))]
+
+    def grads(t):
+        h = cuda_ops.rotary_autograd(t[1].view(-1, 5, 64), freq, 3).reshape(t[1].shape)
+        z, y = cuda_ops.residual_norm_autograd(t[0], h, gate=t[2], post_w=t[3], scale=t[4], pre_w=t[5])
+        return torch.autograd.grad((z * y).sum(), t)
+
+    sets, graphs = [leaves(40, 1), leaves(700, 2)], []
+    want = [[g.clone() for g in grads(t)] for t in sets]
+    for t in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = grads(t)
+        graphs.append((graph, out))
+    for _ in range(2):
+        for graph, _out in graphs:
+            graph.replay()
+    torch.cuda.synchronize()
+    for (_, out), ref in zip(graphs, want):
+        for a, b in zip(out, ref):
+            assert torch.equal(a, b)
+
+
+def test_rotary_frequencies_may_be_replaced(dev):
+    import aceflow_b200 as af
+
+    rot = af.nn.Rotary(64)
+    x = af.Tensor(np.random.default_rng(3).standard_normal((2, 3, 64)).astype(np.float32), device="cuda:0")
+    first = rot(x, 5).numpy()
+    rot.inv_freq *= 0.5
+    second = rot(x, 5).numpy()
+    rot.inv_freq = rot.inv_freq * 2.0
+    assert not np.array_equal(first, second) and np.array_equal(first, rot(x, 5).numpy())

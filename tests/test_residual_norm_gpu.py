@@ -249,3 +249,11 @@ def test_what_lies_between_rows_does_not_matter(dev, d, gap, dt):
     for k in ("x", "h", "gate"):
         t[k] = inside(t[k])
     _check(t, inside(dz), inside(dy), dt, 0.9)
+
+
+def test_more_rows_than_counters_hold_are_refused(dev):
+    from aceflow_b200 import cuda_ops
+
+    assert cuda_ops._seam_scratch(0, 2**30, 8) > 0
+    with pytest.raises(ValueError, match="bad sizes"):
+        cuda_ops._seam_scratch(0, 2**30 + 1, 8)
