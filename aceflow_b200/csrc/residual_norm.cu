@@ -21,16 +21,16 @@
 // z is formed again in fp32 from x, h and g (reading x costs what reading z
 // would), so the rounding of the stored z does not enter the gradients.
 //
-// Bound: HBM, every row of every tensor moved once; the backward and odd rows
-// by the issue of instructions and their latency, at 16 warps an SM.  A row is
+// Bound: HBM, every row of every tensor moved once; wide and odd rows by the
+// issue of instructions and their latency, at 16 warps an SM.  A row is
 // held in registers by one group of threads; sums, statistics and the row itself
 // are fp32, and each output is rounded once.  The column sums of the weights'
 // gradients stay with the threads while a block walks its rows, go out as one
 // partial row per group and are added in a fixed order by a second kernel: no
 // atomics, the same bits every run.
 // Measured with gate and all weights (floor: the tensors' bytes at 6547 GB/s):
-//   32768 x 2048 bf16   forward 111 us (0.93 of it), backward 228 (0.72)
-//   16384 x 2048 fp32            123 (0.83),                  188 (0.87)
+//   32768 x 2048 bf16   forward 110 us (0.93 of it), backward 182 (0.90)
+//   16384 x 2048 fp32            122 (0.84),                  186 (0.88)
 //    4096 x 8192 bf16             65 (0.79),                  139 (0.59)
 //   16384 x 1531 bf16             72 (0.53),                  133 (0.46)
 #include "common.cuh"
@@ -502,6 +502,30 @@ struct RawRow {
   }
 };
 
+// A row's statistics.
+struct RowStats {
+  float r1 = 1.f, r2 = 1.f;
+  __device__ __forceinline__ void load(const SeamParams &p, int row) {
+    if (row >= p.rows) return;
+    if (p.w1) r1 = p.stats[row];
+    if (p.w2) r2 = p.stats[p.rows + row];
+  }
+};
+
+__device__ __forceinline__ void ahead(const void *p, int64_t i, bool b16) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char *>(p) + i * (b16 ? 2 : 4)));
+}
+
+// Sends a chunk of a row that is not the first on its way into L2 (what is in
+// front of it is there); one thread in four reaches every 128 bytes.
+template <int VEC, bool SHIFT>
+__device__ __forceinline__ void ahead(const SeamParams &p, const Chunk<VEC, SHIFT> &k, int row, bool x16, bool h16) {
+  ahead(p.h, row * p.ldh + k.col, h16);
+  if (p.g) ahead(p.g, row * p.ldg + k.col, h16);
+  if (p.dz) ahead(p.dz, row * p.lddz + k.col, x16);
+  if (p.dy) ahead(p.dy, row * p.lddy + k.col, p.y16), ahead(p.x, row * p.ldx + k.col, x16);
+}
+
 // A row group's column sums, each its part of the planes.
 template <int VEC, int K, bool SHIFT>
 __device__ __forceinline__ void write_part(const SeamParams &p, int part, int phase, const float (&a1)[K][VEC],
@@ -520,6 +544,13 @@ template <int VEC, int K, int TX, int TH, bool one_warp, bool SHIFT>
 __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
   constexpr bool kAhead = VEC * K <= 8 && K <= 4;
   static_assert(kAhead || !SHIFT, "a group's rows share their phase");
+  // A row's statistics are read with the row before it (else it waits for them:
+  // 32768 x 2048 bf16 196 us against 224), and the row behind the next is sent on
+  // its way into L2 (182 against 196; fp32 rows have bytes enough under way
+  // without, 8192 x 4096 took 206 us against 194).  Where the threads at a row's
+  // ends need registers for their masks, either spills: 16384 x 1531 bf16 146 us
+  // against 132.
+  constexpr bool kStats = !SHIFT, kToL2 = VEC == 8 && !SHIFT && (TX || TH);
   __shared__ __align__(16) float red[kRed];
   int flip = 0;
   clear_red(red);
@@ -543,10 +574,13 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
       if (k.in) raw[c].load(p, k, row, x16, h16);
     }
   };
+  RowStats stats;
+  if (kStats) stats.load(p, part);
   if (kAhead && part < p.rows) fetch(part);
   for (int row = part; row < p.rows; row += p.parts) {
     if (!kAhead) fetch(row);
-    const float r1 = p.w1 ? p.stats[row] : 1.f, r2 = p.w2 ? p.stats[p.rows + row] : 1.f;
+    if (!kStats) stats.load(p, row);
+    const float r1 = stats.r1, r2 = stats.r2;
     Dot tz, eq, zq;  // t zh, e q, zh q
     // hh (h without post_w), swish and sigmoid of the gate, zh, e = dz + r2 t; q is what z has of n
     float hh[K][VEC], sw[K][VEC], sg[K][VEC], zh[K][VEC], e[K][VEC];
@@ -591,7 +625,15 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
         eq.add(e[c], q);
       }
     }
+    if (kStats) stats.load(p, row + p.parts);
     if (kAhead && row + p.parts < p.rows) fetch(row + p.parts);
+    if (kToL2 && row + 2 * p.parts < p.rows && threadIdx.x % 4 == 0) {
+#pragma unroll
+      for (int c = 0; c < K; ++c) {
+        const Chunk<VEC, SHIFT> k(p, c, phase);
+        if (k.in) ahead(p, k, row + 2 * p.parts, x16, h16);
+      }
+    }
     float sum[3] = {tz.sum(), eq.sum(), zq.sum()};
     if (p.w1 || p.dy) row_sum(sum, one_warp, red, flip);
     const float m2 = p.dy ? r2 * (sum[0] * p.inv_d) : 0.f;  // r2 mean(t zh)
@@ -715,10 +757,6 @@ struct Own {
   __device__ __forceinline__ void pre(float (&v)[8]) const { read(kind, v); }
 };
 
-__device__ __forceinline__ void ahead(const void *p, int64_t i, bool b16) {
-  asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char *>(p) + i * (b16 ? 2 : 4)));
-}
-
 // Rows of up to K 512 chunks: the row as it lies in memory stays in registers,
 // the columns' sums in shared memory where each thread alone touches its own, the
 // block's next row is on its way into L2.  So do weights of rows that start
@@ -763,12 +801,7 @@ __global__ void __launch_bounds__(512, 1) seam_backward_held_kernel(SeamParams p
 #pragma unroll
       for (int c = 0; c < K; ++c) {
         const Chunk<VEC, SHIFT> k(p, c, phase);
-        if (k.in) {  // next is not the first row: what is in front of it is there
-          ahead(p.h, next * p.ldh + k.col, h16);
-          if (p.g) ahead(p.g, next * p.ldg + k.col, h16);
-          if (p.dz) ahead(p.dz, next * p.lddz + k.col, x16);
-          if (p.dy) ahead(p.dy, next * p.lddy + k.col, p.y16), ahead(p.x, next * p.ldx + k.col, x16);
-        }
+        if (k.in) ahead(p, k, next, x16, h16);
       }
     }
     const float r1 = p.w1 ? p.stats[row] : 1.f, r2 = p.w2 ? p.stats[p.rows + row] : 1.f;
