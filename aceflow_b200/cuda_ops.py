@@ -652,6 +652,11 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: str | No
     return torch.tensor(freq, dtype=F32, device=device), scale
 
 
+def _new(t: torch.Tensor, dtype=None) -> torch.Tensor:
+    """A new contiguous tensor of t's shape and device."""
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def _same_device(x: torch.Tensor, **others) -> None:
     dev = x.get_device()  # -1 on the CPU
     for n, t in others.items():
@@ -719,7 +724,7 @@ def rotary(x: torch.Tensor, inv_freq: torch.Tensor, positions=0, *, layout: str 
             reach = s * (n - 1) + reach
         out, ost = x, st
     else:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _new(x)
         ost = (T * H * D, H * D, D)
     _device_call("af_rotary", dev, x.data_ptr(), out.data_ptr(), x.dtype == BF16, _Strides(*st), _Strides(*ost), B, T, H,
                  D, inv_freq.data_ptr(), rot, _p(pos), pos is not None and pos.dtype == torch.int64,
@@ -834,8 +839,8 @@ def residual_norm(x: torch.Tensor, h: torch.Tensor, *, gate: torch.Tensor | None
     if out_dtype not in (F32, BF16):
         raise ValueError("out_dtype must be float32 or bfloat16")
     dev = _dev(x)
-    z = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    y = None if pre_w is None else torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    z = _new(x)
+    y = None if pre_w is None else _new(x, out_dtype)
     stats = torch.empty(2, rows, dtype=F32, device=x.device) if want_stats else None
     _device_call("af_residual_norm", dev, _p(xt), ldx, x.dtype == BF16, _p(ht), ldh, h.dtype == BF16, _p(gt), ldg,
                  _p(post_w), _p(scale), _p(pre_w), alpha, eps, rows, d, _p(z), _p(y), out_dtype == BF16, _p(stats))
@@ -862,7 +867,7 @@ def residual_norm_backward(dz: torch.Tensor | None, dy: torch.Tensor | None, x: 
         raise ValueError(f"dz: expected {x.dtype} as x, got {dz.dtype}")
     _same_device(x, stats=stats, dz=dz, dy=dy)
     dev = _dev(x)
-    new = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+    new = lambda t: None if t is None else _new(t)  # noqa: E731
     g = ResidualNormGrads(new(x), new(h), new(gate), new(post_w), new(scale), new(pre_w))
     floats, scratch = 0, None
     if not (post_w is None and scale is None and pre_w is None):
