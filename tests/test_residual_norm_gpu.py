@@ -257,3 +257,25 @@ def test_more_rows_than_counters_hold_are_refused(dev):
     assert cuda_ops._seam_scratch(0, 2**30, 8) > 0
     with pytest.raises(ValueError, match="bad sizes"):
         cuda_ops._seam_scratch(0, 2**30 + 1, 8)
+
+
+def test_offsets_beyond_31_bits(dev):
+    """More than 2^31 values: the last rows are those of a small call."""
+    from aceflow_b200 import cuda_ops
+
+    rows, d, last = 1073800, 2001, 5  # rows that start anywhere
+    g = torch.Generator(device=dev).manual_seed(5)
+    x, h, dz = (torch.zeros(rows, d, device=dev, dtype=BF16) for _ in range(3))
+    w = 1 + 0.1 * torch.randn(d, generator=g, device=dev)
+    for t in (x, h, dz):
+        t[-last:] = torch.randn(last, d, generator=g, device=dev).to(BF16)
+    small = [t[-last:].clone() for t in (x, h, dz)]
+    z, y, stats = cuda_ops.residual_norm(x, h, post_w=w, pre_w=w, want_stats=True)
+    sz, sy, sstats = cuda_ops.residual_norm(*small[:2], post_w=w, pre_w=w, want_stats=True)
+    assert torch.equal(z[-last:], sz) and torch.equal(y[-last:], sy) and not z[0].any()
+    del z, y
+    got = cuda_ops.residual_norm_backward(dz, None, x, h, stats, post_w=w, pre_w=w)
+    ref = cuda_ops.residual_norm_backward(small[2], None, *small[:2], sstats, post_w=w, pre_w=w)
+    assert torch.equal(got.x[-last:], ref.x) and torch.equal(got.h[-last:], ref.h)
+    # the same terms and zeros, in another grouping
+    assert torch.allclose(got.post_w, ref.post_w, rtol=1e-5, atol=1e-5)

@@ -215,3 +215,17 @@ def test_many_rows_take_fewer_blocks_each(dev, rows, V):
     assert (many[0][:2] == few[0]).all() and (many[1][:2] == few[1]).all()
     part = _draw(dev, logits[:48], u[:48], **{k: v[:48] for k, v in kw.items()})
     assert (many[0][:48] == part[0]).all() and (many[1][:48] == part[1]).all()
+
+
+def test_offsets_beyond_31_bits(dev):
+    """Logits with more than 2^31 values: the last rows draw as they do alone."""
+    from aceflow_b200 import cuda_ops
+
+    rows, V, last = 16400, 131072, 4
+    g = torch.Generator(device=dev).manual_seed(9)
+    lg = torch.zeros(rows, V, device=dev, dtype=torch.bfloat16)
+    lg[-last:] = (2.5 * torch.randn(last, V, generator=g, device=dev)).bfloat16()
+    u = torch.rand(rows, generator=g, device=dev)
+    kw = dict(top_k=50, top_p=0.9, return_logprobs=True)
+    many, few = cuda_ops.sample_tokens(lg, u, **kw), cuda_ops.sample_tokens(lg[-last:].clone(), u[-last:].clone(), **kw)
+    assert torch.equal(many[0][-last:], few[0]) and torch.equal(many[1][-last:], few[1])
