@@ -178,6 +178,11 @@ __device__ __forceinline__ uint32_t cluster_ctas() {
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
+// Another CTA's memory may be touched only once that CTA runs: each says so as
+// it starts and waits for the others in front of the first exchange, by when
+// its slice is loaded.
+__device__ __forceinline__ void cluster_started() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_all_started() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
 // All threads of the cluster, whether or not their warps have reconverged.
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
@@ -813,6 +818,7 @@ __device__ __noinline__ void descend(Row row, Weigher weigh, Filters f, int32_t 
 }
 
 __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams p) {
+  cluster_started();
   extern __shared__ __align__(16) unsigned char smem[];
   const uint32_t sm = sm100::smem_u32(smem), logits = sm + Layout::logits;
   const uint32_t seen = logits + 4 * p.slice;  // a bit for each token of the context in this slice
@@ -912,6 +918,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
   __syncthreads();
 
   // 1. the maximum
+  cluster_all_started();
   top = value_of(row.largest(key_of(top)));
   auto write = [&](int token, float logp) {
     p.token[r] = token;
