@@ -273,6 +273,32 @@ def retention_chunkwise_backward_bf16(qkv: torch.Tensor, dout: torch.Tensor, B: 
     return dqkv, dstate
 
 
+class _GradientsOnly(torch.autograd.Function):
+    """Gradients on their way out of a backward pass that has none of its own.
+    With create_graph they depend on `sources` (torch takes a node's results
+    for constants otherwise, and a second derivative would lose its terms
+    through it without a word); whoever asks for that dependence gets an error."""
+
+    @staticmethod
+    def forward(ctx, name, count, *grads_and_sources):
+        ctx.name = name
+        return tuple(g.view_as(g) for g in grads_and_sources[:count])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.name} has no second derivative")
+
+
+def _gradients_only(name: str, grads, sources):
+    """`grads` (None where there is none) as a backward pass returns them that
+    has no derivative, see _GradientsOnly."""
+    if not torch.is_grad_enabled():
+        return tuple(grads)
+    given = [g for g in grads if g is not None]
+    out = iter(_GradientsOnly.apply(name, len(given), *given, *(s for s in sources if s is not None)))
+    return tuple(None if g is None else next(out) for g in grads)
+
+
 class _RetentionChunkwise(torch.autograd.Function):
     """Autograd node of the chunkwise retention core: forward
     af_retention_chunkwise_bf16 (no norm weight), backward
@@ -732,15 +758,20 @@ def rotary(x: torch.Tensor, inv_freq: torch.Tensor, positions=0, *, layout: str 
     return out
 
 
+def _rotary_turn(x, inv_freq, positions, layout, scale, inverse):
+    return rotary(x, inv_freq, positions, layout=layout, scale=scale, inverse=inverse)
+
+
 class _Rotary(torch.autograd.Function):
-    """Autograd node of `rotary`: the gradient is the inverse rotation."""
+    """Autograd node of `rotary`: the gradient is the inverse rotation, and so
+    differentiable itself."""
 
     @staticmethod
     def forward(ctx, x, inv_freq, positions, layout, scale, inverse):
         tensors = (inv_freq, positions) if isinstance(positions, torch.Tensor) else (inv_freq,)
         ctx.save_for_backward(*tensors)
         ctx.args = (positions if len(tensors) == 1 else None, layout, scale, inverse)
-        return rotary(x, inv_freq, positions, layout=layout, scale=scale, inverse=inverse)
+        return _rotary_turn(x, inv_freq, positions, layout, scale, inverse)
 
     @staticmethod
     def backward(ctx, dout):
@@ -749,13 +780,14 @@ class _Rotary(torch.autograd.Function):
         pos = start if start is not None else ctx.saved_tensors[1]
         if dout.stride(-1) != 1:
             dout = dout.contiguous()
-        return rotary(dout, inv_freq, pos, layout=layout, scale=scale, inverse=not inverse), None, None, None, None, None
+        turn = _Rotary.apply if torch.is_grad_enabled() else _rotary_turn  # with create_graph, a node of its own
+        return turn(dout, inv_freq, pos, layout, scale, not inverse), None, None, None, None, None
 
 
 def rotary_autograd(x: torch.Tensor, inv_freq: torch.Tensor, positions=0, *, layout: str = "interleaved",
                     scale: float = 1.0, inverse: bool = False) -> torch.Tensor:
-    """`rotary` as a differentiable torch op (gradients flow to x; inv_freq
-    and positions are constants).  Forward and backward can be captured into a
+    """`rotary` as a differentiable torch op (gradients of any order flow to x;
+    inv_freq and positions are constants).  Forward and backward can be captured into a
     CUDA graph; as for every torch op, not while an eager graph of the same
     leaves is alive (torch then accumulates on the eager stream and the capture
     raises)."""
@@ -905,14 +937,15 @@ class _ResidualNorm(torch.autograd.Function):
         x, h, gate, post_w, scale, pre_w, stats = ctx.saved_tensors
         g = residual_norm_backward(dz, dy, x, h, stats, gate=gate, post_w=post_w, scale=scale, pre_w=pre_w,
                                    alpha=ctx.alpha)
-        return g.x, g.h, g.gate, g.post_w, g.scale, g.pre_w, None, None, None
+        return _gradients_only("residual_norm", g, (dz, dy, x, h, gate, post_w, scale, pre_w)) + (None, None, None)
 
 
 def residual_norm_autograd(x: torch.Tensor, h: torch.Tensor, *, gate: torch.Tensor | None = None,
                            post_w: torch.Tensor | None = None, scale: torch.Tensor | None = None,
                            pre_w: torch.Tensor | None = None, alpha: float = 1.0, eps: float = 1e-6, out_dtype=None):
     """residual_norm as a differentiable torch op: (z, y), gradients to x, h,
-    gate and the weights.  Captured as rotary_autograd is."""
+    gate and the weights, which have none themselves (a second derivative
+    raises).  Captured as rotary_autograd is."""
     return _ResidualNorm.apply(x, h, gate, post_w, scale, pre_w, float(alpha), float(eps), out_dtype)
 
 

@@ -1,0 +1,60 @@
+"""What needs no GPU of the operators around the retention core, where it goes
+wrong first: second derivatives (of stand-ins for the device calls), in-place
+turns of tensors that autograd needs, settings and positions out of range."""
+import numpy as np
+import pytest
+import torch
+
+from aceflow_b200 import cuda_ops
+
+
+def _turn(x, f, positions=0, *, layout="half", scale=1.0, inverse=False, inplace=False):
+    th = torch.as_tensor(positions + torch.arange(x.shape[-3]))[:, None, None] * f
+    c, s = scale * th.cos(), scale * (-th.sin() if inverse else th.sin())
+    a, b = x.chunk(2, -1)
+    return torch.cat((a * c - b * s, a * s + b * c), -1).detach()
+
+
+def test_second_derivative_of_the_rotation(monkeypatch):
+    """|gradient|^2 as a penalty, against the same through torch's own operations."""
+    monkeypatch.setattr(cuda_ops, "rotary", _turn)
+    f = torch.tensor([0.5, 0.1])
+    got = []
+    for own in (True, False):
+        x = torch.linspace(-1, 2, 24).view(1, 3, 2, 4).requires_grad_()
+        if own:
+            y = cuda_ops.rotary_autograd(x, f, 3, layout="half", scale=1.5)
+        else:
+            th = (3 + torch.arange(3))[:, None, None] * f
+            a, b = x.chunk(2, -1)
+            y = 1.5 * torch.cat((a * th.cos() - b * th.sin(), a * th.sin() + b * th.cos()), -1)
+        g, = torch.autograd.grad((y ** 3).sum(), x, create_graph=True)
+        assert g.requires_grad
+        got.append(torch.autograd.grad(g.square().sum() + x.sum(), x)[0])
+    assert torch.allclose(got[0], got[1], rtol=1e-4, atol=1e-4)
+
+
+def _seam(*args, want_stats=False, out_dtype=None, **kw):
+    return args[0] * 2, args[0] * 3, torch.zeros(2, args[0].shape[0])
+
+
+def _seam_grads(dz, dy, x, h, stats, *, gate, post_w, scale, pre_w, alpha):
+    like = [None if t is None else torch.ones_like(t) for t in (x, h, gate, post_w, scale, pre_w)]
+    return cuda_ops.ResidualNormGrads(*like)
+
+
+@pytest.mark.parametrize("linear", [True, False])
+def test_second_derivative_of_the_seam_raises(monkeypatch, linear):
+    """Also where the loss is linear in the outputs, so that the upstream gradient
+    is a constant: the seam's gradients depend on x all the same."""
+    monkeypatch.setattr(cuda_ops, "residual_norm", _seam)
+    monkeypatch.setattr(cuda_ops, "residual_norm_backward", _seam_grads)
+    x, h, w = torch.ones(3, 4).requires_grad_(), torch.ones(3, 4), torch.ones(4).requires_grad_()
+    z, y = cuda_ops.residual_norm_autograd(x, h, pre_w=w)
+    loss = z.sum() + y.sum() if linear else (z * y).sum()
+    gx, gw = torch.autograd.grad(loss, (x, w), create_graph=True)
+    with pytest.raises(RuntimeError, match="residual_norm has no second derivative"):
+        torch.autograd.grad(gx.square().sum() + x.square().sum(), x)
+    loss = cuda_ops.residual_norm_autograd(x, h, pre_w=w)[0].sum()
+    loss.backward()  # without create_graph nothing changes
+    assert x.grad is not None and not x.grad.requires_grad and torch.all(x.grad == 1)
