@@ -316,13 +316,14 @@ class _RetentionChunkwise(torch.autograd.Function):
         qkv, gamma = ctx.saved_tensors
         B, T, H = ctx.dims
         dqkv, _ = retention_chunkwise_backward_bf16(qkv, dout.to(BF16).contiguous(), B, T, H, gamma)
-        return dqkv, None, None, None, None, None
+        return _gradients_only("retention_chunkwise", (dqkv,), (dout, qkv)) + (None,) * 5
 
 
 def retention_chunkwise_autograd(qkv: torch.Tensor, B: int, T: int, H: int, gamma: torch.Tensor,
                                  chunk: int = 128) -> torch.Tensor:
     """The chunkwise retention core [B*T, 3*H*256] bf16 -> [B*T, H*256] bf16
-    as a differentiable torch op (training: gradients flow to qkv)."""
+    as a differentiable torch op (training: gradients flow to qkv; a second
+    derivative raises)."""
     return _RetentionChunkwise.apply(qkv, B, T, H, gamma, chunk)
 
 

@@ -58,3 +58,13 @@ def test_second_derivative_of_the_seam_raises(monkeypatch, linear):
     loss = cuda_ops.residual_norm_autograd(x, h, pre_w=w)[0].sum()
     loss.backward()  # without create_graph nothing changes
     assert x.grad is not None and not x.grad.requires_grad and torch.all(x.grad == 1)
+
+
+def test_second_derivative_of_the_retention_core_raises(monkeypatch):
+    monkeypatch.setattr(cuda_ops, "retention_chunkwise_bf16", lambda qkv, *a, **k: (qkv[:, :4] * 1, None, None))
+    monkeypatch.setattr(cuda_ops, "retention_chunkwise_backward_bf16", lambda qkv, *a: (torch.ones_like(qkv), None))
+    qkv = torch.ones(3, 12, dtype=torch.bfloat16).requires_grad_()
+    g, = torch.autograd.grad(cuda_ops.retention_chunkwise_autograd(qkv, 1, 3, 1, torch.ones(1)).sum(), qkv,
+                             create_graph=True)
+    with pytest.raises(RuntimeError, match="retention_chunkwise has no second derivative"):
+        torch.autograd.grad(g.sum() + qkv.sum(), qkv)
