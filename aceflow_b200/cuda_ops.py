@@ -718,7 +718,8 @@ def rotary(x: torch.Tensor, inv_freq: torch.Tensor, positions=0, *, layout: str 
     of each head; positions is the first token's position (tokens follow one
     by one), or an int32 / int64 tensor [T] or [B, T] ([rows] for a 3-D x).
     inverse turns back (times scale all the same: the gradient).  Returns a
-    new contiguous tensor, or x itself with inplace."""
+    new contiguous tensor, or x itself with inplace (autograd sees it as changed;
+    one that requires a gradient is refused while gradients are recorded)."""
     B, T, H, D, st = _rotary_dims(x)
     _need(inv_freq, F32, "inv_freq")
     if layout not in ROTARY_LAYOUTS:
@@ -743,6 +744,8 @@ def rotary(x: torch.Tensor, inv_freq: torch.Tensor, positions=0, *, layout: str 
         start = int(positions)
         _same_device(x, inv_freq=inv_freq)
     if inplace:
+        if x.requires_grad and torch.is_grad_enabled():
+            raise ValueError("inplace: x requires a gradient; use rotary_autograd")
         ext = sorted((s, n) for s, n in zip(st + (1,), (B, T, H, D)) if n > 1)
         reach = 1
         for s, n in ext:
@@ -756,6 +759,8 @@ def rotary(x: torch.Tensor, inv_freq: torch.Tensor, positions=0, *, layout: str 
     _device_call("af_rotary", dev, x.data_ptr(), out.data_ptr(), x.dtype == BF16, _Strides(*st), _Strides(*ost), B, T, H,
                  D, inv_freq.data_ptr(), rot, _p(pos), pos is not None and pos.dtype == torch.int64,
                  _PosStrides(*pst), start, layout == "interleaved", scale, inverse)
+    if inplace:
+        torch.autograd.graph.increment_version(x)
     return out
 
 

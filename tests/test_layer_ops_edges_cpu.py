@@ -68,3 +68,23 @@ def test_second_derivative_of_the_retention_core_raises(monkeypatch):
                              create_graph=True)
     with pytest.raises(RuntimeError, match="retention_chunkwise has no second derivative"):
         torch.autograd.grad(g.sum() + qkv.sum(), qkv)
+
+
+def test_turning_in_place_what_autograd_needs(monkeypatch):
+    monkeypatch.setattr(cuda_ops, "_dev", lambda t: 0)
+    monkeypatch.setattr(cuda_ops, "_device_call", lambda *a: None)
+    f = torch.ones(2)
+    x = torch.ones(1, 3, 2, 4)
+    w = torch.ones_like(x).requires_grad_()
+    loss = (w * x).sum()  # the product keeps x
+    assert cuda_ops.rotary(x, f, inplace=True) is x
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with pytest.raises(ValueError, match="inplace: x requires a gradient"):
+        cuda_ops.rotary(w, f, inplace=True)
+    with pytest.raises(ValueError, match="inplace: x requires a gradient"):
+        cuda_ops.rotary((w * 2)[:, 1:], f, inplace=True)
+    with torch.no_grad():
+        assert cuda_ops.rotary(w, f, inplace=True) is w
+    with torch.inference_mode():
+        cuda_ops.rotary(torch.ones(1, 3, 2, 4), f, inplace=True)
