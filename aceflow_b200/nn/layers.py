@@ -124,19 +124,28 @@ class Rotary(Module):
                                                            original_length=original_length)
         self._on = {}  # (inv_freq, its version, its copy) for each device it was used on
 
+    def _frequencies_on(self, device):
+        """inv_freq's copy on a device."""
+        import torch
+
+        src = self.inv_freq
+        # tensors made in inference mode count no versions: their values stand for one
+        version = src.tolist() if src.is_inference() else src._version
+        kept = self._on.get(device)
+        if kept is None or kept[0] is not src or kept[1] != version:
+            with torch.inference_mode(False):
+                kept = self._on[device] = (src, version, src.to(device, copy=True))
+        return kept[2]
+
     def turn(self, x, positions=0, inplace: bool = False):
         """The CUDA form on torch tensors (af_rotary)."""
         import torch
 
-        src = self.inv_freq
-        kept = self._on.get(x.device)
-        if kept is None or kept[0] is not src or kept[1] != src._version:
-            kept = self._on[x.device] = (src, src._version, src.to(x.device))
         if not isinstance(positions, (int, np.integer)):
             if not isinstance(positions, torch.Tensor):
                 positions = torch.as_tensor(np.asarray(positions))
             positions = positions.to(x.device)
-        return _cuda_ops().rotary(x, kept[2], positions, layout=self.layout, scale=self.scale, inplace=inplace)
+        return _cuda_ops().rotary(x, self._frequencies_on(x.device), positions, layout=self.layout, scale=self.scale, inplace=inplace)
 
     def turn_numpy(self, x: np.ndarray, positions=0) -> np.ndarray:
         """The same formula on the host, angles in 64 bits."""

@@ -88,3 +88,24 @@ def test_turning_in_place_what_autograd_needs(monkeypatch):
         assert cuda_ops.rotary(w, f, inplace=True) is w
     with torch.inference_mode():
         cuda_ops.rotary(torch.ones(1, 3, 2, 4), f, inplace=True)
+
+
+def _given_frequencies(monkeypatch):
+    """nn.Rotary.turn returns the frequencies that it hands to the device call."""
+    monkeypatch.setattr(cuda_ops, "rotary", lambda x, f, *a, **k: f)
+
+
+def test_rotary_module_made_in_inference_mode(monkeypatch):
+    import aceflow_b200 as af
+
+    _given_frequencies(monkeypatch)
+    with torch.inference_mode():
+        rot = af.nn.Rotary(8)
+        x = torch.zeros(1, 2, 1, 8)
+        assert torch.equal(rot.turn(x), rot.inv_freq)
+    assert torch.equal(rot.turn(x), rot.inv_freq)
+    with torch.inference_mode():
+        rot.inv_freq *= 0.5
+        assert torch.equal(rot.turn(x), rot.inv_freq)
+        rot.inv_freq = rot.inv_freq * 3
+    assert torch.equal(rot.turn(x), rot.inv_freq)
