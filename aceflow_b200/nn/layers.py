@@ -106,7 +106,8 @@ class Rotary(Module):
 
     forward(x, positions=0): x [B, T, heads, head_dim] or [rows, heads, head_dim],
     positions the first token's position or an integer array [T] or [B, T]
-    ([rows] for a 3-D x)."""
+    ([rows] for a 3-D x).  The first call on a device copies inv_freq there, so
+    it comes before a capture, as does one after inv_freq was changed."""
 
     def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, base: float = 10000.0, *,
                  layout: str = "interleaved", scaling: Optional[str] = None, factor: float = 1.0,
@@ -125,7 +126,8 @@ class Rotary(Module):
         self._on = {}  # (inv_freq, its version, its copy) for each device it was used on
 
     def _frequencies_on(self, device):
-        """inv_freq's copy on a device."""
+        """inv_freq's copy on a device.  New frequencies of the same number go into
+        the same memory, so steps captured before turn by them as well."""
         import torch
 
         src = self.inv_freq
@@ -134,7 +136,12 @@ class Rotary(Module):
         kept = self._on.get(device)
         if kept is None or kept[0] is not src or kept[1] != version:
             with torch.inference_mode(False):
-                kept = self._on[device] = (src, version, src.to(device, copy=True))
+                if kept is not None and kept[2].shape == src.shape and kept[2].dtype == src.dtype:
+                    copy = kept[2].copy_(src)
+                else:
+                    copy = src.to(device, copy=True)
+                self._on[device] = (src, version, copy)
+            return copy
         return kept[2]
 
     def turn(self, x, positions=0, inplace: bool = False):

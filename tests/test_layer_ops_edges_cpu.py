@@ -109,3 +109,20 @@ def test_rotary_module_made_in_inference_mode(monkeypatch):
         assert torch.equal(rot.turn(x), rot.inv_freq)
         rot.inv_freq = rot.inv_freq * 3
     assert torch.equal(rot.turn(x), rot.inv_freq)
+
+
+def test_new_frequencies_reach_captured_steps(monkeypatch):
+    """They go where a captured step reads them; the tensor they replace stays."""
+    import aceflow_b200 as af
+
+    _given_frequencies(monkeypatch)
+    rot, x = af.nn.Rotary(8), torch.zeros(1, 2, 1, 8)
+    first = rot.inv_freq
+    read = rot.turn(x)
+    for change in (lambda f: f * 0.5, lambda f: f.mul_(3), lambda f: f.clone()):
+        rot.inv_freq = change(rot.inv_freq)
+        again = rot.turn(x)
+        assert again.data_ptr() == read.data_ptr() and torch.equal(read, rot.inv_freq)
+    assert first[0] == 1.0
+    rot.inv_freq = torch.ones(2)
+    assert rot.turn(x).tolist() == [1.0, 1.0] and read.numel() == 4
