@@ -155,9 +155,14 @@ class Rotary(Module):
         return _cuda_ops().rotary(x, self._frequencies_on(x.device), positions, layout=self.layout, scale=self.scale, inplace=inplace)
 
     def turn_numpy(self, x: np.ndarray, positions=0) -> np.ndarray:
-        """The same formula on the host, angles in 64 bits."""
+        """The same formula on the host, angles in 64 bits; positions as for turn."""
         if isinstance(positions, (int, np.integer)):
             positions = int(positions) + np.arange(x.shape[-3])
+        positions = np.asarray(positions)
+        if positions.dtype not in (np.int32, np.int64):
+            raise ValueError(f"positions: expected int32 or int64, got {positions.dtype}")
+        if positions.shape not in (x.shape[-3:-2], x.shape[:-2]):
+            raise ValueError(f"positions of shape {positions.shape} do not match x {x.shape}")
         th = np.asarray(positions, np.float64)[..., None, None] * self.inv_freq.numpy().astype(np.float64)
         cos, sin = (self.scale * f(th) for f in (np.cos, np.sin))
         half = self.inv_freq.numel()

@@ -218,6 +218,8 @@ class MultiScaleRetention(Module):
                 state = self.init_state(B, x.device)
             outs = []
             at = position + np.arange(T) if isinstance(position, (int, np.integer)) else np.asarray(position)
+            if at.shape not in ((T,), (B, T)):
+                raise ValueError(f"positions of shape {at.shape} do not match x {(B, T, d)}")
             at = np.broadcast_to(at, (B, T))
             for t in range(T):
                 o, state = self.forward_recurrent(Tensor(x.numpy()[:, t]), state,
@@ -333,7 +335,7 @@ class MultiScaleRetention(Module):
             return Tensor._wrap(out, x_t.device), state
         H, hd = self.num_heads, self.head_dim
         arr = x_t.numpy()
-        at = np.broadcast_to(position, (B,)) if self.rotary is not None else None
+        at = np.full(B, position) if isinstance(position, (int, np.integer)) else position
         turned = (lambda a: a) if self.rotary is None else (lambda a: self.rotary.turn_numpy(a, at))
         q = turned((arr @ self.w_q.numpy().T).reshape(B, H, hd))
         k = turned((arr @ self.w_k.numpy().T).reshape(B, H, hd))

@@ -126,3 +126,37 @@ def test_new_frequencies_reach_captured_steps(monkeypatch):
     assert first[0] == 1.0
     rot.inv_freq = torch.ones(2)
     assert rot.turn(x).tolist() == [1.0, 1.0] and read.numel() == 4
+
+
+@pytest.mark.parametrize("bad", [1.5, np.array([0.0, 1.0, 2.0]), np.array(3), np.arange(2), np.zeros((3, 2), int),
+                                 np.zeros((1, 3), int), np.zeros(3, np.int16), None])
+def test_positions_that_the_device_refuses_are_refused_on_the_host(bad):
+    import aceflow_b200 as af
+
+    x = af.Tensor(np.ones((2, 3, 4, 8)))
+    with pytest.raises(ValueError, match="positions"):
+        af.nn.Rotary(8)(x, bad)
+    m = af.nn.MultiScaleRetention(32, 4, rotary=af.nn.Rotary(8))
+    for call in (lambda: m(af.Tensor(np.ones((2, 3, 32))), bad),
+                 lambda: m.forward_chunkwise(af.Tensor(np.ones((2, 3, 32))), position=bad if bad is not None else 0.5),
+                 lambda: m.forward_recurrent(af.Tensor(np.ones((3, 32))), None,
+                                             bad if bad is not None and np.shape(bad) != (3,) else np.ones(3))):
+        with pytest.raises(ValueError, match="positions"):
+            call()
+
+
+def test_positions_on_the_host():
+    import aceflow_b200 as af
+
+    rng = np.random.default_rng(1)
+    rot = af.nn.Rotary(8)
+    x = rng.standard_normal((2, 3, 4, 8)).astype(np.float32)
+    want = rot(af.Tensor(x), 4).numpy()
+    for same in (np.arange(4, 7), np.arange(4, 7, dtype=np.int32), np.tile(np.arange(4, 7), (2, 1)), np.int64(4),
+                 torch.arange(4, 7)):
+        assert np.array_equal(rot(af.Tensor(x), same).numpy(), want)
+    m = af.nn.MultiScaleRetention(32, 4, rotary=rot)
+    t = rng.standard_normal((3, 32)).astype(np.float32)
+    a, _ = m.forward_recurrent(af.Tensor(t), None, 5)
+    b, _ = m.forward_recurrent(af.Tensor(t), None, np.array([5, 5, 5]))
+    assert np.array_equal(a.numpy(), b.numpy())
