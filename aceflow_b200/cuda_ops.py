@@ -605,6 +605,12 @@ def rms_norm_to_bf16(x: torch.Tensor, w: torch.Tensor | None, eps: float) -> tor
     return y
 
 
+def c_int(k) -> int:
+    """A top_k as the C int that means the same (beyond 2^31 it would mean another
+    one): more than every token cuts nothing, and less than none is less than none."""
+    return min(max(int(k), -2 ** 31), 2 ** 31 - 1)
+
+
 def sample_rows(logits: torch.Tensor, uniforms: torch.Tensor | None = None, context: torch.Tensor | None = None,
                 temperature: float = 0.7, top_k: int = 40, top_p: float = 0.9,
                 repetition_penalty: float = 1.2) -> torch.Tensor:
@@ -628,7 +634,7 @@ def sample_rows(logits: torch.Tensor, uniforms: torch.Tensor | None = None, cont
         ctx_ptr, stride, clen = _p(context), context.stride(0), context.shape[1]
     out = torch.empty(rows, dtype=torch.int32, device=logits.device)
     _lib.call("af_sample_rows", _ctx(logits), _p(logits), rows, V, ctx_ptr, int(stride), int(clen), float(temperature),
-              int(top_k), float(top_p), float(repetition_penalty), _p(uniforms), _p(out), _stream(logits))
+              c_int(top_k), float(top_p), float(repetition_penalty), _p(uniforms), _p(out), _stream(logits))
     return out
 
 
@@ -1005,6 +1011,6 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1
     token = torch.empty(rows, dtype=torch.int32, device=dev)
     logp = torch.empty(rows, dtype=F32, device=dev) if return_logprobs else None
     _device_call("af_sample_tokens", index, logits.data_ptr(), logits.dtype == BF16, logits.stride(0), rows, V, c_ptr,
-                 c_stride, c_len, t_ptr, t_all, k_ptr, int(k_all), p_ptr, p_all, m_ptr, m_all, r_ptr, r_all,
+                 c_stride, c_len, t_ptr, t_all, k_ptr, c_int(k_all), p_ptr, p_all, m_ptr, m_all, r_ptr, r_all,
                  uniforms.data_ptr(), token.data_ptr(), _p(logp))
     return (token, logp) if return_logprobs else token

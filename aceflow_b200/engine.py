@@ -469,7 +469,7 @@ class AceEngine:
                 seen[:, n_seen] = toks
             elif sampling:
                 _lib.call("af_sample_rows", self._ctx(), logits.data_ptr(), B, V, win.data_ptr() if n_seen else None,
-                          seen.stride(0), n_seen - w0, float(temperature), int(top_k), float(top_p),
+                          seen.stride(0), n_seen - w0, float(temperature), cuda_ops.c_int(top_k), float(top_p),
                           float(repetition_penalty), ur.data_ptr(), toks.data_ptr(), st)
                 seen[:, n_seen] = toks
             out[:, s] = torch.where(alive, toks, torch.full_like(toks, -1))
@@ -497,9 +497,10 @@ class AceEngine:
         out = {}
         for name, v in given.items():
             if np.ndim(v) == 0:
-                out[name] = int(v) if name == "top_k" else float(v)
+                out[name] = cuda_ops.c_int(v) if name == "top_k" else float(v)
                 continue
-            a = np.asarray(v, np.int32 if name == "top_k" else np.float32).reshape(-1)
+            a = [cuda_ops.c_int(k) for k in v] if name == "top_k" else v
+            a = np.asarray(a, np.int32 if name == "top_k" else np.float32).reshape(-1)
             if a.size != self.batch:
                 raise ValueError(f"{name}: expected one value or {self.batch}, got {a.size}")
             if name == "repetition_penalty" and not np.all(a > 0):

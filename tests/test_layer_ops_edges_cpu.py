@@ -160,3 +160,26 @@ def test_positions_on_the_host():
     a, _ = m.forward_recurrent(af.Tensor(t), None, 5)
     b, _ = m.forward_recurrent(af.Tensor(t), None, np.array([5, 5, 5]))
     assert np.array_equal(a.numpy(), b.numpy())
+
+
+def test_top_k_beyond_31_bits_cuts_nothing(monkeypatch):
+    from types import SimpleNamespace
+
+    from aceflow_b200.engine import AceEngine
+
+    for k, means in ((2 ** 32 + 5, 2 ** 31 - 1), (2 ** 31, 2 ** 31 - 1), (-2 ** 32 + 5, -2 ** 31), (7, 7), (0, 0)):
+        calls = []
+        monkeypatch.setattr(cuda_ops, "_dev", lambda t: 0)
+        monkeypatch.setattr(cuda_ops, "_ctx", lambda t: 0)
+        monkeypatch.setattr(cuda_ops, "_stream", lambda t: 0)
+        monkeypatch.setattr(cuda_ops, "_device_call", lambda name, *a: calls.append(a))
+        monkeypatch.setattr(cuda_ops._lib, "call", lambda name, *a: calls.append(a))
+        cuda_ops.sample_tokens(torch.zeros(2, 5), torch.zeros(2), top_k=k)
+        cuda_ops.sample_rows(torch.zeros(2, 5), torch.zeros(2), top_k=k, temperature=1.0)
+        for call in calls:
+            assert means in call and (k in call) == (k == means)
+        engine = SimpleNamespace(batch=2, vocab_size=5, device="cpu")
+        got = AceEngine._filters(engine, 1.0, k, 1.0, 0.1, 1.0)["top_k"]
+        assert got == means
+        got = AceEngine._filters(engine, 1.0, [k, 3], 1.0, 0.0, 1.0)["top_k"]
+        assert got.dtype == torch.int32 and got.tolist() == [means, 3]
