@@ -415,7 +415,9 @@ class AceEngine:
         [batch]; per-stream settings, a min_p (not in the reference) and
         vocabularies beyond af_sample_rows' run af_sample_tokens."""
         self._check_generate()
-        sampling = bool(np.any(np.asarray(temperature) > 1e-4) or np.any(np.asarray(repetition_penalty) != 1.0))
+        temperature, top_k, top_p, min_p, repetition_penalty = map(
+            self._setting, (temperature, top_k, top_p, min_p, repetition_penalty))
+        sampling = bool(np.any(temperature > 1e-4) or np.any(repetition_penalty != 1.0))
         filters = self._filters(temperature, top_k, top_p, min_p, repetition_penalty) if sampling else None
         pr = torch.as_tensor(np.asarray(prompts, np.int32)).to(self.device)
         B, P = pr.shape
@@ -489,6 +491,12 @@ class AceEngine:
             return res, torch.stack(all_logits, 1).cpu().numpy()
         return res
 
+    @staticmethod
+    def _setting(v) -> np.ndarray:
+        """A sampling setting on the host, whatever holds it (a number, a list, an
+        array, a tensor of any type on any device)."""
+        return np.asarray(v.tolist() if isinstance(v, torch.Tensor) else v)
+
     def _filters(self, temperature, top_k, top_p, min_p, repetition_penalty):
         """sample_tokens' settings, those given per stream on the device; None
         where af_sample_rows (one setting for all, no min_p) will do."""
@@ -499,7 +507,7 @@ class AceEngine:
             if np.ndim(v) == 0:
                 out[name] = cuda_ops.c_int(v) if name == "top_k" else float(v)
                 continue
-            a = [cuda_ops.c_int(k) for k in v] if name == "top_k" else v
+            a = [cuda_ops.c_int(k) for k in np.ravel(v)] if name == "top_k" else v
             a = np.asarray(a, np.int32 if name == "top_k" else np.float32).reshape(-1)
             if a.size != self.batch:
                 raise ValueError(f"{name}: expected one value or {self.batch}, got {a.size}")

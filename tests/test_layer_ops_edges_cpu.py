@@ -183,3 +183,28 @@ def test_top_k_beyond_31_bits_cuts_nothing(monkeypatch):
         assert got == means
         got = AceEngine._filters(engine, 1.0, [k, 3], 1.0, 0.0, 1.0)["top_k"]
         assert got.dtype == torch.int32 and got.tolist() == [means, 3]
+
+
+def test_settings_of_any_kind_reach_generation():
+    """generate_batch's settings as it takes them before it looks at the device."""
+    from types import SimpleNamespace
+
+    from aceflow_b200.engine import AceEngine
+
+    class Reached(Exception):
+        pass
+
+    def stop(*settings):
+        raise Reached(settings)
+
+    engine = SimpleNamespace(_check_generate=lambda: None, _filters=stop, batch=2, vocab_size=5, device="cpu")
+    engine._setting = getattr(AceEngine, "_setting", None)
+    for t in (torch.tensor(0.5, dtype=torch.bfloat16), torch.tensor([0.5, 0.5]).bfloat16(), [0.5, 0.5], 0.5,
+              np.float32(0.5)):
+        with pytest.raises(Reached) as e:
+            AceEngine.generate_batch(engine, [[1], [1]], 1, temperature=t, top_k=torch.tensor([1, 2]), top_p=0.5)
+        t, k, p, m, r = (np.asarray(v) for v in e.value.args[0])
+        assert np.all(t == 0.5) and k.tolist() == [1, 2] and p == 0.5 and m == 0.0 and r == 1.0
+    got = AceEngine._filters(engine, np.asarray([[0.5], [1.0]]), np.asarray([[3], [2 ** 40]]), np.asarray(0.9), 0.1, 1.0)
+    assert got["temperature"].tolist() == [0.5, 1.0] and got["top_k"].tolist() == [3, 2 ** 31 - 1]
+    assert got["top_p"] == 0.9 and got["min_p"] == 0.1
