@@ -27,9 +27,13 @@
 //      equal logits, or a top_k above kList) every place is found by
 //      descending the digits of its key over histograms.
 //
-// Masses are whole numbers in units of 2^-44, w to 31 significant bits (less
-// than 2^-29 of itself off), in 64 bits: their sums do not depend on any
-// order, so a row's token is the same in every run and in every launch shape.
+// Masses are whole numbers in units of 2^-44, in 64 bits: their sums do not
+// depend on any order, so a row's token is the same in every run and in every
+// launch shape.  A mass has at most 31 significant bits and is off by at most
+// the larger of 2^-29 of itself and half a unit (a token below 2^-45 has none
+// and is never drawn): together no more than 2^-29 + vocab 2^-45 of a row, 1.2e-8
+// at the largest vocabulary.  What min-p keeps is decided on the logits in 64
+// bits, not on these masses, so that it holds for small weights too.
 //
 // Bound: one read of the logits would take 20.5 us for 256 rows of 131072 in
 // fp32; with top-p 0.95 over a broad row the call takes 183 us: in 7 waves of
@@ -781,7 +785,7 @@ struct Filters {
   bool cut_k, cut_p, cut_m;
   int top_k;
   double share;  // top_p
-  u64 floor_m;   // min_p
+  float lowest;  // the lowest logit that min_p keeps
   float u;
   __device__ __forceinline__ u64 over(u64 z) const { return (u64)floor(share * (double)z) + 1; }  // F > top_p Z
 };
@@ -803,7 +807,7 @@ __device__ __noinline__ void descend(Row row, Weigher weigh, Filters f, int32_t 
     u64 m = 0;
     d.row.each([&](float x, int) {
       const u64 w = d.mass(x);
-      m += w >= f.floor_m ? w : 0;
+      m += x >= f.lowest ? w : 0;
     });
     stop = shorter(d.find(true, d.row.total(m)), stop);
   }
@@ -944,7 +948,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
   f.cut_p = !(top_p >= 1.0f), f.cut_k = top_k > 0 && top_k < p.V, f.cut_m = min_p > 0.0f;
   f.top_k = top_k, f.u = u;
   f.share = f.cut_p ? (top_p > 0.f ? (double)top_p : 0.0) : 1.0;
-  f.floor_m = f.cut_m ? (u64)ceil(fmin((double)min_p, 1.0) * (double)kOne) : 1;
+  // w >= min_p where (l - max) c >= log2(min_p): the first fp32 value that is
+  f.lowest = kLowest;
+  if (f.cut_m) f.lowest = fmaxf(__double2float_ru(weigh.dtop + log2(fmin((double)min_p, 1.0)) / c), kLowest);
 
   unsigned m = kList + 1;
   int last = 0, in_front = 0;
@@ -965,8 +971,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
       m = row.bring(sm + Layout::list, [&](float x) { return weigh.lead(x) < end; });
   } else if (!f.cut_p && f.cut_m) {
     // 2. the tokens that min-p may keep
-    const float lowest = weigh.logit_below(44.0 - (double)log2f((float)f.floor_m));
-    m = row.bring(sm + Layout::list, [&](float x) { return x >= lowest; });
+    m = row.bring(sm + Layout::list, [&](float x) { return x >= f.lowest; });
   }
 
   if (m <= kList) {
@@ -981,8 +986,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
     if (f.cut_m) {
       u64 v = 0;
       for (int i = tid; i < (int)m; i += kThreads) {
-        const u64 w = weigh(Row::logit_of(head.entry(i)));
-        v += w >= f.floor_m ? w : 0;
+        const float x = Row::logit_of(head.entry(i));
+        v += x >= f.lowest ? weigh(x) : 0;
       }
       mass = min(mass, row.block_sum(v));
     }
@@ -1012,8 +1017,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_tokens_kernel(SampleParams
       for (int j = 0; j < 4; ++j)
         if (weigh.some(t[j])) {
           row.add_to_bin(b[j], q[j]);
-          const u64 w = (u64)q[j] << weigh.shift(b[j]);
-          if (f.cut_m) kept_m += w >= f.floor_m ? w : 0;
+          if (f.cut_m) kept_m += x[j] >= f.lowest ? (u64)q[j] << weigh.shift(b[j]) : 0;
         }
     }
     if (f.cut_m) kept_m = row.block_sum(kept_m);

@@ -4,6 +4,8 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import layer_ops_ref as L
+
 pytestmark = pytest.mark.gpu
 
 
@@ -28,3 +30,61 @@ def test_every_block_hears_of_a_maximum_in_every_other(dev, rows, V):
         tok, logp = cuda_ops.sample_tokens(lg, u, return_logprobs=True, **kw)
         assert torch.equal(tok.long(), at), kw
         assert torch.all(logp.abs() < 1e-6)  # what is left weighs V exp(-63) at most
+
+
+# A mass is off by at most the larger of 2^-29 of itself and 2^-45 of the largest
+# weight, so the mass of what is kept by 2^-29 + vocab 2^-45 of the row, and its
+# logarithm by the same; the result is rounded to fp32.
+def _mass_error(V):
+    return 2.0 ** -29 + V * 2.0 ** -45
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=200), dict(top_p=0.9999999), dict(temperature=0.5)])
+@pytest.mark.parametrize("V", [301, 4001, 131001])
+def test_min_p_among_small_weights(dev, V, kw):
+    """Half of a row's tokens 1e-5 above a min-p of 2^-30 and half as far below it:
+    a weight of 2^-30 is a whole number of units of 2^-44 to 3e-5 of itself only."""
+    from aceflow_b200 import cuda_ops
+
+    temp, min_p = kw.get("temperature", 1.0), float(np.float32(2.0 ** -30))
+    top = np.float32(temp * 20.794415)
+    edge = float(top) + temp * np.log(min_p)
+    row = np.full(V, edge + 1e-5 * temp, np.float32)
+    row[1::2] = edge - 1e-5 * temp
+    row[V // 2] = top
+    want, logp, margin = L.sample64(row, 0.5, temp, kw.get("top_k", 0), kw.get("top_p", 1.0), min_p)
+    above = int((row > edge).sum()) - 1
+    kept = min(above, kw.get("top_k", V) - 1)
+    if "top_p" not in kw:
+        assert abs(logp + np.log1p(kept * np.exp(1e-5) * min_p)) < 1e-3 * kept * min_p
+    tok, got = cuda_ops.sample_tokens(torch.from_numpy(row[None]).to(dev), torch.tensor([0.5], device=dev), min_p=min_p,
+                                      return_logprobs=True, **kw)
+    assert tok.item() == want == V // 2
+    assert abs(got.item() - logp) <= _mass_error(V) + 2.0 ** -24 * abs(logp)
+
+
+@pytest.mark.parametrize("min_p", [0.3, 1e-3, 1e-9, 3e-14])
+def test_min_p_of_any_size(dev, min_p):
+    """Weights spread over some octaves on either side of min-p; every row is
+    compared unless its own border is nearer than its masses' error."""
+    from aceflow_b200 import cuda_ops
+
+    rng = np.random.default_rng(3)
+    rows, V = 24, 20000
+    lg = (np.log(min_p) + 1.5 * rng.standard_normal((rows, V))).astype(np.float32)
+    lg[np.arange(rows), rng.integers(0, V, rows)] = 0.0
+    lg = np.minimum(lg, 0.0)
+    u = rng.random(rows).astype(np.float32)
+    tok, got = cuda_ops.sample_tokens(torch.from_numpy(lg).to(dev), torch.from_numpy(u).to(dev), min_p=min_p,
+                                      return_logprobs=True)
+    compared = 0
+    for r in range(rows):
+        want, logp, _ = L.sample64(lg[r], u[r], min_p=min_p)
+        w = np.exp(lg[r].astype(np.float64))
+        share = np.sort(w[w >= float(np.float32(min_p))])[::-1].cumsum()
+        if share.size > 1 and np.min(np.abs(share[:-1] / share[-1] - float(u[r]))) < _mass_error(V):
+            continue
+        compared += 1
+        assert tok[r].item() == want
+        assert abs(got[r].item() - logp) <= _mass_error(V) + 2.0 ** -23 * max(1.0, abs(logp))
+    assert compared >= 12
