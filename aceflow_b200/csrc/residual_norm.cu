@@ -206,10 +206,15 @@ struct Dot {
   __device__ __forceinline__ float sum() const { return x + y; }
 };
 
-// The sigmoid with the hardware's exponential and reciprocal: 2^-21 of itself
-// off (4 times that at |g| = 16), against 2^-9 of a bf16 result; with expf and
-// an IEEE division the forward spent half its instructions here.
-__device__ __forceinline__ float sigmoid(float g) {
+// The sigmoid.  Where x and h are bf16 (`fast`) by the hardware's exponential and
+// reciprocal: 2^-21 and |g| 2^-24 of itself off, against the 2^-9 of
+// the tensors (y, if asked for in fp32, and the weights' gradients carry it
+// too); expf and a division took 32768 x 2048 from 109 and 181 us (forward,
+// backward) to 135 and 234.  Where either is fp32, expf and a division all the
+// same: 16384 x 2048 fp32 122 and 185 us without, 118 and 190 with, 16384 x 1531 fp32
+// 100 and 194, 115 and 220.
+__device__ __forceinline__ float sigmoid(float g, bool fast) {
+  if (!fast) return 1.0f / (1.0f + expf(-g));
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
@@ -217,10 +222,11 @@ __device__ __forceinline__ float sigmoid(float g) {
 }
 // sw = swish(g), sg = sigmoid(g), o = o sw
 template <int VEC>
-__device__ __forceinline__ void gate_by(float (&o)[VEC], const float (&g)[VEC], float (&sw)[VEC], float (&sg)[VEC]) {
+__device__ __forceinline__ void gate_by(float (&o)[VEC], const float (&g)[VEC], float (&sw)[VEC], float (&sg)[VEC],
+                                        bool fast) {
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    sg[i] = sigmoid(g[i]);
+    sg[i] = sigmoid(g[i], fast);
     sw[i] = fmaxf(g[i], -3.0e38f);  // at -inf (where sg is 0) swish has the limit 0
   }
   mul(sw, sw, sg);
@@ -428,7 +434,7 @@ __global__ void __launch_bounds__(VEC == 8 && K == 1 ? 1024 : 512, VEC == 8 ? 1 
         if (p.g) {
           float v[VEC], sw[VEC], sg[VEC];
           k.get(gr[c], v, h16);
-          gate_by(z[c], v, sw, sg);
+          gate_by(z[c], v, sw, sg, x16 && h16);
         }
         if (kAhead) {
           mul(z[c], z[c], kept1[c]);
@@ -599,7 +605,7 @@ __global__ void __launch_bounds__(512, 1) seam_backward_kernel(SeamParams p) {
         }
         if (p.g) {
           k.get(raw[c].g, v, h16);
-          gate_by(q, v, sw[c], sg[c]);
+          gate_by(q, v, sw[c], sg[c], x16 && h16);
         }
         if (p.dz)
           k.get(raw[c].dz, e[c], x16);
@@ -690,7 +696,7 @@ struct SeamValues {
     if (p.g) {
       float g[VEC];
       k.get(r.g, g, h16);
-      gate_by(q, g, sw, sg);
+      gate_by(q, g, sw, sg, x16 && h16);
     }
     fill(e, 0.f), fill(zh, 0.f), fill(t, 0.f), fill(dy, 0.f);
     if (p.dz) k.get(r.dz, e, x16);
