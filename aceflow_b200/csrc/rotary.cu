@@ -9,12 +9,13 @@
 //
 // Angles.  position * inv_freq in fp32 is off by 2^-24 of the angle: 0.06 rad
 // at position 10^6.  The product is therefore formed in 64 bits, in turns,
-// reduced to [-1/2, 1/2] there, and only the remainder goes to sincospif
-// (2^-26 turns off, 1e-7 rad).
+// reduced to [-1/2, 1/2] there, and only the remainder goes to sincospif in
+// fp32; what its rounding leaves (2^-26 turns, 1e-7 rad at most) turns the result
+// on to first order, so that cos and sin are off by their own roundings alone.
 //
 // Bound: HBM, each value read once and written once: 84 us for q and k of 8 x
 // 4096 tokens (16 heads of 256, bf16, 0.54 GB), 0.97 of the measured copy rate.
-// An angle costs two 64-bit multiplies and a sincospif (about 40
+// An angle costs two 64-bit multiplies and a sincospif (about 45
 // instructions), so a thread keeps the angles of its few pairs in registers
 // for up to 16 heads, whose first loads are under way while they are formed.
 // bf16 values are taken apart and put together two at a time: one by one the
@@ -106,10 +107,12 @@ __device__ __forceinline__ double position_of(const RotaryParams &p, unsigned b,
 // cos and sin (times the scale) of pair i at this position.
 __device__ __forceinline__ float2 angle(const RotaryParams &p, double pos, int i) {
   const double turns = pos * ((double)p.inv_freq[i] * 0.15915494309189535);
-  const float r = (float)(turns - rint(turns));
+  const double left = turns - rint(turns);
+  const float r = (float)left, rest = (float)(left - (double)r) * 6.2831855f;
   float c, s;
   sincospif(2.0f * r, &s, &c);
-  return make_float2(c * p.scale, s * (p.inverse ? -p.scale : p.scale));
+  const float cr = fmaf(-s, rest, c), sr = fmaf(c, rest, s);
+  return make_float2(cr * p.scale, sr * (p.inverse ? -p.scale : p.scale));
 }
 
 constexpr int kThreads = 256;
