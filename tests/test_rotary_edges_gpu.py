@@ -51,3 +51,53 @@ def test_rounded_angles_add_no_error_on_average(dev):
     got = cuda_ops.rotary(x, f, 17).double().cpu().numpy()
     ref = L.rotary64(x.double().cpu().numpy(), f.cpu().numpy(), 17 + np.arange(2000))
     assert np.linalg.norm(got - ref) <= 0.8 * 2.0 ** -24 * np.linalg.norm(ref)
+
+
+def test_second_derivative(dev):
+    """|gradient|^2 as a penalty, against torch's own operations in 64 bits."""
+    from aceflow_b200 import cuda_ops
+
+    g = torch.Generator(device=dev).manual_seed(4)
+    x = torch.randn(2, 5, 3, 16, generator=g, device=dev, requires_grad=True)
+    f, _ = cuda_ops.rotary_frequencies(16, 100.0, device=dev)
+    y = cuda_ops.rotary_autograd(x, f, 3, layout="half", scale=1.5)
+    d, = torch.autograd.grad((y ** 3).sum(), x, create_graph=True)
+    got, = torch.autograd.grad(d.square().sum() + x.sum(), x)
+    xd = x.detach().double().requires_grad_()
+    th = (3 + torch.arange(5, device=dev))[:, None, None] * f.double()
+    a, b = xd.chunk(2, -1)
+    y = 1.5 * torch.cat((a * th.cos() - b * th.sin(), a * th.sin() + b * th.cos()), -1)
+    d, = torch.autograd.grad((y ** 3).sum(), xd, create_graph=True)
+    ref, = torch.autograd.grad(d.square().sum() + xd.sum(), xd)
+    # some ten roundings of a polynomial of degree 3 in y, each relative to its terms
+    assert float((got - ref).abs().max()) <= 40 * 2.0 ** -24 * float(ref.abs().max())
+
+
+def test_in_place_is_seen_by_autograd(dev):
+    from aceflow_b200 import cuda_ops
+
+    f, _ = cuda_ops.rotary_frequencies(8, device=dev)
+    x = torch.randn(1, 3, 2, 8, device=dev)
+    w = torch.ones_like(x, requires_grad=True)
+    loss = (w * x).sum()
+    cuda_ops.rotary(x[:, :, :1], f, inplace=True)  # a view of it
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_captured_steps_turn_by_new_frequencies(dev):
+    import aceflow_b200 as af
+
+    with torch.inference_mode():
+        rot = af.nn.Rotary(64)
+    x = torch.randn(2, 3, 4, 64, device=dev)
+    rot.turn(x, 7)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = rot.turn(x, 7)
+    for change in (1.0, 0.25, 3.0):
+        rot.inv_freq = rot.inv_freq * change
+        want = rot.turn(x, 7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)

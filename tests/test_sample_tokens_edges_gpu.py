@@ -88,3 +88,54 @@ def test_min_p_of_any_size(dev, min_p):
         assert tok[r].item() == want
         assert abs(got[r].item() - logp) <= _mass_error(V) + 2.0 ** -23 * max(1.0, abs(logp))
     assert compared >= 12
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=1), dict(top_k=50), dict(top_p=0.95), dict(min_p=0.02),
+                                dict(temperature=0.7, top_k=40, top_p=0.9), dict(temperature=30.0),
+                                dict(temperature=0.01), dict(top_k=20000, top_p=0.999, min_p=1e-6)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_row_under_each_filter(dev, kw, dtype):
+    """Twenty draws of one row alone.  Both sides of a share are off by the masses'
+    error at most, so a share by twice that (6e-9 here): a draw whose deciding
+    border is nearer is left out, and so may be two in twenty at most."""
+    from aceflow_b200 import cuda_ops
+
+    rng = np.random.default_rng(len(str(kw)))
+    lg = torch.from_numpy(3.0 * rng.standard_normal((1, 32000)).astype(np.float32)).to(dev).to(dtype)
+    row = lg.float().cpu().numpy()[0]
+    args = [kw.get(k, v) for k, v in (("temperature", 1.0), ("top_k", 0), ("top_p", 1.0), ("min_p", 0.0))]
+    compared = 0
+    for u in rng.random(20).astype(np.float32):
+        tok, logp = cuda_ops.sample_tokens(lg, torch.tensor([u], device=dev), return_logprobs=True, **kw)
+        want, ref, _ = L.sample64(row, u, *args)
+        if _share_margin(row, u, *args) < 2 * _mass_error(32000):
+            continue
+        compared += 1
+        assert tok.item() == want and abs(logp.item() - ref) <= 2e-7 * max(1.0, abs(ref))
+    assert compared >= 18
+
+
+def _share_margin(row, u, temperature, top_k, top_p, min_p):
+    """How far, in shares of the mass that decides, u's draw and the crossing of
+    top_p lie from the borders next to them (min-p is decided without sums)."""
+    x = np.sort(row.astype(np.float64))[::-1]
+    w = np.exp((x[:top_k] if top_k else x) - x[0]) if temperature == 1.0 else np.exp(
+        ((x[:top_k] if top_k else x) - x[0]) / float(np.float32(temperature)))
+    run, keep, margin = np.cumsum(w), w.size, 1.0
+    if top_p < 1.0:
+        p = float(np.float32(top_p))
+        keep = 1 + int(np.searchsorted(run, p * run[-1], side="right"))
+        margin = float(np.min(np.abs(run / run[-1] - p)))
+    keep = min(keep, int((w >= float(np.float32(min_p))).sum()))
+    return min(margin, float(np.min(np.abs(run[:keep - 1] / run[keep - 1] - float(u)), initial=1.0)))
+
+
+def test_a_top_k_beyond_31_bits(dev):
+    from aceflow_b200 import cuda_ops
+
+    lg = 2.5 * torch.randn(30, 9000, generator=torch.Generator(device=dev).manual_seed(1), device=dev)
+    u = torch.rand(30, generator=torch.Generator(device=dev).manual_seed(2), device=dev)
+    want = cuda_ops.sample_tokens(lg, u)
+    assert torch.equal(cuda_ops.sample_tokens(lg, u, top_k=2 ** 32 + 1), want)
+    assert torch.equal(cuda_ops.sample_tokens(lg, u, top_k=-2 ** 32 + 1), want)
+    assert not torch.equal(cuda_ops.sample_tokens(lg, u, top_k=1), want)
