@@ -29,10 +29,11 @@
 // partial row per group and are added in a fixed order by a second kernel: no
 // atomics, the same bits every run.
 // Measured with gate and all weights (floor: the tensors' bytes at 6547 GB/s):
-//   32768 x 2048 bf16   forward 110 us (0.93 of it), backward 182 (0.90)
-//   16384 x 2048 fp32            122 (0.84),                  186 (0.88)
-//    4096 x 8192 bf16             65 (0.79),                  139 (0.59)
-//   16384 x 1531 bf16             72 (0.53),                  133 (0.46)
+//   32768 x 2048 bf16   forward 110 us (0.93 of it), backward 181 (0.91)
+//   16384 x 2048 fp32            118 (0.87),                  190 (0.86)
+//    4096 x 8192 bf16             64 (0.80),                  134 (0.61)
+//   16384 x 1531 bf16             72 (0.53),                  135 (0.45)
+//   16384 x 1531 fp32            115 (0.67),                  220 (0.56)
 #include "common.cuh"
 
 #include <algorithm>
@@ -207,7 +208,7 @@ struct Dot {
 };
 
 // The sigmoid.  Where x and h are bf16 (`fast`) by the hardware's exponential and
-// reciprocal: 2^-21 and |g| 2^-24 of itself off, against the 2^-9 of
+// reciprocal: 2^-21 and |g| 2^-24 of itself off, against the 2^-8 of
 // the tensors (y, if asked for in fp32, and the weights' gradients carry it
 // too); expf and a division took 32768 x 2048 from 109 and 181 us (forward,
 // backward) to 135 and 234.  Where either is fp32, expf and a division all the
@@ -943,9 +944,9 @@ constexpr int kMaxWidth = 16384;
 // suffice, few values a thread, so that much is under way.  Vectors where the
 // rows' addresses allow them (vec 8): in rows of any width, `shift` then says
 // that they start anywhere in 16 bytes and a thread's vectors may start 7 values
-// in front of the row.  16384 x 1531 bf16: forward 72 us, backward 133, against
+// in front of the row.  16384 x 1531 bf16: forward 72 us, backward 135, against
 // 181 and 241 with single values.  Backward rows wider than 4096 (k 2; 4, where x
-// and h are bf16, `narrow`) keep their raw values: 4096 x 8192 bf16 139 us,
+// and h are bf16, `narrow`) keep their raw values: 4096 x 8192 bf16 134 us,
 // against 323 with a second reading of the row (k 0), which remains for what no
 // thread can hold.
 struct Shape {

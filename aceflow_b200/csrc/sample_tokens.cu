@@ -36,12 +36,12 @@
 // bits, not on these masses, so that it holds for small weights too.
 //
 // Bound: one read of the logits would take 20.5 us for 256 rows of 131072 in
-// fp32; with top-p 0.95 over a broad row the call takes 183 us: in 7 waves of
+// fp32; with top-p 0.95 over a broad row the call takes 184 us: in 7 waves of
 // clusters, each a chain of about 48000 cycles (8300 to load, 9300 for the
 // masses, the rest barriers, scans and the first CTA's search).  Summing Z in
 // a pass of its own, with a second one for the bins and a collection for each
 // place, took 365 us.  Few rows are bound by the chain alone: 12.4 us for one
-// row of 32000 with top-k 40, 23 us for 64 such rows with mixed settings.
+// row of 32000 with top-k 40, 24 us for 64 such rows with mixed settings.
 // Step 5 costs a row of 131072 0.3 ms (all logits equal) to 0.5 ms (all within a
 // few bins).
 #include "common.cuh"

@@ -260,7 +260,8 @@ class MultiScaleRetention(Module):
     def _prefill_turned(self, xb, p: dict, state, out_dtype, want_state: bool, chunk: int, position):
         """The tensor-core prefill with the rotation between the QKV product
         and the chunkwise kernel (which read and write the same packed bf16
-        qkv); bf16 q and k are rounded once more by it."""
+        qkv).  That rounds q and k to bf16 twice, by 2^-8 each: the kernel takes
+        bf16 operands, and an fp32 q and k would cost the prompt twice their bytes."""
         import torch
 
         from .. import cuda_ops

@@ -484,8 +484,10 @@ int af_sample_rows(af_ctx *ctx, const float *logits, int rows, int vocab, const 
  * af_sample_rows' filters in its order (repetition penalty, temperature,
  * top-k, top-p, draw), with min-p in front of the draw: of the tokens that
  * the other filters leave, those at least min_p times as likely as the
- * likeliest.  The sums that decide a token are exact (64-bit whole numbers),
- * so a row's token does not depend on the batch around it.
+ * likeliest (decided on the logits in 64 bits).  The weights that are summed are
+ * whole units of 2^-44 of the largest, off by 2^-29 of themselves or half a unit;
+ * their sums are exact, so a row's token does not depend on the batch around
+ * it.  A token below 2^-45 of the likeliest is never drawn.
  *   logits  [rows][vocab] fp32 or bf16 (logits_bf16), rows row_stride elements
  *           apart.  -inf marks a token that may not be drawn, NaN counts as
  *           -inf; among +inf only these are drawn.  Not modified.
