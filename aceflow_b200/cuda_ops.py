@@ -282,7 +282,8 @@ class _GradientsOnly(torch.autograd.Function):
     @staticmethod
     def forward(ctx, name, count, *grads_and_sources):
         ctx.name = name
-        return tuple(g.view_as(g) for g in grads_and_sources[:count])
+        ctx.mark_dirty(*grads_and_sources[:count])  # the same tensors: nobody else has them yet
+        return grads_and_sources[:count]
 
     @staticmethod
     def backward(ctx, *_):

@@ -208,3 +208,20 @@ def test_settings_of_any_kind_reach_generation():
     got = AceEngine._filters(engine, np.asarray([[0.5], [1.0]]), np.asarray([[3], [2 ** 40]]), np.asarray(0.9), 0.1, 1.0)
     assert got["temperature"].tolist() == [0.5, 1.0] and got["top_k"].tolist() == [3, 2 ** 31 - 1]
     assert got["top_p"] == 0.9 and got["min_p"] == 0.1
+
+
+def test_gradients_with_a_graph_may_be_changed_in_place(monkeypatch):
+    monkeypatch.setattr(cuda_ops, "residual_norm", _seam)
+    monkeypatch.setattr(cuda_ops, "residual_norm_backward", _seam_grads)
+    x, h, w = (torch.ones(3, 4, requires_grad=True), torch.ones(3, 4, requires_grad=True),
+               torch.ones(4, requires_grad=True))
+    z, y = cuda_ops.residual_norm_autograd(x, h, pre_w=w)
+    for g in torch.autograd.grad((z * y).sum(), (x, h, w), create_graph=True):
+        assert g.requires_grad
+        g.mul_(2.0)
+        assert torch.all(g == 2)
+    z, y = cuda_ops.residual_norm_autograd(x, h, pre_w=w)
+    (z * y).sum().backward(create_graph=True)
+    opt = torch.optim.SGD([x, h, w], lr=0.1)
+    opt.zero_grad(set_to_none=False)
+    assert torch.all(x.grad == 0) and not x.grad.requires_grad
