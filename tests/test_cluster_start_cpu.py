@@ -1,6 +1,6 @@
 """Distributed shared memory may be touched only once every CTA of the cluster
-runs.  What that takes is visible in a kernel's source alone: no output shows a
-write that came too early on a box where it did not matter."""
+runs.  What that takes is visible in a kernel's source alone: a write that comes
+too early need not show in any output."""
 import os
 import re
 
